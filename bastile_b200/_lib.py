@@ -89,6 +89,12 @@ SIGNATURES = {
                               c_float, c_float, c_int64, c_int, c_int, c_void_p]),
     "bt_adamw_master_step": (c_int, [c_void_p] * 5 + [c_int64] + [c_float] * 5 + [c_int64, c_float, c_int, c_int,
                                      c_void_p]),
+    "bt_attn_plan_words": (c_int64, [c_int64]),
+    "bt_attn_plan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "bt_attn_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 5 + [POINTER(c_int64)] * 4 +
+                    [c_float, c_int, c_void_p, c_void_p]),
+    "bt_attn_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
+                    [c_float, c_int, c_void_p, c_void_p]),
     "bt_scale_cast": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),
 }
 
@@ -273,7 +279,7 @@ class timed:
         return False
 
 
-STATUS_WAIT_MASK, STATUS_BAD_LABEL = 0x0F, 0x10  # BT_STATUS_* of include/bastile_b200.h
+STATUS_WAIT_MASK, STATUS_BAD_LABEL, STATUS_BAD_SEQUENCES = 0x0F, 0x10, 0x20  # BT_STATUS_* of include/bastile_b200.h
 
 
 def _describe_status(v: int) -> str:
@@ -282,6 +288,8 @@ def _describe_status(v: int) -> str:
         parts.append(f"a bounded device-side wait ran out (bits {v & STATUS_WAIT_MASK:#x}): results are invalid")
     if v & STATUS_BAD_LABEL:
         parts.append("fused_linear_cross_entropy got a label that is neither ignore_index nor a vocabulary row")
+    if v & STATUS_BAD_SEQUENCES:
+        parts.append("sequence offsets do not start at 0, fall, or run past the packed tokens")
     return "; ".join(parts) or f"status {v:#x}"
 
 

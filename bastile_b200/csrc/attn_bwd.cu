@@ -1,0 +1,698 @@
+// Causal attention over packed sequences, backward.  With P = exp(scale S - lse), D_i = dO_i . O_i:
+//
+//   dV_j = sum_i P_ij dO_i     dS_ij = P_ij (dO_i . V_j - D_i)
+//   dK_j = scale sum_i dS_ij Q_i     dQ_i = scale sum_j dS_ij K_j
+//
+// Two kernels, each with its sums in tensor memory from the first tile to the last and one store at
+// the end: dK and dV per key tile (query rows of all heads of the group are rows of the same tiles),
+// dQ per query tile.  S and dO V^T are computed by both - seven products where one kernel could do
+// with five - but that one would have to add dQ tiles into memory by atomics, whose order changes
+// the result; here every launch gives the same bits.
+#include "attn_sm100.cuh"
+
+namespace bt {
+namespace attn {
+namespace {
+
+constexpr int kBwdThreads = 384;
+
+// ------------------------------------------------------------------ D = dO . O
+// Half a warp per (token, head) row, 16 bytes of each tensor per lane.
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* __restrict__ delta, int64_t rows,
+                  int heads, int64_t total, int d, int64_t o_st, int64_t o_sh, int64_t g_st, int64_t g_sh) {
+  grid_dependency_wait();
+  const int sub = threadIdx.x & 15;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 16;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16; r0 < rows; r0 += step) {
+    const int64_t r = r0 + (threadIdx.x >> 4);
+    float acc = 0.f;
+    const int64_t tok = r / heads;
+    const int head = static_cast<int>(r - tok * heads);
+    if (r < rows && sub * 8 < d) {
+      float a[8], b[8];
+      Cvt<T>::unpack(ld_stream_v4(out + tok * o_st + head * o_sh + sub * 8), a);
+      Cvt<T>::unpack(ld_global_v4(dout + tok * g_st + head * g_sh + sub * 8), b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc = fmaf(a[e], b[e], acc);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (r < rows && sub == 0) delta[head * total + tok] = acc;
+  }
+}
+
+template <int DT>
+struct BwdGeo {
+  static constexpr int kTileBytes = (DT / 64) * kBoxBytes;
+  static constexpr int kVecBytes = 2 * 2 * 128 * 4;  // two stages of -lse and D of a query tile
+  static constexpr int kSmem = 6 * kTileBytes + kVecBytes + 1024 + 1024;
+};
+
+template <typename T>
+__host__ __device__ constexpr uint32_t mma_fmt() {
+  return std::is_same<T, __half>::value ? 0u : 1u;
+}
+
+// One tile through the ring slot `dst`: rows from `valid` on are cleared before the consumers see it.
+// Called by the whole load warp; returns false when a wait ran out.
+template <int DT>
+__device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, int head, int token, int valid,
+                                          uint64_t* full, uint64_t* empty, uint32_t empty_parity, uint64_t* fix,
+                                          uint32_t* fix_phase, int lane, volatile int* cta_abort, int32_t* status) {
+  bool ok = true;
+  const bool ragged = valid < kTile;
+  if (lane == 0) {
+    ok = ptx::mbar_wait(empty, empty_parity, cta_abort, status, ST_LOAD);
+    if (ok) {
+      uint64_t* bar = ragged ? fix : full;
+      ptx::mbar_arrive_expect_tx(bar, (DT / 64) * kBoxBytes);
+      load_tile<DT>(dst, tm, head, token, bar);
+      if (ragged) ok = ptx::mbar_wait(fix, *fix_phase, cta_abort, status, ST_LOAD);
+    }
+  }
+  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  if (ok && ragged) {
+    *fix_phase ^= 1u;
+    zero_rows<DT>(dst, valid, lane);
+    if (lane == 0) ptx::mbar_arrive(full);
+  }
+  return ok;
+}
+
+__device__ __forceinline__ void drain_copies() {
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
+// 32 accumulator columns of one row, scaled and stored.
+template <typename T>
+__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, int col0, int d, float scale, bool row_ok) {
+  float v[32];
+  tmem_ld32(taddr, v);
+  tmem_wait_ld();
+  if (!row_ok) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[g * 8 + 2 * e] * scale, v[g * 8 + 2 * e + 1] * scale);
+    if (col0 + g * 8 < d) st_global_v4(dst + col0 + g * 8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
+// ----------------------------------------------------------------- dK and dV
+// One CTA per (128 keys, key/value head).  Warps 0..7: one key row and half of the 128 query columns
+// per thread; warp 8 issues, warp 9 loads.  Transposed scores, so that P^T and dS^T are the
+// tensor-memory operands of the two sums:
+//   S^T = K Q_i^T -> P^T (16 bits, in place) ; dV += P^T dO_i ; dP^T = V dO_i^T -> dS^T ; dK += dS^T Q_i
+// A half's 16-bit P^T lies in the first 32 of the 64 columns it read, so no warp overwrites another's.
+template <typename T, int DT>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const Params p) {
+  using G = BwdGeo<DT>;
+  constexpr int TB = G::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sK = ptx::smem_u32(smem), sV = sK + TB, sQ = sK + 2 * TB, sG = sK + 4 * TB;
+  float* vec = reinterpret_cast<float*>(smem + 6 * TB);  // [stage][-lse | D][128]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + 6 * TB + G::kVecBytes);
+  uint64_t* v_full = k_full + 1;
+  uint64_t* q_full = v_full + 1;    // [2]
+  uint64_t* q_empty = q_full + 2;   // [2]
+  uint64_t* g_full = q_empty + 2;   // [2]
+  uint64_t* g_empty = g_full + 2;   // [2]
+  uint64_t* vec_full = g_empty + 2; // [2]
+  uint64_t* s_full = vec_full + 2;
+  uint64_t* p_ready = s_full + 1;
+  uint64_t* dp_full = p_ready + 1;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* done = ds_ready + 1;
+  uint64_t* fix = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(k_full, 1);
+    ptx::mbar_init(v_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&q_empty[i], 1);
+      ptx::mbar_init(&g_full[i], 1);
+      ptx::mbar_init(&g_empty[i], 1);
+      ptx::mbar_init(&vec_full[i], 32);
+    }
+    ptx::mbar_init(s_full, 1);
+    ptx::mbar_init(p_ready, 256);
+    ptx::mbar_init(dp_full, 1);
+    ptx::mbar_init(ds_ready, 256);
+    ptx::mbar_init(done, 1);
+    ptx::mbar_init(fix, 1);
+    *cta_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmQ);
+    ptx::prefetch_tensormap(&tmK);
+    ptx::prefetch_tensormap(&tmV);
+    ptx::prefetch_tensormap(&tmG);
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish_alloc_permit();
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  const int hk = static_cast<int>(blockIdx.x) % p.hk;
+  Item it{};
+  const bool live = plan_item(p.plan, p.gran, static_cast<int>(blockIdx.x) / p.hk, lane, &it);
+  const bool behind = live && it.entry == p.plan.n - 1;
+  const int kv0 = live ? it.tile * kTile : 0;
+  const int i0 = kv0 / p.tq;                                     // first query tile that sees a key of this one
+  const int per = live ? (it.len + p.tq - 1) / p.tq - i0 : 0;    // query tiles of one packed group
+  const int n = (live && !behind) ? per * p.nsub : 0;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 9 && n > 0) {
+      // ---------------------------------------------------------------- loads
+      if (lane == 0) {
+        ptx::mbar_arrive_expect_tx(k_full, TB);
+        load_tile<DT>(sK, &tmK, hk, it.start + kv0, k_full);
+        ptx::mbar_arrive_expect_tx(v_full, TB);
+        load_tile<DT>(sV, &tmV, hk, it.start + kv0, v_full);
+      }
+      uint32_t fix_phase = 0;
+      bool ok = true;
+      int sub = 0, i = i0;
+      for (int x = 0; ok && x < n; ++x) {
+        const int st = x & 1;
+        const uint32_t par = ((x >> 1) & 1) ^ 1u;
+        const int head = (hk * p.nsub + sub) * p.gp;
+        const int tok0 = i * p.tq;
+        const int valid = min(p.tq, it.len - tok0) << p.gp_shift;
+        // rows of Q and dO behind the sequence are cleared: they meet P = dS = 0, as the rest of a
+        // product they only have to be finite
+        ok = ring_load<DT>(sQ + st * TB, &tmQ, head, it.start + tok0, valid, &q_full[st], &q_empty[st], par, fix,
+                           &fix_phase, lane, cta_abort, p.status);
+        if (!ok) break;
+        // q_empty also says that the math warps are done with this stage of the row vectors
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = e * 32 + lane;
+          const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + it.start + tok0 + (r >> p.gp_shift);
+          const bool in = r < valid;
+          vec[st * 256 + r] = in ? -__ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
+          vec[st * 256 + 128 + r] = in ? __ldg(p.delta + at) : 0.f;
+        }
+        ptx::mbar_arrive(&vec_full[st]);
+        ok = ring_load<DT>(sG + st * TB, &tmG, head, it.start + tok0, valid, &g_full[st], &g_empty[st], par, fix,
+                           &fix_phase, lane, cta_abort, p.status);
+        if (++i == i0 + per) {
+          i = i0;
+          ++sub;
+        }
+      }
+      if (!ok || *cta_abort != 0) drain_copies();
+    } else if (warp == 8 && n > 0 && lane == 0) {
+      // ----------------------------------------------------------- MMA issuer
+      constexpr uint32_t id_s = ptx::make_idesc(mma_fmt<T>(), false, false, 128, 128);
+      constexpr uint32_t id_o = ptx::make_idesc(mma_fmt<T>(), false, true, 128, DT);
+      const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DT;
+      bool ok = ptx::mbar_wait(k_full, 0, cta_abort, p.status, ST_ISSUE) &&
+                ptx::mbar_wait(&q_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        mma_abt<DT>(tS, sK, sQ, id_s);
+        ptx::umma_commit(s_full);
+        ok = ptx::mbar_wait(v_full, 0, cta_abort, p.status, ST_ISSUE) &&
+             ptx::mbar_wait(&g_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      }
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        mma_abt<DT>(tP, sV, sG, id_s);
+        ptx::umma_commit(dp_full);
+      }
+      for (int x = 0; ok && x < n; ++x) {
+        const int st = x & 1, nst = st ^ 1;
+        const uint32_t npar = ((x + 1) >> 1) & 1;
+        const bool more = x + 1 < n;
+        ok = ptx::mbar_wait(p_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        mma_pb<DT>(tV, tS, tS + 64, sG + st * TB, id_o, x > 0);
+        ptx::umma_commit(&g_empty[st]);
+        if (more) {
+          ok = ptx::mbar_wait(&q_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tS, sK, sQ + nst * TB, id_s);
+          ptx::umma_commit(s_full);
+        }
+        ok = ptx::mbar_wait(ds_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        mma_pb<DT>(tK, tP, tP + 64, sQ + st * TB, id_o, x > 0);
+        ptx::umma_commit(&q_empty[st]);
+        if (more) {
+          ok = ptx::mbar_wait(&g_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tP, sV, sG + nst * TB, id_s);
+          ptx::umma_commit(dp_full);
+        }
+      }
+      if (ok) ptx::umma_commit(done);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // --------------------------------------------------------- P^T, dS^T, stores
+    const int half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int kv = kv0 + row;
+    if (behind && kv < it.len) {
+      const int64_t token = static_cast<int64_t>(it.start) + kv;
+      T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
+      T* dv = static_cast<T*>(p.dv.ptr) + token * p.dv.st + hk * p.dv.sh;
+      for (int c = half * 8; c < p.d; c += 16) {
+        st_global_v4(dk + c, make_uint4(0, 0, 0, 0));
+        st_global_v4(dv + c, make_uint4(0, 0, 0, 0));
+      }
+    }
+    if (n > 0) {
+      const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lane_base + half * 64, tp = ts + 128;
+      const f32x2 c2 = pair(p.scale_log2, p.scale_log2);
+      bool ok = true;
+      int i = i0;
+      for (int x = 0; x < n; ++x) {
+        const int st = x & 1;
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&vec_full[st], (x >> 1) & 1, cta_abort, p.status, ST_MATH) &&
+                                         ptx::mbar_wait(s_full, x & 1, cta_abort, p.status, ST_MATH));
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        const float4* nl = reinterpret_cast<const float4*>(vec + st * 256 + half * 64);
+        const float4* dl = nl + 32;
+        float s[64];
+        tmem_ld32(ts, s);
+        tmem_ld32(ts + 32, s + 32);
+        tmem_wait_ld();
+        const int tok0 = i * p.tq;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float4 l4 = nl[e];
+          const f32x2 a = fma2(pair(s[4 * e], s[4 * e + 1]), c2, pair(l4.x, l4.y));
+          const f32x2 b = fma2(pair(s[4 * e + 2], s[4 * e + 3]), c2, pair(l4.z, l4.w));
+          s[4 * e] = ex2(lo_of(a));
+          s[4 * e + 1] = ex2(hi_of(a));
+          s[4 * e + 2] = ex2(lo_of(b));
+          s[4 * e + 3] = ex2(hi_of(b));
+        }
+        if (tok0 < kv0 + kTile - 1) {  // the diagonal: query rows before this key
+          const int lo = (max(kv - tok0, 0) << p.gp_shift) - half * 64;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) s[e] = e >= lo ? s[e] : 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(s[g * 32 + 2 * e], s[g * 32 + 2 * e + 1]);
+          tmem_st16(ts + g * 16, pk);
+        }
+        tmem_wait_st();
+        ptx::tcgen05_fence_before_sync();
+        ptx::mbar_arrive(p_ready);
+
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(dp_full, x & 1, cta_abort, p.status, ST_MATH));
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        float dp[64];
+        tmem_ld32(tp, dp);
+        tmem_ld32(tp + 32, dp + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 d4 = dl[g * 8 + e];
+            const int b = g * 32 + 4 * e;
+            const f32x2 u = mul2(pair(s[b], s[b + 1]), add2(pair(dp[b], dp[b + 1]), neg2(pair(d4.x, d4.y))));
+            const f32x2 v = mul2(pair(s[b + 2], s[b + 3]), add2(pair(dp[b + 2], dp[b + 3]), neg2(pair(d4.z, d4.w))));
+            pk[2 * e] = pack2<T>(lo_of(u), hi_of(u));
+            pk[2 * e + 1] = pack2<T>(lo_of(v), hi_of(v));
+          }
+          tmem_st16(tp + g * 16, pk);
+        }
+        tmem_wait_st();
+        ptx::tcgen05_fence_before_sync();
+        ptx::mbar_arrive(ds_ready);
+        if (++i == i0 + per) i = i0;
+      }
+      if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, cta_abort, p.status, ST_MATH));
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        const bool row_ok = kv < it.len;
+        const int64_t token = static_cast<int64_t>(it.start) + kv;
+        T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
+        T* dv = static_cast<T*>(p.dv.ptr) + token * p.dv.st + hk * p.dv.sh;
+#pragma unroll 1
+        for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
+          store_cols<T>(tmem + lane_base + 256 + c, dv, c, p.d, 1.0f, row_ok);
+          store_cols<T>(tmem + lane_base + 256 + DT + c, dk, c, p.d, p.scale, row_ok);
+        }
+      }
+    }
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------ dQ
+// One CTA per (query tile of 128 packed rows, key/value head).  Warps 0..7: one query row and half of
+// the 128 key columns per thread.  S is double-buffered in tensor memory (its buffer then holds the
+// 16-bit dS), so the tensor pipe computes S_{j+1} and dP_{j+1} while the math warps work on tile j:
+//   S = Q K_j^T ; dP = dO V_j^T ; dS = P (dP - D) ; dQ += dS K_j
+template <typename T, int DT>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const Params p) {
+  using G = BwdGeo<DT>;
+  constexpr int TB = G::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sQ = ptx::smem_u32(smem), sG = sQ + TB, sK = sQ + 2 * TB, sV = sQ + 4 * TB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + 6 * TB);
+  uint64_t* g_full = q_full + 1;
+  uint64_t* k_full = g_full + 1;   // [2]
+  uint64_t* k_empty = k_full + 2;  // [2]
+  uint64_t* v_full = k_empty + 2;  // [2]
+  uint64_t* v_empty = v_full + 2;  // [2]
+  uint64_t* s_full = v_empty + 2;  // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* done = ds_ready + 1;
+  uint64_t* fix = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(q_full, 1);
+    ptx::mbar_init(g_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&k_full[i], 1);
+      ptx::mbar_init(&k_empty[i], 1);
+      ptx::mbar_init(&v_full[i], 1);
+      ptx::mbar_init(&v_empty[i], 1);
+      ptx::mbar_init(&s_full[i], 1);
+    }
+    ptx::mbar_init(dp_full, 1);
+    ptx::mbar_init(ds_ready, 256);
+    ptx::mbar_init(done, 1);
+    ptx::mbar_init(fix, 1);
+    *cta_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmQ);
+    ptx::prefetch_tensormap(&tmK);
+    ptx::prefetch_tensormap(&tmV);
+    ptx::prefetch_tensormap(&tmG);
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish_alloc_permit();
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  const int groups = p.hk * p.nsub;
+  const int hs = static_cast<int>(blockIdx.x) % groups;
+  Item it{};
+  const bool live = plan_item(p.plan, p.gran, static_cast<int>(blockIdx.x) / groups, lane, &it);
+  const bool behind = live && it.entry == p.plan.n - 1;
+  const int first = live ? (behind ? it.tile : (it.len + p.tq - 1) / p.tq - 1 - it.tile) * p.tq : 0;
+  const int n = (live && !behind) ? (min(it.len, first + p.tq) + kTile - 1) / kTile : 0;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 9 && n > 0) {
+      // ---------------------------------------------------------------- loads
+      if (lane == 0) {
+        ptx::mbar_arrive_expect_tx(q_full, TB);
+        load_tile<DT>(sQ, &tmQ, hs * p.gp, it.start + first, q_full);
+        ptx::mbar_arrive_expect_tx(g_full, TB);
+        load_tile<DT>(sG, &tmG, hs * p.gp, it.start + first, g_full);
+      }
+      uint32_t fix_phase = 0;
+      bool ok = true;
+      for (int j = 0; ok && j < n; ++j) {
+        const int st = j & 1;
+        const uint32_t par = ((j >> 1) & 1) ^ 1u;
+        // K rows behind the sequence meet dS = 0 and have to be finite; V's only give masked columns
+        ok = ring_load<DT>(sK + st * TB, &tmK, hs / p.nsub, it.start + j * kTile, min(kTile, it.len - j * kTile),
+                           &k_full[st], &k_empty[st], par, fix, &fix_phase, lane, cta_abort, p.status) &&
+             ring_load<DT>(sV + st * TB, &tmV, hs / p.nsub, it.start + j * kTile, kTile, &v_full[st], &v_empty[st],
+                           par, fix, &fix_phase, lane, cta_abort, p.status);
+      }
+      if (!ok || *cta_abort != 0) drain_copies();
+    } else if (warp == 8 && n > 0 && lane == 0) {
+      // ----------------------------------------------------------- MMA issuer
+      constexpr uint32_t id_s = ptx::make_idesc(mma_fmt<T>(), false, false, 128, 128);
+      constexpr uint32_t id_o = ptx::make_idesc(mma_fmt<T>(), false, true, 128, DT);
+      const uint32_t tP = tmem + 256, tQ = tmem + 384;
+      bool ok = ptx::mbar_wait(q_full, 0, cta_abort, p.status, ST_ISSUE) &&
+                ptx::mbar_wait(&k_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        mma_abt<DT>(tmem, sQ, sK, id_s);
+        ptx::umma_commit(&s_full[0]);
+        ok = ptx::mbar_wait(g_full, 0, cta_abort, p.status, ST_ISSUE) &&
+             ptx::mbar_wait(&v_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      }
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        mma_abt<DT>(tP, sG, sV, id_s);
+        ptx::umma_commit(dp_full);
+        ptx::umma_commit(&v_empty[0]);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int st = j & 1, nst = st ^ 1;
+        const uint32_t npar = ((j + 1) >> 1) & 1;
+        const bool more = j + 1 < n;
+        if (more) {
+          ok = ptx::mbar_wait(&k_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tmem + nst * 128, sQ, sK + nst * TB, id_s);
+          ptx::umma_commit(&s_full[nst]);
+        }
+        ok = ptx::mbar_wait(ds_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        mma_pb<DT>(tQ, tmem + st * 128, tmem + st * 128 + 64, sK + st * TB, id_o, j > 0);
+        ptx::umma_commit(&k_empty[st]);
+        if (more) {
+          ok = ptx::mbar_wait(&v_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tP, sG, sV + nst * TB, id_s);
+          ptx::umma_commit(dp_full);
+          ptx::umma_commit(&v_empty[nst]);
+        }
+      }
+      if (ok) ptx::umma_commit(done);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---------------------------------------------------------------- dS, store
+    const int half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int tok = first + (row >> p.gp_shift);
+    const int head = hs * p.gp + (row & (p.gp - 1));
+    const int64_t token = static_cast<int64_t>(it.start) + tok;
+    const bool row_ok = live && tok < it.len;
+    T* dq = static_cast<T*>(p.dq.ptr) + token * p.dq.st + head * p.dq.sh;
+    if (behind && row_ok)
+      for (int c = half * 8; c < p.d; c += 16) st_global_v4(dq + c, make_uint4(0, 0, 0, 0));
+    if (n > 0) {
+      const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t ts0 = tmem + lane_base + half * 64, tp = ts0 + 256;
+      const int64_t at = static_cast<int64_t>(head) * p.total + token;
+      const float nl = row_ok ? -p.lse2[at] : -INFINITY;
+      const float dl = row_ok ? -p.delta[at] : 0.f;
+      const f32x2 c2 = pair(p.scale_log2, p.scale_log2), nl2 = pair(nl, nl), dl2 = pair(dl, dl);
+      const int lim = min(tok, it.len - 1);
+      const int safe = min(first, it.len - 1);
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t ts = ts0 + (j & 1) * 128;
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[j & 1], (j >> 1) & 1, cta_abort, p.status, ST_MATH));
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        float s[64];
+        tmem_ld32(ts, s);
+        tmem_ld32(ts + 32, s + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const f32x2 a = fma2(pair(s[2 * e], s[2 * e + 1]), c2, nl2);
+          s[2 * e] = ex2(lo_of(a));
+          s[2 * e + 1] = ex2(hi_of(a));
+        }
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(dp_full, j & 1, cta_abort, p.status, ST_MATH));
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        float dp[64];
+        tmem_ld32(tp, dp);
+        tmem_ld32(tp + 32, dp + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const f32x2 u = mul2(pair(s[2 * e], s[2 * e + 1]), add2(pair(dp[2 * e], dp[2 * e + 1]), dl2));
+          s[2 * e] = lo_of(u);
+          s[2 * e + 1] = hi_of(u);
+        }
+        if (j * kTile + kTile - 1 > safe) {
+          const int last = lim - j * kTile - half * 64;
+#pragma unroll
+          for (int e = 0; e < 64; ++e) s[e] = e <= last ? s[e] : 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(s[g * 32 + 2 * e], s[g * 32 + 2 * e + 1]);
+          tmem_st16(ts + g * 16, pk);
+        }
+        tmem_wait_st();
+        ptx::tcgen05_fence_before_sync();
+        ptx::mbar_arrive(ds_ready);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, cta_abort, p.status, ST_MATH));
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+#pragma unroll 1
+        for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
+          store_cols<T>(tmem + lane_base + 384 + c, dq, c, p.d, p.scale, row_ok);
+      }
+    }
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename K>
+int launch_bwd(K* kern, int smem, int64_t grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+               const CUtensorMap& g, const Params& p, cudaStream_t s, const char* what) {
+  BT_CHECK_LAUNCHED(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
+  BT_CHECK_ARG(grid <= 0x7fffffffll, "%s: too many tiles (%lld)", what, (long long)grid);
+  BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kBwdThreads), smem, s, q, k, v, g, p),
+                    what);
+  return BT_OK;
+}
+
+template <typename T, int DT>
+int run_bwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, Params p,
+            int64_t batch, cudaStream_t s) {
+  if (p.dk.ptr != nullptr) {
+    p.gran = gran_index(kTile);
+    if (int rc = launch_bwd(attn_dkv_kernel<T, DT>, BwdGeo<DT>::kSmem, max_items(p.total, batch, kTile) * p.hk, q, k,
+                            v, g, p, s, "attn_bwd dk, dv"))
+      return rc;
+  }
+  if (p.dq.ptr != nullptr) {
+    p.gran = gran_index(p.tq);
+    if (int rc = launch_bwd(attn_dq_kernel<T, DT>, BwdGeo<DT>::kSmem,
+                            max_items(p.total, batch, p.tq) * p.hk * p.nsub, q, k, v, g, p, s, "attn_bwd dq"))
+      return rc;
+  }
+  return BT_OK;
+}
+
+template <typename T>
+int run_delta(const void* out, const void* dout, float* delta, int64_t total, int64_t hq, int64_t d,
+              const int64_t* os, const int64_t* gs, cudaStream_t s) {
+  const int64_t rows = total * hq;
+  const int64_t want = ceil_div(rows, 16), cap = static_cast<int64_t>(sm_count()) * 8;
+  BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(static_cast<unsigned>(want < cap ? want : cap)),
+                                     dim3(256), 0, s, static_cast<const T*>(out), static_cast<const T*>(dout), delta,
+                                     rows, static_cast<int>(hq), total, static_cast<int>(d), os[0], os[1], gs[0],
+                                     gs[1]),
+                    "attn_bwd delta");
+  return BT_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace bt
+
+int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns) {
+  return bt::ptx::set_wait_limit_ns(ns) == cudaSuccess ? 0 : -1;
+}
+
+extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                           const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan,
+                           int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides,
+                           const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                           const int64_t* o_strides, const int64_t* dq_strides, const int64_t* dk_strides,
+                           const int64_t* dv_strides, float scale, int dtype, int32_t* status, void* stream) {
+  using namespace bt;
+  using namespace bt::attn;
+  Params p{};
+  if (int rc = fill_params(&p, "attn_bwd", plan, batch, total, hq, hk, d, scale, dtype)) return rc;
+  const int nq = static_cast<int>(hq), nk = static_cast<int>(hk), nd = static_cast<int>(d);
+  BT_CHECK_ARG(lse2 != nullptr && delta != nullptr, "attn_bwd: null pointer");
+  BT_CHECK_ARG((dk == nullptr) == (dv == nullptr), "attn_bwd: dk and dv are computed together");
+  if (int rc = check_view("attn_bwd dout", dout, g_strides[0], g_strides[1], nq, total)) return rc;
+  if (int rc = check_view("attn_bwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
+  if (int rc = check_view("attn_bwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;
+  if (int rc = check_view("attn_bwd v", v, v_strides[0], v_strides[1], nk, total)) return rc;
+  if (int rc = check_view("attn_bwd out", out, o_strides[0], o_strides[1], nq, total)) return rc;
+  if (dq != nullptr) {
+    if (int rc = check_view("attn_bwd dq", dq, dq_strides[0], dq_strides[1], nq, total)) return rc;
+    p.dq = View{dq, dq_strides[0], dq_strides[1]};
+  }
+  if (dk != nullptr) {
+    if (int rc = check_view("attn_bwd dk", dk, dk_strides[0], dk_strides[1], nk, total)) return rc;
+    if (int rc = check_view("attn_bwd dv", dv, dv_strides[0], dv_strides[1], nk, total)) return rc;
+    p.dk = View{dk, dk_strides[0], dk_strides[1]};
+    p.dv = View{dv, dv_strides[0], dv_strides[1]};
+  }
+  p.lse2 = const_cast<float*>(lse2);
+  p.delta = delta;
+  p.status = status;
+  bind_context();
+  CUtensorMap tq, tk, tv, tg;
+  if (int rc = encode_rows(&tq, q, dtype, nd, nq, total, q_strides[1], q_strides[0], p.gp, p.tq, "attn_bwd q")) return rc;
+  if (int rc = encode_rows(&tk, k, dtype, nd, nk, total, k_strides[1], k_strides[0], 1, kTile, "attn_bwd k")) return rc;
+  if (int rc = encode_rows(&tv, v, dtype, nd, nk, total, v_strides[1], v_strides[0], 1, kTile, "attn_bwd v")) return rc;
+  if (int rc = encode_rows(&tg, dout, dtype, nd, nq, total, g_strides[1], g_strides[0], p.gp, p.tq, "attn_bwd dout"))
+    return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == BT_BF16) {
+    if (int rc = run_delta<__nv_bfloat16>(out, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+    return d <= 64 ? run_bwd<__nv_bfloat16, 64>(tq, tk, tv, tg, p, batch, s)
+                   : run_bwd<__nv_bfloat16, 128>(tq, tk, tv, tg, p, batch, s);
+  }
+  if (int rc = run_delta<__half>(out, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+  return d <= 64 ? run_bwd<__half, 64>(tq, tk, tv, tg, p, batch, s) : run_bwd<__half, 128>(tq, tk, tv, tg, p, batch, s);
+}

@@ -1,0 +1,533 @@
+// Causal attention over packed sequences, forward, and the plan that all attention kernels share.
+//
+//   O_i = sum_{j <= i} P_ij V_j,   P_ij = exp(scale q_i.k_j - lse_i),   i, j in the same sequence
+//
+// One CTA per (two consecutive query tiles of 128 packed rows, key/value head): 384 threads,
+//   warps 0..3 / 4..7  softmax of tile 0 / tile 1, one row per thread, then the tile's epilogue
+//   warp 8             issues tcgen05.mma:  S_t = Q_t K_j^T,  O_t += P_t V_j
+//   warp 9             TMA loads: Q once, then K_0, V_0, K_1, ... through one ring
+// (warps 10, 11 complete the warpgroup that hands its registers to the softmax warps).
+// Tensor memory (512 columns): S_0, S_1 (fp32, 128 columns each; P_t in 16 bits replaces the first
+// half of S_t and is the A operand of the second product), O_0, O_1 (fp32).  While the softmax of one
+// tile runs, the tensor pipe works on the other tile.
+#include <mutex>
+
+#include "attn_sm100.cuh"
+
+namespace bt {
+namespace attn {
+namespace {
+
+// ------------------------------------------------------------------ the plan
+constexpr int kPlanThreads = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads)
+attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* __restrict__ words,
+                 int32_t* __restrict__ status) {
+  grid_dependency_wait();
+  __shared__ int s_len[kPlanSort];
+  const int tid = threadIdx.x;
+  const int n = batch + 1;
+  int32_t* start = words;
+  int32_t* len = words + n;
+  // offsets have to start at 0, never fall, and end within the tensor; anything else is reported and
+  // read as "no sequence at all", so that no kernel that follows the plan can leave the tensors
+  bool bad = false;
+  for (int i = tid; i < batch; i += kPlanThreads) {
+    const int a = cu[i], b = cu[i + 1];
+    bad |= a < 0 || b < a || b > total || (i == 0 && a != 0);
+  }
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0 && status != nullptr) atomicOr(status, BT_STATUS_BAD_SEQUENCES);
+  if (batch <= kPlanSort) {
+    // longest first: the tiles of a launch are started in plan order, so the last ones are small
+    if (tid < batch) s_len[tid] = bad ? 0 : cu[tid + 1] - cu[tid];
+    __syncthreads();
+    if (tid < batch) {
+      const int mine = s_len[tid];
+      int rank = 0;
+      for (int j = 0; j < batch; ++j) rank += s_len[j] > mine || (s_len[j] == mine && j < tid);
+      start[rank] = bad ? 0 : cu[tid];
+      len[rank] = mine;
+    }
+  } else {
+    for (int i = tid; i < batch; i += kPlanThreads) {
+      start[i] = bad ? 0 : cu[i];
+      len[i] = bad ? 0 : cu[i + 1] - cu[i];
+    }
+  }
+  if (tid == 0) {
+    const int covered = (bad || batch == 0) ? 0 : cu[batch];
+    start[batch] = covered;
+    len[batch] = total - covered;
+  }
+  __syncthreads();
+  const int g = tid >> 5, lane = tid & 31;
+  if (g < kGrans) {  // one warp per tile height: running tile counts
+    int32_t* pre = words + 2 * n + g * (n + 1);
+    int run = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      int c = i < n ? (len[i] + gran_of(g) - 1) / gran_of(g) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += up;
+      }
+      if (i < n) pre[i + 1] = run + c;
+      run += __shfl_sync(0xffffffffu, c, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+}
+
+// --------------------------------------------------------------- the forward
+constexpr int kFwdThreads = 384;
+
+template <int DT>
+struct FwdGeo {
+  static constexpr int kTileBytes = (DT / 64) * kBoxBytes;
+  static constexpr int kStages = DT == 128 ? 5 : 8;
+  static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024 + 1024;
+};
+
+// Rescaling the output accumulator is put off until a row's maximum has grown by more than this many
+// powers of two: P then stays below 2^8, far inside both 16-bit types, and the sums stay fp32.
+constexpr float kLazyMax = 8.0f;
+
+template <typename T, int DT>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const Params p) {
+  using G = FwdGeo<DT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const uint32_t sQ = ptx::smem_u32(smem);
+  const uint32_t sRing = sQ + 2 * G::kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + (2 + G::kStages) * G::kTileBytes);  // [2]
+  uint64_t* full = q_full + 2;
+  uint64_t* empty = full + G::kStages;
+  uint64_t* s_full = empty + G::kStages;  // [2]
+  uint64_t* p_ready = s_full + 2;         // [2]
+  uint64_t* pv_done = p_ready + 2;        // [2]
+  uint64_t* fix = pv_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_ready[i], 128);
+      ptx::mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < G::kStages; ++i) {
+      ptx::mbar_init(&full[i], 1);
+      ptx::mbar_init(&empty[i], 1);
+    }
+    ptx::mbar_init(fix, 1);
+    *cta_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmQ);
+    ptx::prefetch_tensormap(&tmK);
+    ptx::prefetch_tensormap(&tmV);
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish_alloc_permit();
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  const int groups = p.hk * p.nsub;
+  const int hs = static_cast<int>(blockIdx.x) % groups;
+  Item it{};
+  const bool live = plan_item(p.plan, p.gran, static_cast<int>(blockIdx.x) / groups, lane, &it);
+  const int span = 2 * p.tq;  // tokens of the two tiles
+  const bool behind = live && it.entry == p.plan.n - 1;
+  const int first = live ? (behind ? it.tile : (it.len + span - 1) / span - 1 - it.tile) * span : 0;
+  const int kv_end = live ? min(it.len, first + span) : 0;
+  const int nblk = (live && !behind) ? (kv_end + kTile - 1) / kTile : 0;
+
+  // 384 x 168 registers at launch = 2 x 128 x 208 + 128 x 88
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 9 && nblk > 0) {
+      // ------------------------------------------------------------------ loads
+      bool ok = true;
+      if (lane == 0) {
+  #pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ptx::mbar_arrive_expect_tx(&q_full[t], G::kTileBytes);
+          load_tile<DT>(sQ + t * G::kTileBytes, &tmQ, hs * p.gp, it.start + first + t * p.tq, &q_full[t]);
+        }
+      }
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < 2 * nblk; ++i) {
+        const int kv0 = (i >> 1) * kTile;
+        const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
+        const uint32_t dst = sRing + stage * G::kTileBytes;
+        // rows of V behind the sequence meet P = 0, which is only harmless if they are finite: they are
+        // cleared before the product reads them (rows of K give columns that the mask overwrites)
+        const bool ragged = (i & 1) && kv0 + kTile > it.len;
+        if (lane == 0) {
+          ok = ptx::mbar_wait(&empty[stage], phase ^ 1u, cta_abort, p.status, ST_LOAD);
+          if (ok) {
+            uint64_t* bar = ragged ? fix : &full[stage];
+            ptx::mbar_arrive_expect_tx(bar, G::kTileBytes);
+            load_tile<DT>(dst, tm, hs / p.nsub, it.start + kv0, bar);
+            if (ragged) ok = ptx::mbar_wait(fix, 0, cta_abort, p.status, ST_LOAD);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        if (ragged) {
+          zero_rows<DT>(dst, it.len - kv0, lane);
+          if (lane == 0) ptx::mbar_arrive(&full[stage]);
+        }
+        if (++stage == G::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok || *cta_abort != 0) {  // copies in flight land before the shared memory is handed on
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+    } else if (warp == 8 && nblk > 0) {
+      // ------------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
+        constexpr uint32_t id_s = ptx::make_idesc(fmt, false, false, 128, 128);
+        constexpr uint32_t id_o = ptx::make_idesc(fmt, false, true, 128, DT);
+        const uint32_t o0 = tmem + 256;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = ptx::mbar_wait(&full[0], 0, cta_abort, p.status, ST_ISSUE);
+        for (int t = 0; ok && t < 2; ++t) {
+          ok = ptx::mbar_wait(&q_full[t], 0, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tmem + t * 128, sQ + t * G::kTileBytes, sRing, id_s);
+          ptx::umma_commit(&s_full[t]);
+        }
+        if (ok) ptx::umma_commit(&empty[0]);
+        stage = 1;
+        for (int j = 0; ok && j < nblk; ++j) {
+          const int v_stage = stage;
+          ok = ptx::mbar_wait(&full[v_stage], phase, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          if (++stage == G::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          const int k_stage = stage;
+          const bool more = j + 1 < nblk;
+          const uint32_t k_phase = phase;
+          if (more && ++stage == G::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+  #pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            ok = ptx::mbar_wait(&p_ready[t], j & 1, cta_abort, p.status, ST_ISSUE2);
+            if (!ok) break;
+            ptx::tcgen05_fence_after_sync();
+            const uint32_t pt = tmem + t * 128;
+            mma_pb<DT>(o0 + t * DT, pt, pt + 32, sRing + v_stage * G::kTileBytes, id_o, j > 0);
+            ptx::umma_commit(&pv_done[t]);
+            if (more) {
+              if (t == 0) {
+                ok = ptx::mbar_wait(&full[k_stage], k_phase, cta_abort, p.status, ST_ISSUE);
+                if (!ok) break;
+                ptx::tcgen05_fence_after_sync();
+              }
+              mma_abt<DT>(pt, sQ + t * G::kTileBytes, sRing + k_stage * G::kTileBytes, id_s);
+              ptx::umma_commit(&s_full[t]);
+            }
+          }
+          if (!ok) break;
+          ptx::umma_commit(&empty[v_stage]);
+          if (more) ptx::umma_commit(&empty[k_stage]);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ------------------------------------------------- softmax and epilogue
+    if (live) {
+      const int t = warp >> 2;
+      const int row = (warp & 3) * 32 + lane;
+      const int tok = first + t * p.tq + (row >> p.gp_shift);
+      const int head = hs * p.gp + (row & (p.gp - 1));
+      const int64_t token = static_cast<int64_t>(it.start) + tok;
+      const bool row_ok = tok < it.len;
+      T* out = static_cast<T*>(p.o.ptr) + token * p.o.st + head * p.o.sh;
+      if (behind) {
+        if (row_ok)
+          for (int c = 0; c < p.d; c += 8) st_global_v4(out + c, make_uint4(0, 0, 0, 0));
+      } else {
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lane_base + t * 128;
+        const uint32_t to = tmem + lane_base + 256 + t * DT;
+        const int lim = min(tok, it.len - 1);  // last key this row sees
+        const int safe = min(first + t * p.tq, it.len - 1);  // last key that every row of the tile sees
+        const float c = p.scale_log2;
+        float m = 0.f, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < nblk; ++j) {
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], j & 1, cta_abort, p.status, ST_MATH));
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          float s[128];
+  #pragma unroll
+          for (int q = 0; q < 4; ++q) tmem_ld32(ts + q * 32, s + q * 32);
+          tmem_wait_ld();
+          if (j * kTile + kTile - 1 > safe) {
+            const int last = lim - j * kTile;
+  #pragma unroll
+            for (int e = 0; e < 128; ++e) s[e] = e <= last ? s[e] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+  #pragma unroll
+          for (int e = 4; e < 128; e += 8) {
+  #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (e + 4 + q < 128) mx[q] = fmaxf(mx[q], fmaxf(s[e + q], s[e + 4 + q]));
+              else mx[q] = fmaxf(mx[q], s[e + q]);
+            }
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (j == 0) {
+            m = top;
+          } else {
+            const bool grow = (top - m) * c > kLazyMax;
+            if (__any_sync(0xffffffffu, grow)) {
+              // the tile's previous product has to be in O before O is rescaled
+              ok = __all_sync(0xffffffffu,
+                              ptx::mbar_wait(&pv_done[t], (j - 1) & 1, cta_abort, p.status, ST_MATH));
+              if (!ok) break;
+              ptx::tcgen05_fence_after_sync();
+              const float nm = fmaxf(m, top);
+              const float alpha = ex2((m - nm) * c);
+              m = nm;
+              l *= alpha;
+  #pragma unroll 1
+              for (int q = 0; q < DT / 32; ++q) {
+                float o[32];
+                tmem_ld32(to + q * 32, o);
+                tmem_wait_ld();
+  #pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                tmem_st32(to + q * 32, o);
+              }
+              tmem_wait_st();
+            }
+          }
+          const f32x2 c2 = pair(c, c), mc2 = pair(-m * c, -m * c);
+          f32x2 sum2 = pair(0.f, 0.f);
+  #pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+  #pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const f32x2 x = fma2(pair(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), c2, mc2);
+              const float a = ex2(lo_of(x)), b = ex2(hi_of(x));
+              sum2 = add2(sum2, pair(a, b));
+              pk[e] = pack2<T>(a, b);  // the product's operand type; the sum keeps fp32
+            }
+            tmem_st16(ts + q * 16, pk);
+          }
+          l += lo_of(sum2) + hi_of(sum2);
+          tmem_wait_st();
+          ptx::tcgen05_fence_before_sync();
+          ptx::mbar_arrive(&p_ready[t]);
+        }
+        if (ok)
+          ok = __all_sync(0xffffffffu,
+                          ptx::mbar_wait(&pv_done[t], (nblk - 1) & 1, cta_abort, p.status, ST_MATH));
+        if (ok) {
+          ptx::tcgen05_fence_after_sync();
+          const float inv = 1.0f / l;
+          if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
+  #pragma unroll 1
+          for (int q = 0; q < DT / 32; ++q) {
+            float o[32];
+            tmem_ld32(to + q * 32, o);
+            tmem_wait_ld();
+            if (row_ok) {
+  #pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint32_t w[4];
+  #pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = pack2<T>(o[v * 8 + 2 * e] * inv, o[v * 8 + 2 * e + 1] * inv);
+                if (q * 32 + v * 8 < p.d) st_global_v4(out + q * 32 + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int DT>
+int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int64_t batch,
+               cudaStream_t s) {
+  auto* kern = attn_fwd_kernel<T, DT>;
+  // per device and cheap: the attribute belongs to the current device's copy of the kernel
+  BT_CHECK_LAUNCHED(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdGeo<DT>::kSmem),
+                    "attn_fwd: shared memory");
+  const int64_t grid = max_items(p.total, batch, 2 * p.tq) * p.hk * p.nsub;
+  BT_CHECK_ARG(grid <= 0x7fffffffll, "attn_fwd: too many tiles (%lld)", (long long)grid);
+  BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdGeo<DT>::kSmem, s,
+                                     q, k, v, p),
+                    "attn_fwd");
+  return BT_OK;
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+}  // namespace
+
+int check_view(const char* what, const void* p, int64_t st, int64_t sh, int heads, int64_t total) {
+  BT_CHECK_ARG(p != nullptr, "%s: null pointer", what);
+  BT_CHECK_ARG(aligned16(p), "%s: must be 16-byte aligned", what);
+  BT_CHECK_ARG((total <= 1 || (st > 0 && st % 8 == 0)) && (heads <= 1 || (sh > 0 && sh % 8 == 0)),
+               "%s: token and head strides must be positive multiples of 8 elements", what);
+  return BT_OK;
+}
+
+int encode_rows(CUtensorMap* tm, const void* ptr, int dtype, int d, int heads, int64_t total, int64_t sh, int64_t st,
+                int box_heads, int box_tokens, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return BT_ERR_DRIVER;
+  }
+  // the stride of a dimension of one element is never used, but it has to be a valid one
+  const int64_t row = (d + 7) / 8 * 8;
+  if (heads <= 1) sh = row;
+  if (total <= 1) st = row * heads;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(total)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(tm, dtype == BT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("%s: cuTensorMapEncodeTiled failed with CUresult %d (%d x %d x %lld, strides %lld %lld)", what,
+              static_cast<int>(r), d, heads, (long long)total, (long long)sh, (long long)st);
+    return BT_ERR_DRIVER;
+  }
+  return BT_OK;
+}
+
+int fill_params(Params* p, const char* what, const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk,
+                int64_t d, float scale, int dtype) {
+  BT_CHECK_ARG(dtype == BT_BF16 || dtype == BT_FP16, "%s: dtype must be bf16 or fp16 (got %d)", what, dtype);
+  BT_CHECK_ARG(plan != nullptr, "%s: null plan", what);
+  BT_CHECK_ARG(batch >= 0 && batch < (1 << 24) && total > 0 && total < (1ll << 30), "%s: bad batch or token count", what);
+  BT_CHECK_ARG(hk >= 1 && hq >= hk && hq % hk == 0 && hq <= 65536, "%s: query heads must be a multiple of key/value heads",
+               what);
+  BT_CHECK_ARG(d >= 8 && d <= 128 && d % 8 == 0, "%s: head_dim must be a multiple of 8, at most 128 (got %lld)", what,
+               (long long)d);
+  p->plan.words = plan;
+  p->plan.n = static_cast<int>(batch) + 1;
+  p->hq = static_cast<int>(hq);
+  p->hk = static_cast<int>(hk);
+  p->d = static_cast<int>(d);
+  p->total = static_cast<int>(total);
+  const int group = static_cast<int>(hq / hk);
+  p->gp = 1;
+  p->gp_shift = 0;
+  while (p->gp < 16 && group % (2 * p->gp) == 0) {
+    p->gp *= 2;
+    ++p->gp_shift;
+  }
+  p->nsub = group / p->gp;
+  p->tq = kTile / p->gp;
+  p->scale = scale;
+  p->scale_log2 = scale * kLog2e;
+  return BT_OK;
+}
+
+}  // namespace attn
+}  // namespace bt
+
+int bt_internal_set_wait_limit_attn_fwd(unsigned long long ns) {
+  return bt::ptx::set_wait_limit_ns(ns) == cudaSuccess ? 0 : -1;
+}
+
+extern "C" int64_t bt_attn_plan_words(int64_t batch) { return batch < 0 ? 0 : bt::attn::plan_words(batch); }
+
+extern "C" int bt_attn_plan(const int32_t* cu_seqlens, int64_t batch, int64_t total, int32_t* plan, int32_t* status,
+                            void* stream) {
+  using namespace bt;
+  BT_CHECK_ARG(batch >= 0 && batch < (1 << 24) && total >= 0 && total < (1ll << 30), "attn_plan: bad batch or token count");
+  BT_CHECK_ARG(cu_seqlens != nullptr && plan != nullptr, "attn_plan: null pointer");
+  BT_CHECK_LAUNCHED(launch_dependent(attn::attn_plan_kernel, dim3(1), dim3(attn::kPlanThreads), 0,
+                                     static_cast<cudaStream_t>(stream), cu_seqlens, static_cast<int>(batch),
+                                     static_cast<int>(total), plan, status),
+                    "attn_plan");
+  return BT_OK;
+}
+
+extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse2, const int32_t* plan,
+                           int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
+                           const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale,
+                           int dtype, int32_t* status, void* stream) {
+  using namespace bt;
+  using namespace bt::attn;
+  Params p{};
+  if (int rc = fill_params(&p, "attn_fwd", plan, batch, total, hq, hk, d, scale, dtype)) return rc;
+  const int nq = static_cast<int>(hq), nk = static_cast<int>(hk), nd = static_cast<int>(d);
+  if (int rc = check_view("attn_fwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
+  if (int rc = check_view("attn_fwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;
+  if (int rc = check_view("attn_fwd v", v, v_strides[0], v_strides[1], nk, total)) return rc;
+  if (int rc = check_view("attn_fwd out", out, o_strides[0], o_strides[1], nq, total)) return rc;
+  p.gran = gran_index(2 * p.tq);
+  p.lse2 = lse2;
+  p.o = View{out, o_strides[0], o_strides[1]};
+  p.status = status;
+  bind_context();
+  CUtensorMap tq, tk, tv;
+  if (int rc = encode_rows(&tq, q, dtype, nd, nq, total, q_strides[1], q_strides[0], p.gp, p.tq, "attn_fwd q")) return rc;
+  if (int rc = encode_rows(&tk, k, dtype, nd, nk, total, k_strides[1], k_strides[0], 1, kTile, "attn_fwd k")) return rc;
+  if (int rc = encode_rows(&tv, v, dtype, nd, nk, total, v_strides[1], v_strides[0], 1, kTile, "attn_fwd v")) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == BT_BF16)
+    return d <= 64 ? launch_fwd<__nv_bfloat16, 64>(tq, tk, tv, p, batch, s)
+                   : launch_fwd<__nv_bfloat16, 128>(tq, tk, tv, p, batch, s);
+  return d <= 64 ? launch_fwd<__half, 64>(tq, tk, tv, p, batch, s) : launch_fwd<__half, 128>(tq, tk, tv, p, batch, s);
+}

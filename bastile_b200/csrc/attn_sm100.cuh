@@ -1,0 +1,227 @@
+// Shared pieces of the packed-attention kernels: the sequence plan, 3-D tile loads of head-packed
+// rows, MMAs whose A operand lies in tensor memory, and the shared-memory layout of the tiles.
+//
+// Row packing.  With grouped heads, GP (the largest power of two that divides Hq / Hk, at most 16)
+// query heads of one key/value head share a tile: row r of a 128-row query tile is token r / GP, head
+// r % GP of the group.  A tile then spans TQ = 128 / GP tokens, all of its rows use the same K and V
+// tiles, and sums over query rows in the backward run over the heads of the group by themselves.
+//
+// Every operand tile is 128 rows of DT (64 or 128) 16-bit elements, stored as DT / 64 boxes of
+// 128 rows x 128 bytes with the 128-byte TMA swizzle.  A head_dim below DT is zero-filled by TMA.
+#pragma once
+
+#include <type_traits>
+
+#include "bt_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace bt {
+namespace attn {
+
+constexpr int kTile = 128;          // rows of every operand tile
+constexpr int kBoxBytes = 128 * 128;  // 128 rows x 64 16-bit elements
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum : int { ST_LOAD = 1, ST_ISSUE = 2, ST_ISSUE2 = 4, ST_MATH = 8 };
+
+// ------------------------------------------------------------------ the plan
+// int32 words written once per batch by bt_attn_plan: start[n], len[n] of the n = batch + 1 entries
+// (the sequences, longest first when there are at most kPlanSort of them, then the rows behind the
+// last sequence), then for each tile height kGran[g] the n + 1 running tile counts.
+constexpr int kGrans = 6;
+constexpr int kPlanSort = 1024;
+__host__ __device__ constexpr int gran_of(int g) { return 8 << g; }
+__host__ __device__ inline int gran_index(int tokens) {
+  int g = 0;
+  while (gran_of(g) < tokens) ++g;
+  return g;
+}
+inline int64_t plan_words(int64_t batch) { return (batch + 1) * 2 + kGrans * (batch + 2); }
+
+struct Plan {
+  const int32_t* words;
+  int n;  // entries
+};
+// a tile of one entry
+struct Item {
+  int start, len, tile, entry;  // entry == n - 1: rows behind the last sequence
+};
+
+// The item-th tile of height kGran[g] (one warp; all lanes get the answer); false: no such tile.
+__device__ __forceinline__ bool plan_item(const Plan& p, int g, int item, int lane, Item* it) {
+  const int32_t* pre = p.words + 2 * p.n + g * (p.n + 1);
+  int lo = 0, hi = p.n;
+  if (item >= __ldg(pre + hi)) return false;
+  while (hi - lo > 1) {  // invariant: pre[lo] <= item < pre[hi]; 32 probes a round
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + (lane + 1) * step;
+    const bool le = at < hi && __ldg(pre + at) <= item;
+    const int c = __popc(__ballot_sync(0xffffffffu, le));
+    const int base = lo;
+    lo = base + c * step;
+    hi = min(base + (c + 1) * step, hi);
+  }
+  it->entry = lo;
+  it->start = __ldg(p.words + lo);
+  it->len = __ldg(p.words + p.n + lo);
+  it->tile = item - __ldg(pre + lo);
+  return true;
+}
+
+// Grid bound for tiles of `tokens`: every entry rounds up by less than one tile.
+inline int64_t max_items(int64_t total, int64_t batch, int64_t tokens) {
+  return (total + (batch + 1) * (tokens - 1)) / tokens;
+}
+
+// ----------------------------------------------------------------- PTX pieces
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* tm, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(ptx::smem_u32(bar))
+      : "memory");
+}
+// One operand tile: DT / 64 boxes.
+template <int DT>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* tm, int head, int token, uint64_t* bar) {
+#pragma unroll
+  for (int j = 0; j < DT / 64; ++j) tma_load_3d(dst + j * kBoxBytes, tm, j * 64, head, token, bar);
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc]; A: 128 lanes, two 16-bit K elements per 32-bit column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 columns of this thread's lane; the registers are valid after tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+      "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+      "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ------------------------------------------------------- MMAs over whole tiles
+// Constant halves of the shared-memory descriptors (tiles above).
+constexpr uint64_t kDescK = ptx::make_smem_desc_hi(true, 0);                // rows = M/N, K along the row
+constexpr uint64_t kDescMN = ptx::make_smem_desc_hi(false, kBoxBytes);      // rows = K, M/N along the row
+
+// D[128 x 128] = A[128 x DT] B[128 x DT]^T, both from shared memory, K-major.
+template <int DT>
+__device__ __forceinline__ void mma_abt(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < DT / 16; ++k) {
+    const uint32_t off = static_cast<uint32_t>((k / 4) * kBoxBytes + (k % 4) * 32);
+    ptx::umma_f16(d, ptx::smem_desc(kDescK, a_smem + off), ptx::smem_desc(kDescK, b_smem + off), idesc, k != 0);
+  }
+}
+// D[128 x DT] (+)= A[128 x 128] B[128 x DT]: A 16-bit in tensor memory with its first 64 columns of K
+// at a_lo and the other 64 at a_hi, B rows = K.
+template <int DT>
+__device__ __forceinline__ void mma_pb(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_smem, uint32_t idesc,
+                                       bool accumulate) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t a = (k < 4 ? a_lo : a_hi) + static_cast<uint32_t>((k % 4) * 8);
+    umma_f16_ts(d, a, ptx::smem_desc(kDescMN, b_smem + static_cast<uint32_t>(k * 16 * 128)), idesc,
+                (accumulate || k != 0) ? 1u : 0u);
+  }
+}
+
+// Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.
+template <int DT>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int first, int lane) {
+#pragma unroll
+  for (int j = 0; j < DT / 64; ++j)
+    for (int i = first * 8 + lane; i < 128 * 8; i += 32)
+      ptx::st_shared_v4(tile + j * kBoxBytes + i * 16, make_uint4(0, 0, 0, 0));
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// What every kernel is told about one [tokens, heads, head_dim] tensor besides its tile map.
+struct View {
+  void* ptr;
+  int64_t st, sh;  // element strides of a token and of a head
+};
+
+struct Params {
+  Plan plan;
+  int hq, hk, d, total;
+  int gp, gp_shift, tq, nsub;  // packed heads, log2, tokens per tile, packed groups per kv head
+  int gran;                    // index of the tile height that this kernel's items have
+  float scale, scale_log2;
+  float* lse2;   // [hq][total] base-2 log-sum-exp of the scaled scores
+  float* delta;  // [hq][total] dot(dO, O)
+  View o, dq, dk, dv;
+  int32_t* status;
+};
+
+// The tensor-map encoder is a driver call and wants a current context: a thread that has made no runtime
+// call yet (an autograd worker, say) gets its device's own.  Allowed during stream capture.
+inline void bind_context() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
+
+// Host side (attn_fwd.cu)
+int fill_params(Params* p, const char* what, const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk,
+                int64_t d, float scale, int dtype);
+int check_view(const char* what, const void* p, int64_t st, int64_t sh, int heads, int64_t total);
+int encode_rows(CUtensorMap* tm, const void* ptr, int dtype, int d, int heads, int64_t total, int64_t sh, int64_t st,
+                int box_heads, int box_tokens, const char* what);
+
+}  // namespace attn
+}  // namespace bt

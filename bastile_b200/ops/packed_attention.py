@@ -1,0 +1,145 @@
+"""Causal attention over packed sequences with grouped heads, on the sm_100a kernels.
+
+The reference leaves attention to torch (its patches stop at q/k-norm + RoPE); here the op stands
+between ``qk_norm_rope`` and ``o_proj``.  A batch of sequences of different lengths lies one behind
+the other along the token axis, without padding, and ``pack_sequences`` turns their offsets into
+what the kernels need, on the device and without a host synchronisation.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+
+_DTYPES = (torch.bfloat16, torch.float16)
+MAX_HEAD_DIM = 128
+
+
+class PackedSequences:
+    """The layout of one packed batch (made by ``pack_sequences``): usable by any number of
+    attention calls, forward and backward, on work ordered behind its creation."""
+
+    __slots__ = ("plan", "batch", "total_tokens", "device")
+
+    def __init__(self, plan: Tensor, batch: int, total_tokens: int):
+        self.plan, self.batch, self.total_tokens, self.device = plan, batch, total_tokens, plan.device
+
+
+def pack_sequences(cu_seqlens: Tensor, total_tokens: int) -> PackedSequences:
+    """``cu_seqlens`` [batch + 1] (int32 or int64, on the GPU): sequence ``b`` is tokens
+    ``cu_seqlens[b] .. cu_seqlens[b + 1]`` of ``total_tokens``; the first offset is 0, sequences may be
+    empty, tokens behind the last one belong to no sequence.  Offsets that start elsewhere, fall or
+    run past ``total_tokens`` are noticed on the device: attention then gives zeros, and
+    ``bastile_b200._lib.check_all_status()`` raises."""
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"pack_sequences: cu_seqlens must be [batch + 1], got {tuple(cu_seqlens.shape)}")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"pack_sequences: cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+    total_tokens = int(total_tokens)
+    if not 0 <= total_tokens < 1 << 30:
+        raise ValueError(f"pack_sequences: total_tokens must be in [0, 2^30), got {total_tokens}")
+    dev = _lib.require_cuda(cu_seqlens)
+    lib = _lib.get_lib()
+    if cu_seqlens.dtype == torch.int64:
+        # an offset that does not fit 32 bits is past the tokens in either type
+        cu_seqlens = cu_seqlens.clamp(-1, 1 << 30).to(torch.int32)
+    cu = cu_seqlens.contiguous()
+    batch = cu.numel() - 1
+    with _lib.device_of(dev), _lib.timed("attn_plan", 1, dev):
+        plan = torch.empty(int(lib.bt_attn_plan_words(batch)), dtype=torch.int32, device=dev)
+        rc = lib.bt_attn_plan(cu.data_ptr(), batch, total_tokens, plan.data_ptr(), _lib.status_word(dev).data_ptr(),
+                              _lib.stream_ptr(dev))
+    _lib.check(rc, "bt_attn_plan")
+    return PackedSequences(plan, batch, total_tokens)
+
+
+def _strides(t: Tensor):
+    return _lib.I64x2(t.stride(0), t.stride(1))
+
+
+def _rows(t: Tensor) -> Tensor:
+    """``t`` if the kernels can read it where it lies (unit stride along the head, 16-byte rows), else a copy."""
+    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2])))
+    return t if ok else t.contiguous()
+
+
+class PackedAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sequences, scale):
+        dev = q.device
+        lib = _lib.get_lib()
+        t, hq, d = q.shape
+        hk = k.shape[1]
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        lse2 = torch.empty((hq, t), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad[:3]) else None
+        if out.numel() > 0:
+            st = _lib.status_word(dev)
+            with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
+                rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                     lse2.data_ptr() if lse2 is not None else None, sequences.plan.data_ptr(),
+                                     sequences.batch, t, hq, hk, d, _strides(q), _strides(k), _strides(v),
+                                     _strides(out), scale, _lib.dtype_code(q.dtype), st.data_ptr(),
+                                     _lib.stream_ptr(dev))
+            _lib.check(rc, "bt_attn_fwd")
+        if lse2 is not None:
+            ctx.save_for_backward(q, k, v, out, lse2, sequences.plan)
+            ctx.meta = (sequences.batch, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse2, plan = ctx.saved_tensors
+        batch, scale = ctx.meta
+        dev = q.device
+        lib = _lib.get_lib()
+        t, hq, d = q.shape
+        hk = k.shape[1]
+        dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq = torch.empty((t, hq, d), dtype=q.dtype, device=dev) if need_q else None
+        dk = torch.empty((t, hk, d), dtype=q.dtype, device=dev) if need_kv else None
+        dv = torch.empty((t, hk, d), dtype=q.dtype, device=dev) if need_kv else None
+        if q.numel() > 0:
+            delta = torch.empty((hq, t), dtype=torch.float32, device=dev)
+            st = _lib.status_word(dev)
+            none = _lib.I64x2(0, 0)
+            with _lib.device_of(dev), _lib.timed("attn_bwd", 1 + int(need_q) + int(need_kv), dev):
+                rc = lib.bt_attn_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                     lse2.data_ptr(), delta.data_ptr(), dq.data_ptr() if need_q else None,
+                                     dk.data_ptr() if need_kv else None, dv.data_ptr() if need_kv else None,
+                                     plan.data_ptr(), batch, t, hq, hk, d, _strides(dout), _strides(q), _strides(k),
+                                     _strides(v), _strides(out), _strides(dq) if need_q else none,
+                                     _strides(dk) if need_kv else none, _strides(dv) if need_kv else none, scale,
+                                     _lib.dtype_code(q.dtype), st.data_ptr(), _lib.stream_ptr(dev))
+            _lib.check(rc, "bt_attn_bwd")
+        return dq, dk, dv, None, None
+
+
+def packed_attention(q: Tensor, k: Tensor, v: Tensor, sequences: PackedSequences, scale: float | None = None) -> Tensor:
+    """``out[t, h] = sum_s softmax_s(scale * q[t, h] . k[s, h // group]) v[s, h // group]`` over the tokens
+    ``s <= t`` of ``t``'s own sequence; q [tokens, Hq, D], k and v [tokens, Hk, D] with Hq a multiple of Hk
+    and D a multiple of 8 up to 128, bf16 or fp16 (scores, softmax statistics and sums are fp32).
+    Strided views are read where they lie as long as heads are contiguous and 16-byte aligned.  Rows
+    behind the last sequence are zeros and get zero gradients.  ``scale`` defaults to ``D ** -0.5``."""
+    if not isinstance(sequences, PackedSequences):
+        raise TypeError("packed_attention: sequences must come from pack_sequences()")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("packed_attention: q, k and v must be [tokens, heads, head_dim]")
+    t, hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d:
+        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} disagree")
+    if k.shape[1] < 1 or hq % k.shape[1] != 0 or hq < 1:
+        raise ValueError(f"packed_attention: {hq} query heads are not a multiple of {k.shape[1]} key/value heads")
+    if d < 8 or d % 8 != 0 or d > MAX_HEAD_DIM:
+        raise ValueError(f"packed_attention: head_dim must be a multiple of 8 up to {MAX_HEAD_DIM}, got {d}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"packed_attention: q, k and v must share bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if t != sequences.total_tokens:
+        raise ValueError(f"packed_attention: q has {t} tokens, the packed sequences {sequences.total_tokens}")
+    _lib.require_cuda(q, k, v, sequences.plan)
+    scale = d ** -0.5 if scale is None else float(scale)
+    return PackedAttentionFunction.apply(q, k, v, sequences, scale)

@@ -41,6 +41,7 @@ extern "C" {
  * are invalid.  BT_STATUS_BAD_LABEL reports invalid INPUT, not a device problem. */
 #define BT_STATUS_WAIT_MASK 0x0f
 #define BT_STATUS_BAD_LABEL 0x10
+#define BT_STATUS_BAD_SEQUENCES 0x20
 
 /* Library version (major*10000 + minor*100 + patch). No reference counterpart
  * (the reference is a JIT Python package: src/bastile/__init__.py:23). */
@@ -443,6 +444,39 @@ int bt_adamw_master_step(float* master, float* exp_avg, float* exp_avg_sq,
                          const void* grad, void* param_out, int64_t numel,
                          float lr, float beta1, float beta2, float eps, float weight_decay,
                          int64_t step, float grad_scale, int ctas_per_sm, int dtype, void* stream);
+
+/* ---- causal attention over packed sequences (no reference counterpart: the reference leaves
+ * attention to torch; its call site is Qwen3Attention.forward) ----
+ *
+ * Sequences lie one behind the other along the token axis: sequence b is tokens [cu_seqlens[b],
+ * cu_seqlens[b + 1]).  bt_attn_plan reads the offsets on the device once per batch and lays out what
+ * the kernels below need to deal tiles: `plan` is bt_attn_plan_words(batch) int32 words, any number
+ * of calls may use it at the same time.  Offsets that do not start at 0, fall, or run past `total`
+ * set BT_STATUS_BAD_SEQUENCES in `status` (may be NULL) and are read as "no sequence": the kernels
+ * then write zeros.  batch < 2^24, total < 2^30.  */
+int64_t bt_attn_plan_words(int64_t batch);
+int bt_attn_plan(const int32_t* cu_seqlens, int64_t batch, int64_t total, int32_t* plan, int32_t* status,
+                 void* stream);
+
+/* out[t, h, :] = sum over s <= t of the same sequence of softmax_s(scale q[t,h].k[s,h/(hq/hk)]) v[s].
+ * q, out [total, hq, d], k, v [total, hk, d]; BT_BF16 or BT_FP16; *_strides = element strides of
+ * (token, head), multiples of 8; unit stride along d; d a multiple of 8, at most 128.  Rows behind the
+ * last sequence are written as zeros.  lse2 (may be NULL): [hq, total] fp32, the base-2 log-sum-exp of
+ * the scaled scores, written for rows of sequences only. */
+int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse2, const int32_t* plan,
+                int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
+                const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale, int dtype,
+                int32_t* status, void* stream);
+
+/* Gradients of bt_attn_fwd for the upstream gradient `dout` (bt_attn_fwd's out and lse2 come back in).
+ * dq may be NULL, and so may dk and dv together; `delta` is [hq, total] fp32 scratch.  Rows behind the
+ * last sequence get zeros.  No atomics: the same inputs give the same bits. */
+int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse2,
+                float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch, int64_t total,
+                int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides, const int64_t* q_strides,
+                const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides, float scale,
+                int dtype, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }
