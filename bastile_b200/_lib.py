@@ -95,6 +95,15 @@ SIGNATURES = {
                     [c_float, c_int, c_void_p, c_void_p]),
     "bt_attn_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
                     [c_float, c_int, c_void_p, c_void_p]),
+    "bt_logp_stats": (c_int, [c_void_p] * 6 + [c_int64] * 6 + [c_int, c_void_p, c_void_p]),
+    "bt_logp_rows": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_void_p, c_void_p]),
+    "bt_logp_coef": (c_int, [c_void_p] * 2 + [c_int64] * 3 + [c_void_p] * 3),
+    "bt_logp_dlogits": (c_int, [c_void_p] * 6 + [c_int64] * 5 + [c_int, c_void_p, c_void_p]),
+    "bt_logp_mask_rows": (c_int, [c_void_p] * 3 + [c_int64] * 5 + [c_int, c_void_p]),
+    "bt_policy_weights": (c_int, [c_void_p, c_int64, c_void_p] + [c_int64] * 3 + [c_void_p] * 4),
+    "bt_policy_rows": (c_int, [c_void_p] * 13 + [c_int64] * 6 + [c_float] * 3 + [c_void_p]),
+    "bt_policy_dlogits": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_int, c_void_p]),
+    "bt_policy_reduce": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "bt_scale_cast": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),
 }
 
@@ -287,7 +296,8 @@ def _describe_status(v: int) -> str:
     if v & STATUS_WAIT_MASK:
         parts.append(f"a bounded device-side wait ran out (bits {v & STATUS_WAIT_MASK:#x}): results are invalid")
     if v & STATUS_BAD_LABEL:
-        parts.append("fused_linear_cross_entropy got a label that is neither ignore_index nor a vocabulary row")
+        parts.append("fused_linear_cross_entropy got a label that is neither ignore_index nor a vocabulary row "
+                     "(or fused_linear_log_probs / fused_linear_policy_loss such a target)")
     if v & STATUS_BAD_SEQUENCES:
         parts.append("sequence offsets do not start at 0, fall, or run past the packed tokens")
     return "; ".join(parts) or f"status {v:#x}"

@@ -72,7 +72,15 @@ struct Geo {
   static constexpr int kBoxBytes = kBk * kRowBytes;                       // one MN-major box
 };
 
-enum : int { EPI_PLAIN = 0, EPI_SWIGLU_FWD = 1, EPI_SWIGLU_BWD = 2, EPI_LCE = 3 };
+enum : int {
+  EPI_PLAIN = 0,
+  EPI_SWIGLU_FWD = 1,
+  EPI_SWIGLU_BWD = 2,
+  EPI_LCE = 3,
+  EPI_LOGP = 4,         // softmax statistics of the unrounded logits
+  EPI_LOGP_SHIFT = 5,   // the same, and logits minus their half tile's maximum to memory
+  EPI_DLOGITS = 6       // coef * (onehot - softmax) from given log-sum-exps
+};
 
 // Status-word bits set when a bounded wait runs out.
 enum : int { ST_PRODUCER = 1, ST_MMA_ACC = 2, ST_MMA_FULL = 4, ST_EPILOGUE = 8 };
@@ -124,6 +132,9 @@ struct Params {
   float* tgt_logit;
   int64_t v_offset, ignore_index;
   int n_vtiles;
+  // --- log-probability gradient epilogue
+  const float* row_lse;
+  const float* row_coef;
 };
 
 __device__ __forceinline__ void tile_coords(const Params& p, int tile, int* m_idx, int* n_idx) {
@@ -511,6 +522,114 @@ __device__ __forceinline__ void epi_lce(const Params& p, uint32_t taddr, int64_t
   }
 }
 
+// Accumulator = logits tile, statistics for log-probabilities: (max, sum exp) of each half tile and
+// the target logit, all from the fp32 accumulator.  (epi_lce rounds the logits to T first, as the
+// model's own lm_head would; a log-probability that is compared with another one to a percent cannot
+// afford the 2^-9 |logit| of that.)  Two passes over the accumulator - maximum, then exponentials -
+// because tensor memory is cheap to read twice while the next tile's 32k-cycle main loop runs.
+// SHIFT: also stores logit - half-tile maximum in T.  Near the maximum, where the softmax has its
+// mass, that difference is small and its rounding harmless.
+template <typename T, bool SHIFT>
+__device__ __forceinline__ void epi_logp(const Params& p, uint32_t taddr, int64_t row, int n0, int n_idx, int half,
+                                         OutStage& stg, const CUtensorMap* tm_logits, int lane) {
+  const bool row_ok = row < p.M;
+  const int row0 = static_cast<int>(row) - lane;
+  constexpr float kNegBig = -1e30f;
+  constexpr int kCols = BN / 64;  // 32-column chunks of a half
+  int tgt_col = -1;
+  bool owned = false;
+  if (row_ok) {
+    const int64_t label = p.labels[row];
+    owned = label != p.ignore_index && label >= 0 && label < p.N;
+    if (owned && label >= n0 + half * (BN / 2) && label < n0 + (half + 1) * (BN / 2))
+      tgt_col = static_cast<int>(label - n0);
+  }
+  float mx = kNegBig, sum = 0.f, tgt = 0.f;
+#pragma unroll 1
+  for (int c = half * kCols; c < (half + 1) * kCols; ++c) {
+    float v[32];
+    ptx::tmem_ld_32cols(taddr + c * 32, v);
+    const int valid = p.N - n0 - c * 32;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, j < valid ? v[j] : kNegBig);
+  }
+#pragma unroll 1
+  for (int c = half * kCols; c < (half + 1) * kCols; ++c) {
+    float v[32];
+    ptx::tmem_ld_32cols(taddr + c * 32, v);
+    const int col0 = n0 + c * 32;
+    const int valid = p.N - col0;
+    if (valid > 0) {
+      if (tgt_col >= c * 32 && tgt_col < c * 32 + 32) {
+        const int jj = tgt_col - c * 32;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j == jj) tgt = v[j];
+      }
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        v[j] = j < valid ? v[j] - mx : kNegBig;
+        s += __expf(v[j]);
+      }
+      sum += s;
+      if constexpr (SHIFT) {
+        if (stg.base != 0) {
+          if (row0 < p.M) stage_store32<T>(stg, tm_logits, v, col0, row0, lane);
+        } else if (row_ok) {
+          store_row32<T>(static_cast<T*>(p.out) + row * p.ldo + col0, v, valid, p.vec_ok);
+        }
+      }
+    }
+  }
+  if (row_ok) {
+    *reinterpret_cast<float2*>(p.tile_stats + (row * p.n_vtiles + n_idx * 2 + half) * 2) = make_float2(mx, sum);
+    if (tgt_col >= 0)
+      p.tgt_logit[row] = tgt;
+    else if (n_idx == 0 && half == 0 && !owned)
+      p.tgt_logit[row] = 0.f;
+  }
+}
+
+// Accumulator = logits tile; writes coef * (onehot - exp(logit - lse)) in T: the gradient of
+// sum_rows coef * log-probability, straight from the recomputed fp32 logits.  Rows with coef = 0
+// (ignored positions) are zeros whatever their logits hold.
+template <typename T>
+__device__ __forceinline__ void epi_dlogits(const Params& p, uint32_t taddr, int64_t row, int n0, int half,
+                                            OutStage& stg, const CUtensorMap* tm_out, int lane) {
+  const bool row_ok = row < p.M;
+  const int row0 = static_cast<int>(row) - lane;
+  float lse = 0.f, coef = 0.f;
+  int tgt_col = -1;
+  if (row_ok) {
+    lse = p.row_lse[row];
+    coef = p.row_coef[row];
+    const int64_t label = p.labels[row];
+    if (label >= n0 && label < n0 + BN) tgt_col = static_cast<int>(label - n0);
+  }
+#pragma unroll 1
+  for (int c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+    float v[32];
+    ptx::tmem_ld_32cols(taddr + c * 32, v);
+    const int col0 = n0 + c * 32;
+    const int valid = p.N - col0;
+    if (valid <= 0) continue;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = coef != 0.f ? -coef * __expf(v[j] - lse) : 0.f;
+    if (coef != 0.f && tgt_col >= c * 32 && tgt_col < c * 32 + 32) {
+      const int jj = tgt_col - c * 32;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j == jj) v[j] += coef;
+    }
+    if (stg.base != 0) {
+      if (row0 < p.M) stage_store32<T>(stg, tm_out, v, col0, row0, lane);
+    } else if (row_ok) {
+      store_row32<T>(static_cast<T*>(p.out) + row * p.ldo + col0, v, valid, p.vec_ok);
+    }
+  }
+}
+
 // Which tensor map, and which coordinates inside it, hold the A tile of rows m0.. for k-block kb.
 struct ASource {
   const CUtensorMap* map;
@@ -727,6 +846,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
         epi_swiglu_fwd<T>(p, taddr, row, n_idx * (BN / 2), half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_BWD) epi_swiglu_bwd<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, lane);
       if (EPI == EPI_LCE) epi_lce<T>(p, taddr, row, n_idx * BN, n_idx, half, stg, &tmO0, lane);
+      if (EPI == EPI_LOGP || EPI == EPI_LOGP_SHIFT)
+        epi_logp<T, EPI == EPI_LOGP_SHIFT>(p, taddr, row, n_idx * BN, n_idx, half, stg, &tmO0, lane);
+      if (EPI == EPI_DLOGITS) epi_dlogits<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, lane);
       ptx::tcgen05_fence_before_sync();
       ptx::mbar_arrive(&tempty[acc]);
       acc ^= 1;
@@ -776,7 +898,7 @@ constexpr int kSchedRing = 16;
 constexpr int kSchedMaxPairs = 256;
 constexpr int kSchedWords = 1 + kSchedMaxPairs * kSchedRing;
 constexpr int kSchedSlots = 32;
-__device__ unsigned long long g_tile_sched[kSchedSlots][kSchedWords];
+static __device__ unsigned long long g_tile_sched[kSchedSlots][kSchedWords];
 
 __device__ __forceinline__ int sched_draw(const Params& p) {
   const unsigned int t = atomicAdd(reinterpret_cast<unsigned int*>(p.sched), 1u);
@@ -1015,6 +1137,9 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         epi_swiglu_fwd<T>(p, taddr, row, n_idx * (BN / 2), half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_BWD) epi_swiglu_bwd<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, lane);
       if (EPI == EPI_LCE) epi_lce<T>(p, taddr, row, n_idx * BN, n_idx, half, stg, &tmO0, lane);
+      if (EPI == EPI_LOGP || EPI == EPI_LOGP_SHIFT)
+        epi_logp<T, EPI == EPI_LOGP_SHIFT>(p, taddr, row, n_idx * BN, n_idx, half, stg, &tmO0, lane);
+      if (EPI == EPI_DLOGITS) epi_dlogits<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, lane);
       ptx::tcgen05_fence_before_sync();
       if (leader)
         ptx::mbar_arrive(&tempty[acc]);

@@ -627,13 +627,15 @@ extern "C" int64_t bt_rmsnorm_bwd_ws_bytes(int64_t N) {
 int bt_internal_set_wait_limit_tc(unsigned long long ns);        // tc_ops.cu
 int bt_internal_set_wait_limit_attn_fwd(unsigned long long ns);  // attn_fwd.cu
 int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns);  // attn_bwd.cu
+int bt_internal_set_wait_limit_logp(unsigned long long ns);      // logp_ops.cu
 
 extern "C" int bt_set_wait_limit_ms(int64_t ms) {
   using namespace bt;
   BT_CHECK_ARG(ms >= 1 && ms <= 600000, "set_wait_limit_ms: the limit must be 1 ms .. 10 min");
   const unsigned long long ns = static_cast<unsigned long long>(ms) * 1000000ull;
   if (ptx::set_wait_limit_ns(ns) != cudaSuccess || bt_internal_set_wait_limit_tc(ns) != 0 ||
-      bt_internal_set_wait_limit_attn_fwd(ns) != 0 || bt_internal_set_wait_limit_attn_bwd(ns) != 0) {
+      bt_internal_set_wait_limit_attn_fwd(ns) != 0 || bt_internal_set_wait_limit_attn_bwd(ns) != 0 ||
+      bt_internal_set_wait_limit_logp(ns) != 0) {
     set_error("set_wait_limit_ms: writing the limit to the device failed");
     return BT_ERR_LAUNCH;
   }
