@@ -46,8 +46,10 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* 
 template <int DT>
 struct BwdGeo {
   static constexpr int kTileBytes = (DT / 64) * kBoxBytes;
-  static constexpr int kVecBytes = 2 * 2 * 128 * 4;  // two stages of -lse and D of a query tile
-  static constexpr int kSmem = 6 * kTileBytes + kVecBytes + 1024 + 1024;
+  static constexpr int kVecBytes = 2 * 2 * 128 * 4;  // two stages of -lse and -D of a query tile
+  // K, V, three Q and two dO tiles (dK, dV), or Q, dO, three K and two V tiles (dQ); no slack to
+  // align the start: the kernels check that the dynamic shared memory starts on 1024 bytes
+  static constexpr int kSmem = 7 * kTileBytes + kVecBytes + 512;
 };
 
 template <typename T>
@@ -81,6 +83,14 @@ __device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, i
   return ok;
 }
 
+// The tiles need a 1024-byte start, which is where dynamic shared memory begins when a kernel has no
+// other; should that ever change, the call reports itself as failed instead of reading wrong tiles.
+__device__ __forceinline__ bool aligned_start(const uint8_t* smem, int32_t* status) {
+  const bool ok = (ptx::smem_u32(smem) & 1023u) == 0;
+  if (!ok && threadIdx.x == 0 && status != nullptr) atomicOr(status, ST_LOAD);
+  return ok;
+}
+
 __device__ __forceinline__ void drain_copies() {
   const uint64_t t0 = ptx::globaltimer_ns();
   while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
@@ -106,29 +116,32 @@ __device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, int col0, int
 // One CTA per (128 keys, key/value head).  Warps 0..7: one key row and half of the 128 query columns
 // per thread; warp 8 issues, warp 9 loads.  Transposed scores, so that P^T and dS^T are the
 // tensor-memory operands of the two sums:
-//   S^T = K Q_i^T -> P^T (16 bits, in place) ; dV += P^T dO_i ; dP^T = V dO_i^T -> dS^T ; dK += dS^T Q_i
-// A half's 16-bit P^T lies in the first 32 of the 64 columns it read, so no warp overwrites another's.
+//   S^T = K Q_i^T ; dP^T = V dO_i^T ; dV += P^T dO_i ; dK += dS^T Q_i
+// Tensor memory is full (S^T, dP^T, dV, dK: 128 columns each), so the 16-bit P^T and dS^T replace dP^T:
+// a warp writes both into the 64 columns that it has just read, P^T in the first 32.  S^T is free as
+// soon as it is in registers, and S^T of the next tile is computed under this tile's dS phase; the
+// exponentials of the next tile then run under dV, dK and dP^T.
 template <typename T, int DT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const Params p) {
   using G = BwdGeo<DT>;
   constexpr int TB = G::kTileBytes;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  const uint32_t sK = ptx::smem_u32(smem), sV = sK + TB, sQ = sK + 2 * TB, sG = sK + 4 * TB;
-  float* vec = reinterpret_cast<float*>(smem + 6 * TB);  // [stage][-lse | D][128]
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + 6 * TB + G::kVecBytes);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!aligned_start(smem, p.status)) return;
+  const uint32_t sK = ptx::smem_u32(smem), sV = sK + TB, sQ = sK + 2 * TB, sG = sK + 5 * TB;
+  float* vec = reinterpret_cast<float*>(smem + 7 * TB);  // [stage][-lse | -D][128]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + 7 * TB + G::kVecBytes);
   uint64_t* v_full = k_full + 1;
-  uint64_t* q_full = v_full + 1;    // [2]
-  uint64_t* q_empty = q_full + 2;   // [2]
-  uint64_t* g_full = q_empty + 2;   // [2]
-  uint64_t* g_empty = g_full + 2;   // [2]
-  uint64_t* vec_full = g_empty + 2; // [2]
-  uint64_t* s_full = vec_full + 2;
-  uint64_t* p_ready = s_full + 1;
-  uint64_t* dp_full = p_ready + 1;
+  uint64_t* q_full = v_full + 1;      // [3]
+  uint64_t* q_empty = q_full + 3;     // [3]
+  uint64_t* g_full = q_empty + 3;     // [2]
+  uint64_t* g_empty = g_full + 2;     // [2]
+  uint64_t* vec_full = g_empty + 2;   // [2]
+  uint64_t* vec_empty = vec_full + 2; // [2]
+  uint64_t* s_full = vec_empty + 2;
+  uint64_t* s_free = s_full + 1;
+  uint64_t* dp_full = s_free + 1;
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* done = ds_ready + 1;
   uint64_t* fix = done + 1;
@@ -139,17 +152,20 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   if (threadIdx.x == 0) {
     ptx::mbar_init(k_full, 1);
     ptx::mbar_init(v_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
       ptx::mbar_init(&q_full[i], 1);
       ptx::mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&g_full[i], 1);
       ptx::mbar_init(&g_empty[i], 1);
       ptx::mbar_init(&vec_full[i], 32);
+      ptx::mbar_init(&vec_empty[i], 8);
     }
     ptx::mbar_init(s_full, 1);
-    ptx::mbar_init(p_ready, 256);
+    ptx::mbar_init(s_free, 8);
     ptx::mbar_init(dp_full, 1);
-    ptx::mbar_init(ds_ready, 256);
+    ptx::mbar_init(ds_ready, 8);
     ptx::mbar_init(done, 1);
     ptx::mbar_init(fix, 1);
     *cta_abort = 0;
@@ -191,6 +207,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       uint32_t fix_phase = 0;
       bool ok = true;
       int sub = 0, i = i0;
+      int qs = 0;
+      uint32_t q_par = 1;
       for (int x = 0; ok && x < n; ++x) {
         const int st = x & 1;
         const uint32_t par = ((x >> 1) & 1) ^ 1u;
@@ -199,17 +217,17 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const int valid = min(p.tq, it.len - tok0) << p.gp_shift;
         // rows of Q and dO behind the sequence are cleared: they meet P = dS = 0, as the rest of a
         // product they only have to be finite
-        ok = ring_load<DT>(sQ + st * TB, &tmQ, head, it.start + tok0, valid, &q_full[st], &q_empty[st], par, fix,
-                           &fix_phase, lane, cta_abort, p.status);
+        ok = ring_load<DT>(sQ + qs * TB, &tmQ, head, it.start + tok0, valid, &q_full[qs], &q_empty[qs], q_par, fix,
+                           &fix_phase, lane, cta_abort, p.status) &&
+             __all_sync(0xffffffffu, ptx::mbar_wait(&vec_empty[st], par, cta_abort, p.status, ST_LOAD));
         if (!ok) break;
-        // q_empty also says that the math warps are done with this stage of the row vectors
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = e * 32 + lane;
           const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + it.start + tok0 + (r >> p.gp_shift);
           const bool in = r < valid;
           vec[st * 256 + r] = in ? -__ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
-          vec[st * 256 + 128 + r] = in ? __ldg(p.delta + at) : 0.f;
+          vec[st * 256 + 128 + r] = in ? -__ldg(p.delta + at) : 0.f;
         }
         ptx::mbar_arrive(&vec_full[st]);
         ok = ring_load<DT>(sG + st * TB, &tmG, head, it.start + tok0, valid, &g_full[st], &g_empty[st], par, fix,
@@ -217,6 +235,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (++i == i0 + per) {
           i = i0;
           ++sub;
+        }
+        if (++qs == 3) {
+          qs = 0;
+          q_par ^= 1u;
         }
       }
       if (!ok || *cta_abort != 0) drain_copies();
@@ -239,33 +261,45 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         mma_abt<DT>(tP, sV, sG, id_s);
         ptx::umma_commit(dp_full);
       }
-      for (int x = 0; ok && x < n; ++x) {
-        const int st = x & 1, nst = st ^ 1;
-        const uint32_t npar = ((x + 1) >> 1) & 1;
-        const bool more = x + 1 < n;
-        ok = ptx::mbar_wait(p_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
-        if (!ok) break;
-        ptx::tcgen05_fence_after_sync();
-        mma_pb<DT>(tV, tS, tS + 64, sG + st * TB, id_o, x > 0);
-        ptx::umma_commit(&g_empty[st]);
-        if (more) {
-          ok = ptx::mbar_wait(&q_full[nst], npar, cta_abort, p.status, ST_ISSUE);
-          if (!ok) break;
+      if (ok && n > 1) {
+        ok = ptx::mbar_wait(&q_full[1], 0, cta_abort, p.status, ST_ISSUE) &&
+             ptx::mbar_wait(s_free, 0, cta_abort, p.status, ST_ISSUE2);
+        if (ok) {
           ptx::tcgen05_fence_after_sync();
-          mma_abt<DT>(tS, sK, sQ + nst * TB, id_s);
+          mma_abt<DT>(tS, sK, sQ + TB, id_s);
           ptx::umma_commit(s_full);
         }
+      }
+      int qs = 0, q2 = 2;  // Q stages of tiles x and x + 2
+      uint32_t q2_par = 0;
+      for (int x = 0; ok && x < n; ++x) {
+        const int st = x & 1, nst = st ^ 1;
         ok = ptx::mbar_wait(ds_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
         if (!ok) break;
         ptx::tcgen05_fence_after_sync();
-        mma_pb<DT>(tK, tP, tP + 64, sQ + st * TB, id_o, x > 0);
-        ptx::umma_commit(&q_empty[st]);
-        if (more) {
-          ok = ptx::mbar_wait(&g_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+        mma_pb<DT>(tV, tP, tP + 64, sG + st * TB, id_o, x > 0);
+        ptx::umma_commit(&g_empty[st]);
+        mma_pb<DT>(tK, tP + 32, tP + 96, sQ + qs * TB, id_o, x > 0);
+        ptx::umma_commit(&q_empty[qs]);
+        qs = qs == 2 ? 0 : qs + 1;
+        if (x + 1 < n) {
+          ok = ptx::mbar_wait(&g_full[nst], ((x + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tP, sV, sG + nst * TB, id_s);
           ptx::umma_commit(dp_full);
+        }
+        if (x + 2 < n) {
+          ok = ptx::mbar_wait(&q_full[q2], q2_par, cta_abort, p.status, ST_ISSUE) &&
+               ptx::mbar_wait(s_free, (x + 1) & 1, cta_abort, p.status, ST_ISSUE2);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tS, sK, sQ + q2 * TB, id_s);
+          ptx::umma_commit(s_full);
+          if (++q2 == 3) {
+            q2 = 0;
+            q2_par ^= 1u;
+          }
         }
       }
       if (ok) ptx::umma_commit(done);
@@ -303,6 +337,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tmem_ld32(ts, s);
         tmem_ld32(ts + 32, s + 32);
         tmem_wait_ld();
+        ptx::tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(s_free);
         const int tok0 = i * p.tq;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -319,16 +356,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 64; ++e) s[e] = e >= lo ? s[e] : 0.f;
         }
+        uint32_t pp[32];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = pack2<T>(s[g * 32 + 2 * e], s[g * 32 + 2 * e + 1]);
-          tmem_st16(ts + g * 16, pk);
-        }
-        tmem_wait_st();
-        ptx::tcgen05_fence_before_sync();
-        ptx::mbar_arrive(p_ready);
+        for (int e = 0; e < 32; ++e) pp[e] = pack2<T>(s[2 * e], s[2 * e + 1]);
 
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(dp_full, x & 1, cta_abort, p.status, ST_MATH));
         if (!ok) break;
@@ -337,6 +367,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tmem_ld32(tp, dp);
         tmem_ld32(tp + 32, dp + 32);
         tmem_wait_ld();
+        tmem_st16(tp, pp);
+        tmem_st16(tp + 16, pp + 16);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           uint32_t pk[16];
@@ -344,16 +376,20 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           for (int e = 0; e < 8; ++e) {
             const float4 d4 = dl[g * 8 + e];
             const int b = g * 32 + 4 * e;
-            const f32x2 u = mul2(pair(s[b], s[b + 1]), add2(pair(dp[b], dp[b + 1]), neg2(pair(d4.x, d4.y))));
-            const f32x2 v = mul2(pair(s[b + 2], s[b + 3]), add2(pair(dp[b + 2], dp[b + 3]), neg2(pair(d4.z, d4.w))));
+            const f32x2 u = mul2(pair(s[b], s[b + 1]), add2(pair(dp[b], dp[b + 1]), pair(d4.x, d4.y)));
+            const f32x2 v = mul2(pair(s[b + 2], s[b + 3]), add2(pair(dp[b + 2], dp[b + 3]), pair(d4.z, d4.w)));
             pk[2 * e] = pack2<T>(lo_of(u), hi_of(u));
             pk[2 * e + 1] = pack2<T>(lo_of(v), hi_of(v));
           }
-          tmem_st16(tp + g * 16, pk);
+          tmem_st16(tp + 32 + g * 16, pk);
         }
         tmem_wait_st();
         ptx::tcgen05_fence_before_sync();
-        ptx::mbar_arrive(ds_ready);
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(ds_ready);
+          ptx::mbar_arrive(&vec_empty[st]);
+        }
         if (++i == i0 + per) i = i0;
       }
       if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, cta_abort, p.status, ST_MATH));
@@ -382,7 +418,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // ------------------------------------------------------------------------ dQ
 // One CTA per (query tile of 128 packed rows, key/value head).  Warps 0..7: one query row and half of
 // the 128 key columns per thread.  S is double-buffered in tensor memory (its buffer then holds the
-// 16-bit dS), so the tensor pipe computes S_{j+1} and dP_{j+1} while the math warps work on tile j:
+// 16-bit dS) and dP is free once it is in registers, so S_{j+1} and dP_{j+1} are ready when the math
+// warps are done with tile j:
 //   S = Q K_j^T ; dP = dO V_j^T ; dS = P (dP - D) ; dQ += dS K_j
 template <typename T, int DT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -390,19 +427,19 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const Params p) {
   using G = BwdGeo<DT>;
   constexpr int TB = G::kTileBytes;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  const uint32_t sQ = ptx::smem_u32(smem), sG = sQ + TB, sK = sQ + 2 * TB, sV = sQ + 4 * TB;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + 6 * TB);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!aligned_start(smem, p.status)) return;
+  const uint32_t sQ = ptx::smem_u32(smem), sG = sQ + TB, sK = sQ + 2 * TB, sV = sQ + 5 * TB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + 7 * TB);
   uint64_t* g_full = q_full + 1;
-  uint64_t* k_full = g_full + 1;   // [2]
-  uint64_t* k_empty = k_full + 2;  // [2]
-  uint64_t* v_full = k_empty + 2;  // [2]
+  uint64_t* k_full = g_full + 1;   // [3]
+  uint64_t* k_empty = k_full + 3;  // [3]
+  uint64_t* v_full = k_empty + 3;  // [2]
   uint64_t* v_empty = v_full + 2;  // [2]
   uint64_t* s_full = v_empty + 2;  // [2]
   uint64_t* dp_full = s_full + 2;
-  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* dp_free = dp_full + 1;
+  uint64_t* ds_ready = dp_free + 1;
   uint64_t* done = ds_ready + 1;
   uint64_t* fix = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
@@ -412,15 +449,18 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   if (threadIdx.x == 0) {
     ptx::mbar_init(q_full, 1);
     ptx::mbar_init(g_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
       ptx::mbar_init(&k_full[i], 1);
       ptx::mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&v_full[i], 1);
       ptx::mbar_init(&v_empty[i], 1);
       ptx::mbar_init(&s_full[i], 1);
     }
     ptx::mbar_init(dp_full, 1);
-    ptx::mbar_init(ds_ready, 256);
+    ptx::mbar_init(dp_free, 8);
+    ptx::mbar_init(ds_ready, 8);
     ptx::mbar_init(done, 1);
     ptx::mbar_init(fix, 1);
     *cta_abort = 0;
@@ -460,14 +500,20 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       }
       uint32_t fix_phase = 0;
       bool ok = true;
+      int ks = 0;
+      uint32_t k_par = 1;
       for (int j = 0; ok && j < n; ++j) {
         const int st = j & 1;
         const uint32_t par = ((j >> 1) & 1) ^ 1u;
         // K rows behind the sequence meet dS = 0 and have to be finite; V's only give masked columns
-        ok = ring_load<DT>(sK + st * TB, &tmK, hs / p.nsub, it.start + j * kTile, min(kTile, it.len - j * kTile),
-                           &k_full[st], &k_empty[st], par, fix, &fix_phase, lane, cta_abort, p.status) &&
+        ok = ring_load<DT>(sK + ks * TB, &tmK, hs / p.nsub, it.start + j * kTile, min(kTile, it.len - j * kTile),
+                           &k_full[ks], &k_empty[ks], k_par, fix, &fix_phase, lane, cta_abort, p.status) &&
              ring_load<DT>(sV + st * TB, &tmV, hs / p.nsub, it.start + j * kTile, kTile, &v_full[st], &v_empty[st],
                            par, fix, &fix_phase, lane, cta_abort, p.status);
+        if (++ks == 3) {
+          ks = 0;
+          k_par ^= 1u;
+        }
       }
       if (!ok || *cta_abort != 0) drain_copies();
     } else if (warp == 8 && n > 0 && lane == 0) {
@@ -490,29 +536,43 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         ptx::umma_commit(dp_full);
         ptx::umma_commit(&v_empty[0]);
       }
+      if (ok && n > 1) {
+        ok = ptx::mbar_wait(&k_full[1], 0, cta_abort, p.status, ST_ISSUE);
+        if (ok) {
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tmem + 128, sQ, sK + TB, id_s);
+          ptx::umma_commit(&s_full[1]);
+        }
+      }
+      int ks = 0, k2 = 2;  // K stages of tiles j and j + 2
+      uint32_t k2_par = 0;
       for (int j = 0; ok && j < n; ++j) {
         const int st = j & 1, nst = st ^ 1;
-        const uint32_t npar = ((j + 1) >> 1) & 1;
-        const bool more = j + 1 < n;
-        if (more) {
-          ok = ptx::mbar_wait(&k_full[nst], npar, cta_abort, p.status, ST_ISSUE);
-          if (!ok) break;
-          ptx::tcgen05_fence_after_sync();
-          mma_abt<DT>(tmem + nst * 128, sQ, sK + nst * TB, id_s);
-          ptx::umma_commit(&s_full[nst]);
-        }
-        ok = ptx::mbar_wait(ds_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
-        if (!ok) break;
-        ptx::tcgen05_fence_after_sync();
-        mma_pb<DT>(tQ, tmem + st * 128, tmem + st * 128 + 64, sK + st * TB, id_o, j > 0);
-        ptx::umma_commit(&k_empty[st]);
-        if (more) {
-          ok = ptx::mbar_wait(&v_full[nst], npar, cta_abort, p.status, ST_ISSUE);
+        if (j + 1 < n) {  // dP of the next tile as soon as this one's is in registers
+          ok = ptx::mbar_wait(&v_full[nst], ((j + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE) &&
+               ptx::mbar_wait(dp_free, j & 1, cta_abort, p.status, ST_ISSUE2);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tP, sG, sV + nst * TB, id_s);
           ptx::umma_commit(dp_full);
           ptx::umma_commit(&v_empty[nst]);
+        }
+        ok = ptx::mbar_wait(ds_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        mma_pb<DT>(tQ, tmem + st * 128, tmem + st * 128 + 64, sK + ks * TB, id_o, j > 0);
+        ptx::umma_commit(&k_empty[ks]);
+        ks = ks == 2 ? 0 : ks + 1;
+        if (j + 2 < n) {
+          ok = ptx::mbar_wait(&k_full[k2], k2_par, cta_abort, p.status, ST_ISSUE);
+          if (!ok) break;
+          ptx::tcgen05_fence_after_sync();
+          mma_abt<DT>(tmem + st * 128, sQ, sK + k2 * TB, id_s);
+          ptx::umma_commit(&s_full[st]);
+          if (++k2 == 3) {
+            k2 = 0;
+            k2_par ^= 1u;
+          }
         }
       }
       if (ok) ptx::umma_commit(done);
@@ -561,6 +621,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         tmem_ld32(tp, dp);
         tmem_ld32(tp + 32, dp + 32);
         tmem_wait_ld();
+        ptx::tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(dp_free);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const f32x2 u = mul2(pair(s[2 * e], s[2 * e + 1]), add2(pair(dp[2 * e], dp[2 * e + 1]), dl2));
@@ -581,7 +644,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         }
         tmem_wait_st();
         ptx::tcgen05_fence_before_sync();
-        ptx::mbar_arrive(ds_ready);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ds_ready);
       }
       if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, cta_abort, p.status, ST_MATH));
       if (ok) {

@@ -120,7 +120,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&q_full[i], 1);
       ptx::mbar_init(&s_full[i], 1);
-      ptx::mbar_init(&p_ready[i], 128);
+      ptx::mbar_init(&p_ready[i], 4);
       ptx::mbar_init(&pv_done[i], 1);
     }
     for (int i = 0; i < G::kStages; ++i) {
@@ -347,7 +347,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           l += lo_of(sum2) + hi_of(sum2);
           tmem_wait_st();
           ptx::tcgen05_fence_before_sync();
-          ptx::mbar_arrive(&p_ready[t]);
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&p_ready[t]);
         }
         if (ok)
           ok = __all_sync(0xffffffffu,
