@@ -242,67 +242,67 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       if (!ok || *cta_abort != 0) drain_copies();
-    } else if (warp == 8 && n > 0 && lane == 0) {
+    } else if (warp == 8 && n > 0) {
       // ----------------------------------------------------------- MMA issuer
       constexpr uint32_t id_s = ptx::make_idesc(mma_fmt<T>(), false, false, 128, 128);
       constexpr uint32_t id_o = ptx::make_idesc(mma_fmt<T>(), false, true, 128, DT);
       const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DT;
-      bool ok = ptx::mbar_wait(k_full, 0, cta_abort, p.status, ST_ISSUE) &&
-                ptx::mbar_wait(&q_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      bool ok = warp_wait(k_full, 0, cta_abort, p.status, ST_ISSUE) &&
+                warp_wait(&q_full[0], 0, cta_abort, p.status, ST_ISSUE);
       if (ok) {
         ptx::tcgen05_fence_after_sync();
         mma_abt<DT>(tS, sK, sQ, id_s);
-        ptx::umma_commit(s_full);
-        ok = ptx::mbar_wait(v_full, 0, cta_abort, p.status, ST_ISSUE) &&
-             ptx::mbar_wait(&g_full[0], 0, cta_abort, p.status, ST_ISSUE);
+        mma_commit(s_full);
+        ok = warp_wait(v_full, 0, cta_abort, p.status, ST_ISSUE) &&
+             warp_wait(&g_full[0], 0, cta_abort, p.status, ST_ISSUE);
       }
       if (ok) {
         ptx::tcgen05_fence_after_sync();
         mma_abt<DT>(tP, sV, sG, id_s);
-        ptx::umma_commit(dp_full);
+        mma_commit(dp_full);
       }
       if (ok && n > 1) {
-        ok = ptx::mbar_wait(&q_full[1], 0, cta_abort, p.status, ST_ISSUE) &&
-             ptx::mbar_wait(s_free, 0, cta_abort, p.status, ST_ISSUE2);
+        ok = warp_wait(&q_full[1], 0, cta_abort, p.status, ST_ISSUE) &&
+             warp_wait(s_free, 0, cta_abort, p.status, ST_ISSUE2);
         if (ok) {
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tS, sK, sQ + TB, id_s);
-          ptx::umma_commit(s_full);
+          mma_commit(s_full);
         }
       }
       int qs = 0, q2 = 2;  // Q stages of tiles x and x + 2
       uint32_t q2_par = 0;
       for (int x = 0; ok && x < n; ++x) {
         const int st = x & 1, nst = st ^ 1;
-        ok = ptx::mbar_wait(ds_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
+        ok = warp_wait(ds_ready, x & 1, cta_abort, p.status, ST_ISSUE2);
         if (!ok) break;
         ptx::tcgen05_fence_after_sync();
         mma_pb<DT>(tV, tP, tP + 64, sG + st * TB, id_o, x > 0);
-        ptx::umma_commit(&g_empty[st]);
+        mma_commit(&g_empty[st]);
         mma_pb<DT>(tK, tP + 32, tP + 96, sQ + qs * TB, id_o, x > 0);
-        ptx::umma_commit(&q_empty[qs]);
+        mma_commit(&q_empty[qs]);
         qs = qs == 2 ? 0 : qs + 1;
         if (x + 1 < n) {
-          ok = ptx::mbar_wait(&g_full[nst], ((x + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE);
+          ok = warp_wait(&g_full[nst], ((x + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tP, sV, sG + nst * TB, id_s);
-          ptx::umma_commit(dp_full);
+          mma_commit(dp_full);
         }
         if (x + 2 < n) {
-          ok = ptx::mbar_wait(&q_full[q2], q2_par, cta_abort, p.status, ST_ISSUE) &&
-               ptx::mbar_wait(s_free, (x + 1) & 1, cta_abort, p.status, ST_ISSUE2);
+          ok = warp_wait(&q_full[q2], q2_par, cta_abort, p.status, ST_ISSUE) &&
+               warp_wait(s_free, (x + 1) & 1, cta_abort, p.status, ST_ISSUE2);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tS, sK, sQ + q2 * TB, id_s);
-          ptx::umma_commit(s_full);
+          mma_commit(s_full);
           if (++q2 == 3) {
             q2 = 0;
             q2_par ^= 1u;
           }
         }
       }
-      if (ok) ptx::umma_commit(done);
+      if (ok) mma_commit(done);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -516,32 +516,32 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         }
       }
       if (!ok || *cta_abort != 0) drain_copies();
-    } else if (warp == 8 && n > 0 && lane == 0) {
+    } else if (warp == 8 && n > 0) {
       // ----------------------------------------------------------- MMA issuer
       constexpr uint32_t id_s = ptx::make_idesc(mma_fmt<T>(), false, false, 128, 128);
       constexpr uint32_t id_o = ptx::make_idesc(mma_fmt<T>(), false, true, 128, DT);
       const uint32_t tP = tmem + 256, tQ = tmem + 384;
-      bool ok = ptx::mbar_wait(q_full, 0, cta_abort, p.status, ST_ISSUE) &&
-                ptx::mbar_wait(&k_full[0], 0, cta_abort, p.status, ST_ISSUE);
+      bool ok = warp_wait(q_full, 0, cta_abort, p.status, ST_ISSUE) &&
+                warp_wait(&k_full[0], 0, cta_abort, p.status, ST_ISSUE);
       if (ok) {
         ptx::tcgen05_fence_after_sync();
         mma_abt<DT>(tmem, sQ, sK, id_s);
-        ptx::umma_commit(&s_full[0]);
-        ok = ptx::mbar_wait(g_full, 0, cta_abort, p.status, ST_ISSUE) &&
-             ptx::mbar_wait(&v_full[0], 0, cta_abort, p.status, ST_ISSUE);
+        mma_commit(&s_full[0]);
+        ok = warp_wait(g_full, 0, cta_abort, p.status, ST_ISSUE) &&
+             warp_wait(&v_full[0], 0, cta_abort, p.status, ST_ISSUE);
       }
       if (ok) {
         ptx::tcgen05_fence_after_sync();
         mma_abt<DT>(tP, sG, sV, id_s);
-        ptx::umma_commit(dp_full);
-        ptx::umma_commit(&v_empty[0]);
+        mma_commit(dp_full);
+        mma_commit(&v_empty[0]);
       }
       if (ok && n > 1) {
-        ok = ptx::mbar_wait(&k_full[1], 0, cta_abort, p.status, ST_ISSUE);
+        ok = warp_wait(&k_full[1], 0, cta_abort, p.status, ST_ISSUE);
         if (ok) {
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tmem + 128, sQ, sK + TB, id_s);
-          ptx::umma_commit(&s_full[1]);
+          mma_commit(&s_full[1]);
         }
       }
       int ks = 0, k2 = 2;  // K stages of tiles j and j + 2
@@ -549,33 +549,33 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       for (int j = 0; ok && j < n; ++j) {
         const int st = j & 1, nst = st ^ 1;
         if (j + 1 < n) {  // dP of the next tile as soon as this one's is in registers
-          ok = ptx::mbar_wait(&v_full[nst], ((j + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE) &&
-               ptx::mbar_wait(dp_free, j & 1, cta_abort, p.status, ST_ISSUE2);
+          ok = warp_wait(&v_full[nst], ((j + 1) >> 1) & 1, cta_abort, p.status, ST_ISSUE) &&
+               warp_wait(dp_free, j & 1, cta_abort, p.status, ST_ISSUE2);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tP, sG, sV + nst * TB, id_s);
-          ptx::umma_commit(dp_full);
-          ptx::umma_commit(&v_empty[nst]);
+          mma_commit(dp_full);
+          mma_commit(&v_empty[nst]);
         }
-        ok = ptx::mbar_wait(ds_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
+        ok = warp_wait(ds_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
         if (!ok) break;
         ptx::tcgen05_fence_after_sync();
         mma_pb<DT>(tQ, tmem + st * 128, tmem + st * 128 + 64, sK + ks * TB, id_o, j > 0);
-        ptx::umma_commit(&k_empty[ks]);
+        mma_commit(&k_empty[ks]);
         ks = ks == 2 ? 0 : ks + 1;
         if (j + 2 < n) {
-          ok = ptx::mbar_wait(&k_full[k2], k2_par, cta_abort, p.status, ST_ISSUE);
+          ok = warp_wait(&k_full[k2], k2_par, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tmem + st * 128, sQ, sK + k2 * TB, id_s);
-          ptx::umma_commit(&s_full[st]);
+          mma_commit(&s_full[st]);
           if (++k2 == 3) {
             k2 = 0;
             k2_par ^= 1u;
           }
         }
       }
-      if (ok) ptx::umma_commit(done);
+      if (ok) mma_commit(done);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");

@@ -161,7 +161,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       // ------------------------------------------------------------------ loads
       bool ok = true;
       if (lane == 0) {
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
           ptx::mbar_arrive_expect_tx(&q_full[t], G::kTileBytes);
           load_tile<DT>(sQ + t * G::kTileBytes, &tmQ, hs * p.gp, it.start + first + t * p.tq, &q_full[t]);
@@ -202,26 +202,26 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
     } else if (warp == 8 && nblk > 0) {
       // ------------------------------------------------------------- MMA issuer
-      if (lane == 0) {
+      {
         constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
         constexpr uint32_t id_s = ptx::make_idesc(fmt, false, false, 128, 128);
         constexpr uint32_t id_o = ptx::make_idesc(fmt, false, true, 128, DT);
         const uint32_t o0 = tmem + 256;
         int stage = 0;
         uint32_t phase = 0;
-        bool ok = ptx::mbar_wait(&full[0], 0, cta_abort, p.status, ST_ISSUE);
+        bool ok = warp_wait(&full[0], 0, cta_abort, p.status, ST_ISSUE);
         for (int t = 0; ok && t < 2; ++t) {
-          ok = ptx::mbar_wait(&q_full[t], 0, cta_abort, p.status, ST_ISSUE);
+          ok = warp_wait(&q_full[t], 0, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           mma_abt<DT>(tmem + t * 128, sQ + t * G::kTileBytes, sRing, id_s);
-          ptx::umma_commit(&s_full[t]);
+          mma_commit(&s_full[t]);
         }
-        if (ok) ptx::umma_commit(&empty[0]);
+        if (ok) mma_commit(&empty[0]);
         stage = 1;
         for (int j = 0; ok && j < nblk; ++j) {
           const int v_stage = stage;
-          ok = ptx::mbar_wait(&full[v_stage], phase, cta_abort, p.status, ST_ISSUE);
+          ok = warp_wait(&full[v_stage], phase, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           if (++stage == G::kStages) {
             stage = 0;
@@ -234,27 +234,27 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             stage = 0;
             phase ^= 1u;
           }
-  #pragma unroll
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
-            ok = ptx::mbar_wait(&p_ready[t], j & 1, cta_abort, p.status, ST_ISSUE2);
+            ok = warp_wait(&p_ready[t], j & 1, cta_abort, p.status, ST_ISSUE2);
             if (!ok) break;
             ptx::tcgen05_fence_after_sync();
             const uint32_t pt = tmem + t * 128;
             mma_pb<DT>(o0 + t * DT, pt, pt + 32, sRing + v_stage * G::kTileBytes, id_o, j > 0);
-            ptx::umma_commit(&pv_done[t]);
+            mma_commit(&pv_done[t]);
             if (more) {
               if (t == 0) {
-                ok = ptx::mbar_wait(&full[k_stage], k_phase, cta_abort, p.status, ST_ISSUE);
+                ok = warp_wait(&full[k_stage], k_phase, cta_abort, p.status, ST_ISSUE);
                 if (!ok) break;
                 ptx::tcgen05_fence_after_sync();
               }
               mma_abt<DT>(pt, sQ + t * G::kTileBytes, sRing + k_stage * G::kTileBytes, id_s);
-              ptx::umma_commit(&s_full[t]);
+              mma_commit(&s_full[t]);
             }
           }
           if (!ok) break;
-          ptx::umma_commit(&empty[v_stage]);
-          if (more) ptx::umma_commit(&empty[k_stage]);
+          mma_commit(&empty[v_stage]);
+          if (more) mma_commit(&empty[k_stage]);
         }
       }
     }
@@ -286,18 +286,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
           float s[128];
-  #pragma unroll
+#pragma unroll
           for (int q = 0; q < 4; ++q) tmem_ld32(ts + q * 32, s + q * 32);
           tmem_wait_ld();
           if (j * kTile + kTile - 1 > safe) {
             const int last = lim - j * kTile;
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 128; ++e) s[e] = e <= last ? s[e] : -INFINITY;
           }
           float mx[4] = {s[0], s[1], s[2], s[3]};
-  #pragma unroll
+#pragma unroll
           for (int e = 4; e < 128; e += 8) {
-  #pragma unroll
+#pragma unroll
             for (int q = 0; q < 4; ++q) {
               if (e + 4 + q < 128) mx[q] = fmaxf(mx[q], fmaxf(s[e + q], s[e + 4 + q]));
               else mx[q] = fmaxf(mx[q], s[e + q]);
@@ -305,7 +305,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           }
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (j == 0) {
-            m = top;
+            m = fmaxf(top, -1e30f);  // finite, should a whole block score -inf
           } else {
             const bool grow = (top - m) * c > kLazyMax;
             if (__any_sync(0xffffffffu, grow)) {
@@ -318,12 +318,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
               const float alpha = ex2((m - nm) * c);
               m = nm;
               l *= alpha;
-  #pragma unroll 1
+#pragma unroll 1
               for (int q = 0; q < DT / 32; ++q) {
                 float o[32];
                 tmem_ld32(to + q * 32, o);
                 tmem_wait_ld();
-  #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] *= alpha;
                 tmem_st32(to + q * 32, o);
               }
@@ -332,10 +332,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           }
           const f32x2 c2 = pair(c, c), mc2 = pair(-m * c, -m * c);
           f32x2 sum2 = pair(0.f, 0.f);
-  #pragma unroll
+#pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t pk[16];
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 16; ++e) {
               const f32x2 x = fma2(pair(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), c2, mc2);
               const float a = ex2(lo_of(x)), b = ex2(hi_of(x));
@@ -357,16 +357,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           ptx::tcgen05_fence_after_sync();
           const float inv = 1.0f / l;
           if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
-  #pragma unroll 1
+#pragma unroll 1
           for (int q = 0; q < DT / 32; ++q) {
             float o[32];
             tmem_ld32(to + q * 32, o);
             tmem_wait_ld();
             if (row_ok) {
-  #pragma unroll
+#pragma unroll
               for (int v = 0; v < 4; ++v) {
                 uint32_t w[4];
-  #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = pack2<T>(o[v * 8 + 2 * e] * inv, o[v * 8 + 2 * e + 1] * inv);
                 if (q * 32 + v * 8 < p.d) st_global_v4(out + q * 32 + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
               }

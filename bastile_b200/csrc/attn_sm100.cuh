@@ -89,15 +89,44 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* tm, i
   for (int j = 0; j < DT / 64; ++j) tma_load_3d(dst + j * kBoxBytes, tm, j * 64, head, token, bar);
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc]; A: 128 lanes, two 16-bit K elements per 32-bit column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// The MMA warp runs these with all lanes converged and one lane elected inside the instruction
+// sequence: addresses, descriptors and predicates then stay in uniform registers, where tcgen05.mma
+// takes them from.  Issued from a one-lane branch each operand is moved there first, about 80 cycles an
+// MMA beside the math warps - more than the 64 that the MMA itself takes.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A: 16-bit in tensor memory, 128 lanes, two K elements per 32-bit column.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// Arrive on `bar` once every MMA issued so far by the elected lane is done.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "@leader tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          ptx::smem_u32(bar))
+      : "memory");
+}
+// A wait of a whole warp: all lanes leave with the same answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int32_t* status,
+                                          int code) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, cta_abort, status, code));
 }
 // 32 columns of this thread's lane; the registers are valid after tmem_wait_ld().
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -161,10 +190,11 @@ constexpr uint64_t kDescMN = ptx::make_smem_desc_hi(false, kBoxBytes);      // r
 // D[128 x 128] = A[128 x DT] B[128 x DT]^T, both from shared memory, K-major.
 template <int DT>
 __device__ __forceinline__ void mma_abt(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t idesc) {
+  const uint64_t a = ptx::smem_desc(kDescK, a_smem), b = ptx::smem_desc(kDescK, b_smem);
 #pragma unroll
   for (int k = 0; k < DT / 16; ++k) {
-    const uint32_t off = static_cast<uint32_t>((k / 4) * kBoxBytes + (k % 4) * 32);
-    ptx::umma_f16(d, ptx::smem_desc(kDescK, a_smem + off), ptx::smem_desc(kDescK, b_smem + off), idesc, k != 0);
+    const uint64_t off = static_cast<uint64_t>(((k / 4) * kBoxBytes + (k % 4) * 32) >> 4);
+    mma_ss(d, a + off, b + off, idesc, k != 0);
   }
 }
 // D[128 x DT] (+)= A[128 x 128] B[128 x DT]: A 16-bit in tensor memory with its first 64 columns of K
@@ -172,12 +202,11 @@ __device__ __forceinline__ void mma_abt(uint32_t d, uint32_t a_smem, uint32_t b_
 template <int DT>
 __device__ __forceinline__ void mma_pb(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_smem, uint32_t idesc,
                                        bool accumulate) {
+  const uint64_t b = ptx::smem_desc(kDescMN, b_smem);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t a = (k < 4 ? a_lo : a_hi) + static_cast<uint32_t>((k % 4) * 8);
-    umma_f16_ts(d, a, ptx::smem_desc(kDescMN, b_smem + static_cast<uint32_t>(k * 16 * 128)), idesc,
-                (accumulate || k != 0) ? 1u : 0u);
-  }
+  for (int k = 0; k < 8; ++k)
+    mma_ts(d, (k < 4 ? a_lo : a_hi) + static_cast<uint32_t>((k % 4) * 8), b + static_cast<uint64_t>(k * 16 * 128 / 16),
+           idesc, (accumulate || k != 0) ? 1u : 0u);
 }
 
 // Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.
