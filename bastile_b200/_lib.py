@@ -37,6 +37,16 @@ class GemmDesc(ctypes.Structure):
                 ("N1", c_int64)]
 
 
+class PolicyDesc(ctypes.Structure):
+    """``bt_policy_desc`` of include/bastile_b200.h."""
+
+    _fields_ = [(n, c_void_p) for n in ("hidden", "W", "labels", "old_logp", "adv", "ref_logp", "cu_seqlens", "logp",
+                                        "loss", "averages", "dhidden", "dweight_acc", "masked", "logits", "ws")]
+    _fields_ += [(n, c_int64) for n in ("rows", "H", "V", "ld_hidden", "chunk", "n_seq", "ignore_index")]
+    _fields_ += [(n, c_float) for n in ("clip_low", "clip_high", "kl_coef")]
+    _fields_ += [("want_dweight", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 I64x3 = c_int64 * 3
 I64x2 = c_int64 * 2
 
@@ -95,15 +105,11 @@ SIGNATURES = {
                     [c_float, c_int, c_void_p, c_void_p]),
     "bt_attn_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
                     [c_float, c_int, c_void_p, c_void_p]),
-    "bt_logp_stats": (c_int, [c_void_p] * 6 + [c_int64] * 6 + [c_int, c_void_p, c_void_p]),
-    "bt_logp_rows": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_void_p, c_void_p]),
-    "bt_logp_coef": (c_int, [c_void_p] * 2 + [c_int64] * 3 + [c_void_p] * 3),
-    "bt_logp_dlogits": (c_int, [c_void_p] * 6 + [c_int64] * 5 + [c_int, c_void_p, c_void_p]),
-    "bt_logp_mask_rows": (c_int, [c_void_p] * 3 + [c_int64] * 5 + [c_int, c_void_p]),
-    "bt_policy_weights": (c_int, [c_void_p, c_int64, c_void_p] + [c_int64] * 3 + [c_void_p] * 4),
-    "bt_policy_rows": (c_int, [c_void_p] * 13 + [c_int64] * 6 + [c_float] * 3 + [c_void_p]),
-    "bt_policy_dlogits": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_int, c_void_p]),
-    "bt_policy_reduce": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
+    "bt_logp_fwd_ws_floats": (c_int64, [c_int64] * 2),
+    "bt_logp_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 6 + [c_int, c_void_p, c_void_p]),
+    "bt_logp_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_void_p]),
+    "bt_policy_fwd_ws_floats": (c_int64, [c_int64] * 4),
+    "bt_policy_fwd": (c_int, [POINTER(PolicyDesc), c_void_p, c_void_p]),
     "bt_scale_cast": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),
 }
 
@@ -165,7 +171,14 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+# torch.cuda.current_stream() builds a Python object around what the first returns (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_ptr(dev: torch.device) -> int:
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
@@ -177,7 +190,7 @@ class device_of:
         self.prev = -1
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = _current_device()
         if cur != self.idx:
             self.prev = cur
             torch.cuda.set_device(self.idx)

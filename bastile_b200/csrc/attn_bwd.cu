@@ -665,9 +665,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 }
 
 template <typename K>
-int launch_bwd(K* kern, int smem, int64_t grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+int launch_bwd(K* kern, int smem, std::atomic<uint64_t>* reserved, int64_t grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                const CUtensorMap& g, const Params& p, cudaStream_t s, const char* what) {
-  BT_CHECK_LAUNCHED(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
+  BT_CHECK_LAUNCHED(reserve_smem(kern, smem, reserved), what);
   BT_CHECK_ARG(grid <= 0x7fffffffll, "%s: too many tiles (%lld)", what, (long long)grid);
   BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kBwdThreads), smem, s, q, k, v, g, p),
                     what);
@@ -677,15 +677,16 @@ int launch_bwd(K* kern, int smem, int64_t grid, const CUtensorMap& q, const CUte
 template <typename T, int DT>
 int run_bwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, Params p,
             int64_t batch, cudaStream_t s) {
+  static std::atomic<uint64_t> reserved[2];
   if (p.dk.ptr != nullptr) {
     p.gran = gran_index(kTile);
-    if (int rc = launch_bwd(attn_dkv_kernel<T, DT>, BwdGeo<DT>::kSmem, max_items(p.total, batch, kTile) * p.hk, q, k,
-                            v, g, p, s, "attn_bwd dk, dv"))
+    if (int rc = launch_bwd(attn_dkv_kernel<T, DT>, BwdGeo<DT>::kSmem, &reserved[0],
+                            max_items(p.total, batch, kTile) * p.hk, q, k, v, g, p, s, "attn_bwd dk, dv"))
       return rc;
   }
   if (p.dq.ptr != nullptr) {
     p.gran = gran_index(p.tq);
-    if (int rc = launch_bwd(attn_dq_kernel<T, DT>, BwdGeo<DT>::kSmem,
+    if (int rc = launch_bwd(attn_dq_kernel<T, DT>, BwdGeo<DT>::kSmem, &reserved[1],
                             max_items(p.total, batch, p.tq) * p.hk * p.nsub, q, k, v, g, p, s, "attn_bwd dq"))
       return rc;
   }

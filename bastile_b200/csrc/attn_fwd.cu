@@ -388,9 +388,8 @@ template <typename T, int DT>
 int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int64_t batch,
                cudaStream_t s) {
   auto* kern = attn_fwd_kernel<T, DT>;
-  // per device and cheap: the attribute belongs to the current device's copy of the kernel
-  BT_CHECK_LAUNCHED(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdGeo<DT>::kSmem),
-                    "attn_fwd: shared memory");
+  static std::atomic<uint64_t> reserved{0};
+  BT_CHECK_LAUNCHED(reserve_smem(kern, FwdGeo<DT>::kSmem, &reserved), "attn_fwd: shared memory");
   const int64_t grid = max_items(p.total, batch, 2 * p.tq) * p.hk * p.nsub;
   BT_CHECK_ARG(grid <= 0x7fffffffll, "attn_fwd: too many tiles (%lld)", (long long)grid);
   BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdGeo<DT>::kSmem, s,

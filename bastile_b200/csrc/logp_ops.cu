@@ -17,13 +17,6 @@ bool rows_aligned(const void* p, int64_t ld, int elem_bytes) {
 }
 bool known(int dtype) { return dtype == BT_BF16 || dtype == BT_FP16 || dtype == BT_FP32; }
 int esize(int dtype) { return dtype == BT_FP32 ? 4 : 2; }
-int check_sizes(const char* what, int64_t rows, int64_t h, int64_t v, int dtype) {
-  BT_CHECK_ARG(known(dtype), "%s: unknown dtype %d", what, dtype);
-  BT_CHECK_ARG(rows >= 0 && rows <= 0x7fffffffll && h > 0 && h <= 0x7fffffffll && v > 0 && v <= 0x7fffffffll,
-               "%s: bad extents rows=%lld H=%lld V=%lld", what, (long long)rows, (long long)h, (long long)v);
-  return BT_OK;
-}
-
 __device__ __forceinline__ bool counted(int64_t label, int64_t ignore_index, int64_t vocab) {
   return label != ignore_index && label >= 0 && label < vocab;
 }
@@ -240,9 +233,10 @@ policy_rows_kernel(const PolicyArgs a) {
   }
 }
 
-// out[0..2] = sums of the three rows of terms (fp64, fixed order).
+// loss, averages[0..1] = sums of the three rows of terms (fp64, fixed order).
 __global__ void __launch_bounds__(1024)
-policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restrict__ out) {
+policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restrict__ loss,
+                     float* __restrict__ averages) {
   grid_dependency_wait();
   __shared__ double s_sum[32];
   const float* t = terms + blockIdx.x * n;
@@ -255,7 +249,7 @@ policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restri
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int i = 0; i < 32; ++i) s += s_sum[i];
-    out[blockIdx.x] = static_cast<float>(s);
+    (blockIdx.x == 0 ? loss : averages + (blockIdx.x - 1))[0] = static_cast<float>(s);
   }
 }
 
@@ -305,20 +299,115 @@ unsigned grid_for(int64_t blocks, int per_sm) {
   return static_cast<unsigned>(blocks < 1 ? 1 : (blocks < cap ? blocks : cap));
 }
 
-gemm::Launch head_product(const void* hidden, const void* W, const int64_t* labels, int64_t rows, int64_t H, int64_t V,
-                          int64_t ld_hidden, int64_t ignore_index, int dtype, int32_t* status) {
+// What the steps below share: one call's sizes, types and stream.
+struct Head {
+  const void* W;
+  int64_t H, V, ld_logits, ignore_index;
+  int dtype, n_vt;
+  int32_t* status;
+  cudaStream_t s;
+};
+
+gemm::Launch head_product(const Head& h, const void* hidden, const int64_t* labels, int64_t rows, int64_t ld_hidden) {
   gemm::Launch L;
-  L.dtype = dtype;
-  L.a0.ptr = hidden, L.a0.kmajor = 1, L.a0.mn = rows, L.a0.k = H, L.a0.ld = ld_hidden;
-  L.b0.ptr = W, L.b0.kmajor = 1, L.b0.mn = V, L.b0.k = H, L.b0.ld = H;
+  L.dtype = h.dtype;
+  L.a0.ptr = hidden, L.a0.kmajor = 1, L.a0.mn = rows, L.a0.k = h.H, L.a0.ld = ld_hidden;
+  L.b0.ptr = h.W, L.b0.kmajor = 1, L.b0.mn = h.V, L.b0.k = h.H, L.b0.ld = h.H;
   L.p.M = static_cast<int>(rows);
-  L.p.N = static_cast<int>(V);
-  L.p.status = status;
+  L.p.N = static_cast<int>(h.V);
+  L.p.status = h.status;
   L.p.labels = labels;
-  L.p.ignore_index = ignore_index;
-  L.p.n_vtiles = static_cast<int>(bt_lce_num_vtiles(V));
+  L.p.ignore_index = h.ignore_index;
+  L.p.n_vtiles = h.n_vt;
   return L;
 }
+
+// Statistics (and, unless NULL, shifted logits) of one chunk.
+int stats(const Head& h, const void* hidden, const int64_t* labels, void* logits, float* tile_stats, float* tgt,
+          int64_t rows, int64_t ld_hidden) {
+  gemm::Launch L = head_product(h, hidden, labels, rows, ld_hidden);
+  L.p.tile_stats = tile_stats;
+  L.p.tgt_logit = tgt;
+  if (logits == nullptr) return gemm::launch<gemm::EPI_LOGP>(L, h.s);
+  L.p.out = logits;
+  L.p.ldo = h.ld_logits;
+  L.p.vec_ok = rows_aligned(logits, h.ld_logits, esize(h.dtype));
+  return gemm::launch<gemm::EPI_LOGP_SHIFT>(L, h.s);
+}
+
+int mask_rows(const Head& h, const void* x, void* y, const int64_t* labels, int64_t rows, int64_t ld) {
+  const dim3 grid(grid_for(rows, 8)), block(kThreads);
+  const cudaError_t e =
+      h.dtype == BT_FP32
+          ? launch_dependent(logp_mask_rows_kernel<float>, grid, block, 0, h.s, static_cast<const float*>(x),
+                             static_cast<float*>(y), labels, rows, h.H, ld, h.ignore_index, h.V)
+          // a copy: the two 16-bit types are the same
+          : launch_dependent(logp_mask_rows_kernel<__half>, grid, block, 0, h.s, static_cast<const __half*>(x),
+                             static_cast<__half*>(y), labels, rows, h.H, ld, h.ignore_index, h.V);
+  BT_CHECK_LAUNCHED(e, "logp: copy of the counted rows");
+  return BT_OK;
+}
+
+// d hidden[rows, H] = alpha dlogits[rows, V] W[V, H]
+int dhidden(const Head& h, const void* dlogits, void* out, int64_t rows, int out_dtype, const float* alpha) {
+  return bt_gemm(dlogits, h.W, out, rows, h.H, h.V, h.ld_logits, h.H, h.H, 1, 0, h.dtype, out_dtype, nullptr, 0, alpha,
+                 h.status, h.s);
+}
+// out[V, H] = alpha (dlogits^T x + addend), x dense
+int dweight(const Head& h, const void* dlogits, const void* x, void* out, int64_t rows, int out_dtype,
+            const float* addend, const float* alpha) {
+  return bt_gemm(dlogits, x, out, h.V, h.H, rows, h.ld_logits, h.H, h.H, 0, 0, h.dtype, out_dtype, addend, h.H, alpha,
+                 h.status, h.s);
+}
+
+int policy_dlogits(const Head& h, void* logits, const float* tile_stats, const float* lse, const int64_t* labels,
+                   const float* coef, int64_t rows) {
+  const int64_t vec = 16 / esize(h.dtype);
+  // enough CTAs for ~8 per SM: rows are split into column segments when there are few
+  const int sms = sm_count();
+  int64_t gx = rows < static_cast<int64_t>(sms) * 8 ? rows : static_cast<int64_t>(sms) * 8;
+  int64_t gy = 1;
+  const int64_t nvec = (h.V + vec - 1) / vec;
+  while (gx * gy < static_cast<int64_t>(sms) * 4 && gy * 2 * kThreads <= nvec) gy *= 2;
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(kThreads);
+  const float2* ts = reinterpret_cast<const float2*>(tile_stats);
+  cudaError_t e;
+  if (h.dtype == BT_BF16)
+    e = launch_dependent(policy_dlogits_kernel<__nv_bfloat16>, grid, block, 0, h.s, static_cast<__nv_bfloat16*>(logits),
+                         ts, lse, labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+  else if (h.dtype == BT_FP16)
+    e = launch_dependent(policy_dlogits_kernel<__half>, grid, block, 0, h.s, static_cast<__half*>(logits), ts, lse,
+                         labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+  else
+    e = launch_dependent(policy_dlogits_kernel<float>, grid, block, 0, h.s, static_cast<float*>(logits), ts, lse,
+                         labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+  BT_CHECK_LAUNCHED(e, "policy: dlogits");
+  return BT_OK;
+}
+
+int fill_head(Head* h, const char* what, const void* W, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
+              const void* hidden, int64_t chunk, int64_t ignore_index, int dtype, int32_t* status, void* stream) {
+  BT_CHECK_ARG(known(dtype), "%s: unknown dtype %d", what, dtype);
+  BT_CHECK_ARG(rows >= 0 && rows <= 0x7fffffffll && H > 0 && H <= 0x7fffffffll && V > 0 && V <= 0x7fffffffll,
+               "%s: bad extents rows=%lld H=%lld V=%lld", what, (long long)rows, (long long)H, (long long)V);
+  BT_CHECK_ARG(chunk > 0, "%s: chunk must be positive", what);
+  BT_CHECK_ARG(rows == 0 || (hidden != nullptr && W != nullptr), "%s: null pointer", what);
+  BT_CHECK_ARG(rows == 0 || (rows_aligned(hidden, rows > 1 ? ld_hidden : H, esize(dtype)) &&
+                             rows_aligned(W, H, esize(dtype)) && (rows == 1 || ld_hidden >= H)),
+               "%s: rows must be 16-byte aligned", what);
+  h->W = W, h->H = H, h->V = V, h->ignore_index = ignore_index;
+  h->ld_logits = (V + 7) / 8 * 8;
+  h->dtype = dtype;
+  h->n_vt = static_cast<int>(bt_lce_num_vtiles(V));
+  h->status = status;
+  h->s = static_cast<cudaStream_t>(stream);
+  return BT_OK;
+}
+
+const char* row_ptr(const void* base, int64_t row, int64_t ld, int dtype) {
+  return static_cast<const char*>(base) + row * ld * esize(dtype);
+}
+int64_t even(int64_t n) { return (n + 1) / 2 * 2; }  // pairs of floats are read as float2
 
 }  // namespace
 }  // namespace bt
@@ -327,163 +416,144 @@ int bt_internal_set_wait_limit_logp(unsigned long long ns) {
   return bt::ptx::set_wait_limit_ns(ns) == cudaSuccess ? 0 : -1;
 }
 
-extern "C" int bt_logp_stats(const void* hidden, const void* W, const int64_t* labels, void* logits, float* tile_stats,
-                             float* tgt_logit, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t ld_logits,
-                             int64_t ignore_index, int dtype, int32_t* status, void* stream) {
-  using namespace bt;
-  if (int rc = check_sizes("logp_stats", rows, H, V, dtype)) return rc;
-  if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(hidden && W && labels && tile_stats && tgt_logit, "logp_stats: null pointer");
-  BT_CHECK_ARG(logits == nullptr || ld_logits >= V, "logp_stats: logits stride smaller than V");
-  gemm::Launch L = head_product(hidden, W, labels, rows, H, V, ld_hidden, ignore_index, dtype, status);
-  L.p.tile_stats = tile_stats;
-  L.p.tgt_logit = tgt_logit;
-  if (logits == nullptr) return gemm::launch<gemm::EPI_LOGP>(L, static_cast<cudaStream_t>(stream));
-  L.p.out = logits;
-  L.p.ldo = ld_logits;
-  L.p.vec_ok = rows_aligned(logits, ld_logits, esize(dtype));
-  return gemm::launch<gemm::EPI_LOGP_SHIFT>(L, static_cast<cudaStream_t>(stream));
+extern "C" int64_t bt_logp_fwd_ws_floats(int64_t chunk, int64_t V) {
+  if (chunk < 0 || V <= 0) return 0;
+  return chunk * bt_lce_num_vtiles(V) * 2 + chunk;
 }
 
-extern "C" int bt_logp_dlogits(const void* hidden, const void* W, const int64_t* labels, const float* lse,
-                               const float* coef, void* dlogits, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
-                               int64_t ld_dlogits, int dtype, int32_t* status, void* stream) {
+extern "C" int bt_logp_fwd(const void* hidden, const void* W, const int64_t* labels, float* logp, float* lse, float* ws,
+                           int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index,
+                           int dtype, int32_t* status, void* stream) {
   using namespace bt;
-  if (int rc = check_sizes("logp_dlogits", rows, H, V, dtype)) return rc;
+  Head h;
+  if (int rc = fill_head(&h, "logp_fwd", W, rows, H, V, ld_hidden, hidden, chunk, ignore_index, dtype, status, stream))
+    return rc;
   if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(hidden && W && labels && lse && coef && dlogits, "logp_dlogits: null pointer");
-  BT_CHECK_ARG(ld_dlogits >= V, "logp_dlogits: dlogits stride smaller than V");
-  gemm::Launch L = head_product(hidden, W, labels, rows, H, V, ld_hidden, 0, dtype, status);
-  L.p.row_lse = lse;
-  L.p.row_coef = coef;
-  L.p.out = dlogits;
-  L.p.ldo = ld_dlogits;
-  L.p.vec_ok = rows_aligned(dlogits, ld_dlogits, esize(dtype));
-  return gemm::launch<gemm::EPI_DLOGITS>(L, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int bt_logp_rows(const float* tile_stats, const float* tgt_logit, const int64_t* labels, float* logp,
-                            float* lse, int64_t rows, int64_t V, int64_t ignore_index, int32_t* status, void* stream) {
-  using namespace bt;
-  if (int rc = check_sizes("logp_rows", rows, 1, V, BT_BF16)) return rc;
-  if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(tile_stats && tgt_logit && labels && logp, "logp_rows: null pointer");
-  BT_CHECK_LAUNCHED(launch_dependent(logp_rows_kernel, dim3(grid_for(ceil_div(rows, kThreads / 32), 8)), dim3(kThreads),
-                                     0, static_cast<cudaStream_t>(stream), reinterpret_cast<const float2*>(tile_stats),
-                                     tgt_logit, labels, logp, lse, rows, static_cast<int>(bt_lce_num_vtiles(V)),
-                                     ignore_index, V, status),
-                    "logp_rows");
+  BT_CHECK_ARG(labels && logp && ws, "logp_fwd: null pointer");
+  float* tile_stats = ws;
+  float* tgt = ws + chunk * h.n_vt * 2;
+  for (int64_t r = 0; r < rows; r += chunk) {
+    const int64_t n = rows - r < chunk ? rows - r : chunk;
+    if (int rc = stats(h, row_ptr(hidden, r, ld_hidden, dtype), labels + r, nullptr, tile_stats, tgt, n, ld_hidden))
+      return rc;
+    BT_CHECK_LAUNCHED(launch_dependent(logp_rows_kernel, dim3(grid_for(ceil_div(n, kThreads / 32), 8)), dim3(kThreads),
+                                       0, h.s, reinterpret_cast<const float2*>(tile_stats), tgt, labels + r, logp + r,
+                                       lse != nullptr ? lse + r : nullptr, n, h.n_vt, ignore_index, V, status),
+                      "logp_fwd: rows");
+  }
   return BT_OK;
 }
 
-extern "C" int bt_logp_coef(const float* dlogp, const int64_t* labels, int64_t n, int64_t V, int64_t ignore_index,
-                            float* coef, float* scal, void* stream) {
+extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels,
+                           const float* lse, void* masked, void* dlogits, void* dhidden_out, void* dweight_out,
+                           float* dweight_acc, float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
+                           int64_t chunk, int64_t ignore_index, int dtype, int dweight_dtype, int32_t* status,
+                           void* stream) {
   using namespace bt;
-  if (int rc = check_sizes("logp_coef", n, 1, V, BT_BF16)) return rc;
-  BT_CHECK_ARG(scal && (n == 0 || (dlogp && labels && coef)), "logp_coef: null pointer");
-  BT_CHECK_LAUNCHED(launch_dependent(logp_coef_kernel, dim3(1), dim3(1024), 0, static_cast<cudaStream_t>(stream), dlogp,
-                                     labels, n, ignore_index, V, coef, scal),
-                    "logp_coef");
-  return BT_OK;
-}
-
-extern "C" int bt_logp_mask_rows(const void* x, void* y, const int64_t* labels, int64_t rows, int64_t H, int64_t ld,
-                                 int64_t V, int64_t ignore_index, int dtype, void* stream) {
-  using namespace bt;
-  if (int rc = check_sizes("logp_mask_rows", rows, H, V, dtype)) return rc;
+  Head h;
+  if (int rc = fill_head(&h, "logp_bwd", W, rows, H, V, ld_hidden, hidden, chunk, ignore_index, dtype, status, stream))
+    return rc;
   if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(x && y && labels, "logp_mask_rows: null pointer");
-  BT_CHECK_ARG(rows_aligned(x, ld, esize(dtype)) && rows_aligned(y, H, esize(dtype)) && (rows == 1 || ld >= H),
-               "logp_mask_rows: rows must be 16-byte aligned");
-  const dim3 grid(grid_for(rows, 8)), block(kThreads);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == BT_FP32)
-    BT_CHECK_LAUNCHED(launch_dependent(logp_mask_rows_kernel<float>, grid, block, 0, s, static_cast<const float*>(x),
-                                       static_cast<float*>(y), labels, rows, H, ld, ignore_index, V),
-                      "logp_mask_rows");
-  else  // a copy: the two 16-bit types are the same
-    BT_CHECK_LAUNCHED(launch_dependent(logp_mask_rows_kernel<__half>, grid, block, 0, s, static_cast<const __half*>(x),
-                                       static_cast<__half*>(y), labels, rows, H, ld, ignore_index, V),
-                      "logp_mask_rows");
+  BT_CHECK_ARG(dlogp && labels && lse && masked && dlogits && ws, "logp_bwd: null pointer");
+  BT_CHECK_ARG(aligned16(masked) && aligned16(dlogits), "logp_bwd: buffers must be 16-byte aligned");
+  BT_CHECK_ARG(dweight_out == nullptr || rows <= chunk || dweight_acc != nullptr,
+               "logp_bwd: more than one chunk needs an accumulator for the weight gradient");
+  float* scal = ws;  // [1 + rows]: scale back, coefficients
+  float* coef = ws + 1;
+  BT_CHECK_LAUNCHED(launch_dependent(logp_coef_kernel, dim3(1), dim3(1024), 0, h.s, dlogp, labels, rows, ignore_index,
+                                     V, coef, scal),
+                    "logp_bwd: coefficients");
+  if (int rc = mask_rows(h, hidden, masked, labels, rows, rows > 1 ? ld_hidden : H)) return rc;
+  for (int64_t r = 0; r < rows; r += chunk) {
+    const int64_t n = rows - r < chunk ? rows - r : chunk;
+    const char* x = row_ptr(masked, r, H, dtype);
+    gemm::Launch L = head_product(h, x, labels + r, n, H);
+    L.p.row_lse = lse + r;
+    L.p.row_coef = coef + r;
+    L.p.out = dlogits;
+    L.p.ldo = h.ld_logits;
+    L.p.vec_ok = rows_aligned(dlogits, h.ld_logits, esize(dtype));
+    if (int rc = gemm::launch<gemm::EPI_DLOGITS>(L, h.s)) return rc;
+    if (dhidden_out != nullptr) {
+      if (int rc = dhidden(h, dlogits, const_cast<char*>(row_ptr(dhidden_out, r, H, dtype)), n, dtype, scal)) return rc;
+    }
+    if (dweight_out != nullptr) {
+      const bool last = r + n == rows;
+      if (int rc = dweight(h, dlogits, x, last ? dweight_out : dweight_acc, n, last ? dweight_dtype : BT_FP32,
+                           r > 0 ? dweight_acc : nullptr, last ? scal : nullptr))
+        return rc;
+    }
+  }
   return BT_OK;
 }
 
-extern "C" int bt_policy_weights(const int64_t* labels, int64_t n, const int32_t* cu_seqlens, int64_t n_seq, int64_t V,
-                                 int64_t ignore_index, float* weights, float* scal, int32_t* status, void* stream) {
+extern "C" int64_t bt_policy_fwd_ws_floats(int64_t rows, int64_t chunk, int64_t n_seq, int64_t V) {
+  if (rows < 0 || chunk < 0 || n_seq < 0 || V <= 0) return 0;
+  return bt::even(2 + n_seq + 3 * rows + 3 * chunk) + chunk * bt_lce_num_vtiles(V) * 2;
+}
+
+extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* stream) {
   using namespace bt;
-  if (int rc = check_sizes("policy_weights", n, 1, V, BT_BF16)) return rc;
-  BT_CHECK_ARG(n_seq >= 0 && n_seq < (1 << 24) && (cu_seqlens != nullptr || n_seq == 1), "policy_weights: bad sequence count");
-  BT_CHECK_ARG(weights && scal && (n == 0 || labels), "policy_weights: null pointer");
-  BT_CHECK_LAUNCHED(launch_dependent(policy_weights_kernel, dim3(1), dim3(1024), 0, static_cast<cudaStream_t>(stream),
-                                     labels, n, cu_seqlens, static_cast<int>(n_seq), ignore_index, V, weights, scal,
+  BT_CHECK_ARG(d != nullptr, "policy_fwd: null descriptor");
+  Head h;
+  if (int rc = fill_head(&h, "policy_fwd", d->W, d->rows, d->H, d->V, d->ld_hidden, d->hidden, d->chunk,
+                         d->ignore_index, d->dtype, status, stream))
+    return rc;
+  BT_CHECK_ARG(d->n_seq >= 0 && d->n_seq < (1 << 24) && (d->cu_seqlens != nullptr || d->n_seq == 1),
+               "policy_fwd: bad sequence count");
+  BT_CHECK_ARG(d->ws && d->loss && d->averages, "policy_fwd: null pointer");
+  const bool grad = d->dhidden != nullptr || d->want_dweight != 0;
+  if (d->rows > 0) {
+    BT_CHECK_ARG(d->labels && d->old_logp && d->adv && d->logp, "policy_fwd: null pointer");
+    BT_CHECK_ARG(!grad || (d->masked && d->logits && aligned16(d->masked) && aligned16(d->logits)),
+                 "policy_fwd: gradients need 16-byte aligned buffers for the counted rows and the logits");
+    BT_CHECK_ARG(!d->want_dweight || d->rows <= d->chunk || d->dweight_acc != nullptr,
+                 "policy_fwd: more than one chunk needs an accumulator for the weight gradient");
+  }
+  float* scal = d->ws;
+  float* weights = scal + 2;
+  float* terms = weights + d->n_seq;
+  float* lse = terms + 3 * d->rows;
+  float* coef = lse + d->chunk;
+  float* tgt = coef + d->chunk;
+  float* tile_stats = d->ws + even(2 + d->n_seq + 3 * d->rows + 3 * d->chunk);
+  BT_CHECK_LAUNCHED(launch_dependent(policy_weights_kernel, dim3(1), dim3(1024), 0, h.s, d->labels, d->rows,
+                                     d->cu_seqlens, static_cast<int>(d->n_seq), d->ignore_index, d->V, weights, scal,
                                      status),
-                    "policy_weights");
-  return BT_OK;
-}
-
-extern "C" int bt_policy_rows(const float* tile_stats, const float* tgt_logit, const int64_t* labels,
-                              const float* old_logp, const float* adv, const float* ref_logp, const int32_t* cu_seqlens,
-                              const float* weights, const float* scal, float* logp, float* lse, float* coef,
-                              float* terms, int64_t rows, int64_t row0, int64_t total, int64_t n_seq, int64_t V,
-                              int64_t ignore_index, float clip_low, float clip_high, float kl_coef, void* stream) {
-  using namespace bt;
-  if (int rc = check_sizes("policy_rows", total, 1, V, BT_BF16)) return rc;
-  BT_CHECK_ARG(rows >= 0 && row0 >= 0 && row0 + rows <= total, "policy_rows: chunk outside the batch");
-  BT_CHECK_ARG(n_seq >= 0 && n_seq < (1 << 24) && (cu_seqlens != nullptr || n_seq == 1), "policy_rows: bad sequence count");
-  if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(tile_stats && tgt_logit && labels && old_logp && adv && weights && scal && logp && lse && coef && terms,
-               "policy_rows: null pointer");
-  PolicyArgs a{};
-  a.tile_stats = reinterpret_cast<const float2*>(tile_stats);
-  a.tgt_logit = tgt_logit, a.labels = labels, a.old_logp = old_logp, a.adv = adv, a.ref_logp = ref_logp;
-  a.cu = cu_seqlens, a.weights = weights, a.scal = scal, a.logp = logp, a.lse = lse, a.coef = coef, a.terms = terms;
-  a.rows = rows, a.row0 = row0, a.total = total, a.ignore_index = ignore_index, a.vocab = V;
-  a.n_vt = static_cast<int>(bt_lce_num_vtiles(V)), a.n_seq = static_cast<int>(n_seq);
-  a.clip_low = clip_low, a.clip_high = clip_high, a.kl_coef = kl_coef;
-  BT_CHECK_LAUNCHED(launch_dependent(policy_rows_kernel, dim3(grid_for(ceil_div(rows, kThreads / 32), 8)),
-                                     dim3(kThreads), 0, static_cast<cudaStream_t>(stream), a),
-                    "policy_rows");
-  return BT_OK;
-}
-
-extern "C" int bt_policy_dlogits(void* logits, const float* tile_stats, const float* lse, const int64_t* labels,
-                                 const float* coef, int64_t rows, int64_t V, int64_t ld_logits, int dtype,
-                                 void* stream) {
-  using namespace bt;
-  if (int rc = check_sizes("policy_dlogits", rows, 1, V, dtype)) return rc;
-  if (rows == 0) return BT_OK;
-  BT_CHECK_ARG(logits && tile_stats && lse && labels && coef, "policy_dlogits: null pointer");
-  const int64_t vec = 16 / esize(dtype);
-  BT_CHECK_ARG(rows_aligned(logits, ld_logits, esize(dtype)) && ld_logits >= (V + vec - 1) / vec * vec,
-               "policy_dlogits: logits rows must be 16-byte aligned and padded to whole 16-byte vectors");
-  const int sms = sm_count();
-  int64_t gx = rows < static_cast<int64_t>(sms) * 8 ? rows : static_cast<int64_t>(sms) * 8;
-  int64_t gy = 1;
-  const int64_t nvec = (V + vec - 1) / vec;
-  while (gx * gy < static_cast<int64_t>(sms) * 4 && gy * 2 * kThreads <= nvec) gy *= 2;
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(kThreads);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const float2* ts = reinterpret_cast<const float2*>(tile_stats);
-  const int n_vt = static_cast<int>(bt_lce_num_vtiles(V));
-  cudaError_t e;
-  if (dtype == BT_BF16)
-    e = launch_dependent(policy_dlogits_kernel<__nv_bfloat16>, grid, block, 0, s, static_cast<__nv_bfloat16*>(logits),
-                         ts, lse, labels, coef, rows, V, ld_logits, n_vt);
-  else if (dtype == BT_FP16)
-    e = launch_dependent(policy_dlogits_kernel<__half>, grid, block, 0, s, static_cast<__half*>(logits), ts, lse,
-                         labels, coef, rows, V, ld_logits, n_vt);
-  else
-    e = launch_dependent(policy_dlogits_kernel<float>, grid, block, 0, s, static_cast<float*>(logits), ts, lse, labels,
-                         coef, rows, V, ld_logits, n_vt);
-  BT_CHECK_LAUNCHED(e, "policy_dlogits");
-  return BT_OK;
-}
-
-extern "C" int bt_policy_reduce(const float* terms, int64_t n, float* out, void* stream) {
-  using namespace bt;
-  BT_CHECK_ARG(n >= 0 && out && (n == 0 || terms), "policy_reduce: bad args");
-  BT_CHECK_LAUNCHED(launch_dependent(policy_reduce_kernel, dim3(3), dim3(1024), 0, static_cast<cudaStream_t>(stream),
-                                     terms, n, out),
-                    "policy_reduce");
+                    "policy_fwd: weights");
+  const void* x = d->hidden;
+  int64_t ld_x = d->ld_hidden;
+  if (grad && d->rows > 0) {
+    if (int rc = mask_rows(h, d->hidden, d->masked, d->labels, d->rows, d->rows > 1 ? d->ld_hidden : d->H)) return rc;
+    x = d->masked;
+    ld_x = d->H;
+  }
+  for (int64_t r = 0; r < d->rows; r += d->chunk) {
+    const int64_t n = d->rows - r < d->chunk ? d->rows - r : d->chunk;
+    const char* xc = row_ptr(x, r, ld_x, d->dtype);
+    if (int rc = stats(h, xc, d->labels + r, grad ? d->logits : nullptr, tile_stats, tgt, n, ld_x)) return rc;
+    PolicyArgs a{};
+    a.tile_stats = reinterpret_cast<const float2*>(tile_stats);
+    a.tgt_logit = tgt, a.labels = d->labels + r, a.old_logp = d->old_logp, a.adv = d->adv, a.ref_logp = d->ref_logp;
+    a.cu = d->cu_seqlens, a.weights = weights, a.scal = scal, a.logp = d->logp + r, a.lse = lse, a.coef = coef;
+    a.terms = terms, a.rows = n, a.row0 = r, a.total = d->rows, a.ignore_index = d->ignore_index, a.vocab = d->V;
+    a.n_vt = h.n_vt, a.n_seq = static_cast<int>(d->n_seq);
+    a.clip_low = d->clip_low, a.clip_high = d->clip_high, a.kl_coef = d->kl_coef;
+    BT_CHECK_LAUNCHED(launch_dependent(policy_rows_kernel, dim3(grid_for(ceil_div(n, kThreads / 32), 8)),
+                                       dim3(kThreads), 0, h.s, a),
+                      "policy_fwd: rows");
+    if (!grad) continue;
+    if (int rc = policy_dlogits(h, d->logits, tile_stats, lse, d->labels + r, coef, n)) return rc;
+    if (d->dhidden != nullptr) {
+      if (int rc = dhidden(h, d->logits, d->dhidden + r * d->H, n, BT_FP32, nullptr)) return rc;
+    }
+    if (d->want_dweight && r + n < d->rows) {  // the last chunk's product waits for the upstream gradient
+      if (int rc = dweight(h, d->logits, xc, d->dweight_acc, n, BT_FP32, r > 0 ? d->dweight_acc : nullptr, nullptr))
+        return rc;
+    }
+  }
+  BT_CHECK_LAUNCHED(launch_dependent(policy_reduce_kernel, dim3(3), dim3(1024), 0, h.s, terms, d->rows, d->loss,
+                                     d->averages),
+                    "policy_fwd: sums");
   return BT_OK;
 }

@@ -19,6 +19,7 @@ post-training needs, built the same way: ``[tokens, vocab]`` logits exist one ch
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -81,6 +82,10 @@ def _ld(x2: Tensor) -> int:
     return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
 
 
+def _ld_logits(vocab: int) -> int:
+    return (vocab + 7) // 8 * 8  # whole 16-byte vectors
+
+
 def _chunk_rows(chunk_size: int, rows: int, ld_logits: int) -> int:
     """The rule of fused_linear_cross_entropy: the default may grow to AUTO_CHUNK_ROWS rows."""
     want = int(chunk_size)
@@ -89,205 +94,152 @@ def _chunk_rows(chunk_size: int, rows: int, ld_logits: int) -> int:
     return max(1, min(want, rows))
 
 
-class _Head:
-    """One call's view of the C entry points: device, stream, sizes and types filled in."""
+def _f32(dev, *shape) -> Tensor:
+    return torch.empty(shape, dtype=torch.float32, device=dev)
 
-    def __init__(self, x: Tensor, w: Tensor, ignore_index: int):
-        self.lib, self.dev = _lib.get_lib(), x.device
-        self.stream = _lib.stream_ptr(self.dev)
-        self.st = _lib.status_word(self.dev)
-        self.code = _lib.dtype_code(x.dtype)
-        self.w, self.hdim, self.vocab = w, w.shape[1], w.shape[0]
-        self.ignore = int(ignore_index)
-        self.ld = (self.vocab + 7) // 8 * 8
-        self.n_vt = int(self.lib.bt_lce_num_vtiles(self.vocab))
 
-    def f32(self, *shape) -> Tensor:
-        return torch.empty(shape, dtype=torch.float32, device=self.dev)
+def _dweight_out(w: Tensor, w_dtype) -> Tensor:
+    """The weight gradient's buffer: a registered destination if there is one."""
+    out_dtype = w_dtype if w_dtype in (w.dtype, torch.float32) else w.dtype
+    out = _lib.grad_sink(w, out_dtype) if w.dtype == w_dtype else None
+    return out if out is not None else torch.empty(w.shape, dtype=out_dtype, device=w.device)
 
-    def stats(self, xc, labels, logits, tile_stats, tgt) -> None:
-        _lib.check(self.lib.bt_logp_stats(xc.data_ptr(), self.w.data_ptr(), labels.data_ptr(),
-                                          logits.data_ptr() if logits is not None else None, tile_stats.data_ptr(),
-                                          tgt.data_ptr(), xc.shape[0], self.hdim, self.vocab, _ld(xc), self.ld,
-                                          self.ignore, self.code, self.st.data_ptr(), self.stream), "bt_logp_stats")
 
-    def mask_rows(self, x2, labels) -> Tensor:
-        out = torch.empty(x2.shape, dtype=x2.dtype, device=self.dev)
-        _lib.check(self.lib.bt_logp_mask_rows(x2.data_ptr(), out.data_ptr(), labels.data_ptr(), x2.shape[0], self.hdim,
-                                              _ld(x2), self.vocab, self.ignore, self.code, self.stream),
-                   "bt_logp_mask_rows")
-        return out
-
-    def dhidden(self, dlogits, rows, out, alpha) -> None:
-        """out[rows, H] = alpha dlogits[rows, V] W[V, H]"""
-        _lib.check(self.lib.bt_gemm(dlogits.data_ptr(), self.w.data_ptr(), out.data_ptr(), rows, self.hdim, self.vocab,
-                                    self.ld, self.hdim, self.hdim, 1, 0, self.code, _lib.dtype_code(out.dtype), None,
-                                    0, alpha.data_ptr() if alpha is not None else None, self.st.data_ptr(),
-                                    self.stream), "bt_gemm(dhidden)")
-
-    def dweight(self, dlogits, xc, out, addend, alpha) -> None:
-        """out[V, H] = alpha (dlogits^T x + addend)"""
-        _lib.check(self.lib.bt_gemm(dlogits.data_ptr(), xc.data_ptr(), out.data_ptr(), self.vocab, self.hdim,
-                                    xc.shape[0], self.ld, _ld(xc), self.hdim, 0, 0, self.code,
-                                    _lib.dtype_code(out.dtype), addend.data_ptr() if addend is not None else None,
-                                    self.hdim, alpha.data_ptr() if alpha is not None else None, self.st.data_ptr(),
-                                    self.stream), "bt_gemm(dweight)")
-
-    def dweight_out(self, w_dtype) -> Tensor:
-        """The weight gradient's buffer: a registered destination if there is one."""
-        out_dtype = w_dtype if w_dtype in (self.w.dtype, torch.float32) else self.w.dtype
-        out = _lib.grad_sink(self.w, out_dtype) if self.w.dtype == w_dtype else None
-        return out if out is not None else torch.empty((self.vocab, self.hdim), dtype=out_dtype, device=self.dev)
+def _log_probs(hidden, weight, target, ignore_index: int, chunk_size: int, keep: bool):
+    """(log-probabilities, what the backward needs if ``keep``)."""
+    lib = _lib.get_lib()
+    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
+    dev, rows = x.device, x.shape[0]
+    vocab, hdim = w.shape
+    logp = _f32(dev, rows)
+    lse = _f32(dev, rows) if keep else None
+    # without logits in memory a chunk only bounds the statistics (8 bytes per 128 columns)
+    step = max(1, min(rows, max(chunk_size, AUTO_CHUNK_ROWS)))
+    ws = _f32(dev, int(lib.bt_logp_fwd_ws_floats(step, vocab)))
+    st = _lib.status_word(dev)
+    with _lib.device_of(dev), _lib.timed("logp_fwd", 2 * -(-rows // step), dev):
+        rc = lib.bt_logp_fwd(x.data_ptr(), w.data_ptr(), labels.data_ptr(), logp.data_ptr(),
+                             lse.data_ptr() if keep else None, ws.data_ptr(), rows, hdim, vocab, _ld(x), step,
+                             ignore_index, _lib.dtype_code(x.dtype), st.data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "bt_logp_fwd")
+    return logp.view(target.shape), (x, w, labels, lse)
 
 
 class LinearLogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, chunk_size):
-        x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
-        rows = x.shape[0]
-        h = _Head(x, w, ignore_index)
-        grad = any(ctx.needs_input_grad[:2])
-        logp = h.f32(rows)
-        lse = h.f32(rows) if grad else None
-        # without logits in memory a chunk only bounds the statistics (8 bytes per 128 columns)
-        step = max(1, min(rows, max(int(chunk_size), AUTO_CHUNK_ROWS)))
-        tile_stats, tgt = h.f32(step, h.n_vt, 2), h.f32(step)
-        with _lib.device_of(h.dev), _lib.timed("logp_fwd", 2 * -(-rows // step), h.dev):
-            for s in range(0, rows, step):
-                xc, lc = x[s:s + step], labels[s:s + step]
-                h.stats(xc, lc, None, tile_stats, tgt)
-                _lib.check(h.lib.bt_logp_rows(tile_stats.data_ptr(), tgt.data_ptr(), lc.data_ptr(),
-                                              logp[s:].data_ptr(), lse[s:].data_ptr() if grad else None, xc.shape[0],
-                                              h.vocab, h.ignore, h.st.data_ptr(), h.stream), "bt_logp_rows")
-        if grad:
-            ctx.save_for_backward(x, w, labels, lse)
-            ctx.meta = (hidden.shape, weight.dtype, int(ignore_index), int(chunk_size))
-        return logp.view(target.shape)
+        logp, saved = _log_probs(hidden, weight, target, ignore_index, chunk_size, True)
+        ctx.save_for_backward(*saved)
+        ctx.meta = (hidden.shape, weight.dtype, ignore_index, chunk_size)
+        return logp
 
     @staticmethod
     def backward(ctx, dlogp):
+        lib = _lib.get_lib()
         x, w, labels, lse = ctx.saved_tensors
         shape, w_dtype, ignore_index, chunk_size = ctx.meta
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        rows = x.shape[0]
-        h = _Head(x, w, ignore_index)
-        dx = torch.empty((rows, h.hdim), dtype=x.dtype, device=h.dev) if need_x else None
-        dw = h.dweight_out(w_dtype) if need_w else None
+        dev, rows = x.device, x.shape[0]
+        vocab, hdim = w.shape
+        dx = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if need_x else None
+        dw = _dweight_out(w, w_dtype) if need_w else None
         if rows == 0:
             return (dx.view(shape) if need_x else None, dw.zero_().to(w_dtype) if need_w else None, None, None, None)
         g = dlogp.reshape(-1).to(torch.float32).contiguous()
-        coef, scal = h.f32(rows), h.f32(1)
-        step = _chunk_rows(chunk_size, rows, h.ld)
+        ld = _ld_logits(vocab)
+        step = _chunk_rows(chunk_size, rows, ld)
         n_chunks = -(-rows // step)
-        dlogits = torch.empty((step, h.ld), dtype=x.dtype, device=h.dev)
-        acc = h.f32(h.vocab, h.hdim) if need_w and n_chunks > 1 else None
-        with _lib.device_of(h.dev), _lib.timed("logp_bwd", 2 + n_chunks * (1 + int(need_x) + int(need_w)), h.dev):
-            _lib.check(h.lib.bt_logp_coef(g.data_ptr(), labels.data_ptr(), rows, h.vocab, h.ignore, coef.data_ptr(),
-                                          scal.data_ptr(), h.stream), "bt_logp_coef")
-            xm = h.mask_rows(x, labels)
-            for i in range(n_chunks):
-                s = i * step
-                xc = xm[s:s + step]
-                n = xc.shape[0]
-                _lib.check(h.lib.bt_logp_dlogits(xc.data_ptr(), w.data_ptr(), labels[s:].data_ptr(),
-                                                 lse[s:].data_ptr(), coef[s:].data_ptr(), dlogits.data_ptr(), n,
-                                                 h.hdim, h.vocab, _ld(xc), h.ld, h.code, h.st.data_ptr(), h.stream),
-                           "bt_logp_dlogits")
-                if need_x:
-                    h.dhidden(dlogits, n, dx[s:], scal)
-                if need_w:
-                    last = i == n_chunks - 1
-                    h.dweight(dlogits, xc, dw if last else acc, acc if i > 0 else None, scal if last else None)
+        dlogits = torch.empty((step, ld), dtype=x.dtype, device=dev)
+        masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev)
+        acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
+        ws = _f32(dev, rows + 1)
+        st = _lib.status_word(dev)
+        with _lib.device_of(dev), _lib.timed("logp_bwd", 2 + n_chunks * (1 + int(need_x) + int(need_w)), dev):
+            rc = lib.bt_logp_bwd(g.data_ptr(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(),
+                                 masked.data_ptr(), dlogits.data_ptr(), dx.data_ptr() if need_x else None,
+                                 dw.data_ptr() if need_w else None, acc.data_ptr() if acc is not None else None,
+                                 ws.data_ptr(), rows, hdim, vocab, _ld(x), step, ignore_index,
+                                 _lib.dtype_code(x.dtype), _lib.dtype_code(dw.dtype) if need_w else 0, st.data_ptr(),
+                                 _lib.stream_ptr(dev))
+        _lib.check(rc, "bt_logp_bwd")
         return (dx.view(shape) if need_x else None, dw.to(w_dtype) if need_w else None, None, None, None)
+
+
+def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_coef, ignore_index, chunk_size, need_x,
+            need_w):
+    """((loss, log-probabilities, averages), what the backward needs)."""
+    lib = _lib.get_lib()
+    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
+    dev, rows = x.device, x.shape[0]
+    vocab, hdim = w.shape
+    grad = need_x or need_w
+    old, adv, ref = (t if t is None else t.detach().reshape(-1).to(torch.float32).contiguous()
+                     for t in (old, adv, ref))
+    n_seq = 1 if cu is None else cu.numel() - 1
+    ld = _ld_logits(vocab)
+    step = _chunk_rows(chunk_size, rows, ld)
+    n_chunks = -(-rows // step)
+    loss, averages, logp = _f32(dev), _f32(dev, 2), _f32(dev, rows)
+    ws = _f32(dev, int(lib.bt_policy_fwd_ws_floats(rows, step, n_seq, vocab)))
+    logits = torch.empty((step, ld), dtype=x.dtype, device=dev) if grad else None
+    masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
+    # fp32 until the upstream gradient is known: one rounding to the hidden states' type
+    dx = _f32(dev, rows, hdim) if need_x else None
+    acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    d = _lib.PolicyDesc(ptr(x), ptr(w), ptr(labels), ptr(old), ptr(adv), ptr(ref), ptr(cu), ptr(logp), ptr(loss),
+                        ptr(averages), ptr(dx), ptr(acc), ptr(masked), ptr(logits), ptr(ws), rows, hdim, vocab, _ld(x),
+                        step, n_seq, ignore_index, clip_low, clip_high, kl_coef, int(need_w), _lib.dtype_code(x.dtype))
+    st = _lib.status_word(dev)
+    with _lib.device_of(dev), _lib.timed("policy_fwd", 2 + int(grad) + n_chunks *
+                                         (2 + int(grad) + int(need_x) + int(need_w)) - int(need_w), dev):
+        rc = lib.bt_policy_fwd(ctypes.byref(d), st.data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "bt_policy_fwd")
+    last = masked[(n_chunks - 1) * step:] if need_w and n_chunks else None
+    return (loss, logp.view(target.shape), averages), (w, ws[:2], dx, logits if need_w else None, last, acc)
 
 
 class LinearPolicyLossFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_coef, ignore_index, chunk_size):
-        x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
-        rows = x.shape[0]
-        h = _Head(x, w, ignore_index)
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        grad = need_x or need_w
-        old, adv, ref = (t if t is None else t.detach().reshape(-1).to(torch.float32).contiguous()
-                         for t in (old, adv, ref))
-        n_seq = 1 if cu is None else cu.numel() - 1
-        seq_w, scal, sums = h.f32(max(n_seq, 1)), h.f32(2), h.f32(3)
-        logp, terms = h.f32(rows), h.f32(3, rows)
-        step = _chunk_rows(chunk_size, rows, h.ld)
-        n_chunks = -(-rows // step)
-        lse, coef, tgt, tile_stats = h.f32(step), h.f32(step), h.f32(step), h.f32(step, h.n_vt, 2)
-        logits = torch.empty((step, h.ld), dtype=x.dtype, device=h.dev) if grad else None
-        # fp32 until the upstream gradient is known: one rounding to the hidden states' type
-        dx = h.f32(rows, h.hdim) if need_x else None
-        acc = h.f32(h.vocab, h.hdim) if need_w and n_chunks > 1 else None
-        x_last = x
-        cu_ptr = cu.data_ptr() if cu is not None else None
-        with _lib.device_of(h.dev), _lib.timed("policy_fwd", 2 + int(grad) + n_chunks *
-                                               (2 + int(grad) + int(need_x) + int(need_w)) - int(need_w), h.dev):
-            _lib.check(h.lib.bt_policy_weights(labels.data_ptr(), rows, cu_ptr, n_seq, h.vocab, h.ignore,
-                                               seq_w.data_ptr(), scal.data_ptr(), h.st.data_ptr(), h.stream),
-                       "bt_policy_weights")
-            xm = h.mask_rows(x, labels) if grad and rows > 0 else x
-            for i in range(n_chunks):
-                s = i * step
-                xc, lc = xm[s:s + step], labels[s:s + step]
-                n = xc.shape[0]
-                h.stats(xc, lc, logits, tile_stats, tgt)
-                _lib.check(h.lib.bt_policy_rows(tile_stats.data_ptr(), tgt.data_ptr(), lc.data_ptr(), old.data_ptr(),
-                                                adv.data_ptr(), ref.data_ptr() if ref is not None else None, cu_ptr,
-                                                seq_w.data_ptr(), scal.data_ptr(), logp[s:].data_ptr(),
-                                                lse.data_ptr(), coef.data_ptr(), terms.data_ptr(), n, s, rows, n_seq,
-                                                h.vocab, h.ignore, clip_low, clip_high, kl_coef, h.stream),
-                           "bt_policy_rows")
-                if not grad:
-                    continue
-                _lib.check(h.lib.bt_policy_dlogits(logits.data_ptr(), tile_stats.data_ptr(), lse.data_ptr(),
-                                                   lc.data_ptr(), coef.data_ptr(), n, h.vocab, h.ld, h.code, h.stream),
-                           "bt_policy_dlogits")
-                if need_x:
-                    h.dhidden(logits, n, dx[s:], None)
-                if need_w:
-                    if i < n_chunks - 1:
-                        h.dweight(logits, xc, acc, acc if i > 0 else None, None)
-                    else:
-                        x_last = xc
-            _lib.check(h.lib.bt_policy_reduce(terms.data_ptr(), rows, sums.data_ptr(), h.stream), "bt_policy_reduce")
-        if grad:
-            empty = scal[:0]
-            ctx.save_for_backward(w, scal, dx if need_x else empty, logits if need_w else empty, x_last,
-                                  acc if acc is not None else empty)
-            ctx.meta = (hidden.shape, hidden.dtype, weight.dtype, n_chunks, int(ignore_index))
-        loss, kl, clipped = sums[0].clone(), sums[1].clone(), sums[2].clone()
-        logp = logp.view(target.shape)
-        ctx.mark_non_differentiable(logp, kl, clipped)
+    def forward(ctx, hidden, weight, *args):
+        out, saved = _policy(hidden, weight, *args, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        ctx.save_for_backward(*saved)
+        ctx.meta = (hidden.shape, hidden.dtype, weight.dtype)
+        ctx.mark_non_differentiable(out[1], out[2])
         ctx.set_materialize_grads(False)
-        return loss, logp, kl, clipped
+        return out
 
     @staticmethod
     def backward(ctx, dloss, *_):
         none = (None,) * 10
         if dloss is None:
             return (None, None, *none)
+        lib = _lib.get_lib()
         w, scal, dx, dlogits, x_last, acc = ctx.saved_tensors
-        shape, x_dtype, w_dtype, n_chunks, ignore_index = ctx.meta
+        shape, x_dtype, w_dtype = ctx.meta
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        h = _Head(x_last, w, ignore_index)
+        dev = w.device
+        vocab, hdim = w.shape
+        stream, code = _lib.stream_ptr(dev), _lib.dtype_code(x_dtype)
         # the coefficients were stored relative to the largest token weight (scal[0])
-        alpha = (dloss.detach().to(torch.float32) * scal[0]).reshape(1)
+        alpha = dloss.detach().to(torch.float32) * scal[0]
         dx_out = dw = None
-        with _lib.device_of(h.dev), _lib.timed("policy_bwd", int(need_x) + int(need_w and n_chunks > 0), h.dev):
+        with _lib.device_of(dev), _lib.timed("policy_bwd", int(need_x) + int(need_w and x_last is not None), dev):
             if need_x:
-                dx_out = torch.empty(dx.shape, dtype=x_dtype, device=h.dev)
-                _lib.check(h.lib.bt_scale_cast(dx.data_ptr(), dx_out.data_ptr(), dx.numel(), alpha.data_ptr(),
-                                               _lib.BT_FP32, h.code, h.stream), "bt_scale_cast(dhidden)")
-                dx_out = dx_out.view(shape)
+                dx_out = torch.empty(shape, dtype=x_dtype, device=dev)
+                _lib.check(lib.bt_scale_cast(dx.data_ptr(), dx_out.data_ptr(), dx.numel(), alpha.data_ptr(),
+                                             _lib.BT_FP32, code, stream), "bt_scale_cast(dhidden)")
             if need_w:
-                dw = h.dweight_out(w_dtype)
-                if n_chunks == 0:
+                dw = _dweight_out(w, w_dtype)
+                if x_last is None:
                     dw.zero_()
                 else:
-                    h.dweight(dlogits, x_last, dw, acc if n_chunks > 1 else None, alpha)
+                    # dW = alpha (dlogits^T x + the other chunks)
+                    st = _lib.status_word(dev)
+                    _lib.check(lib.bt_gemm(dlogits.data_ptr(), x_last.data_ptr(), dw.data_ptr(), vocab, hdim,
+                                           x_last.shape[0], dlogits.shape[1], hdim, hdim, 0, 0, code,
+                                           _lib.dtype_code(dw.dtype), acc.data_ptr() if acc is not None else None,
+                                           hdim, alpha.data_ptr(), st.data_ptr(), stream), "bt_gemm(dweight)")
                 dw = dw.to(w_dtype)
         return (dx_out, dw, *none)
 
@@ -300,7 +252,9 @@ def fused_linear_log_probs(hidden_states: Tensor, weight: Tensor, target: Tensor
     backward.  fp32 tensors are multiplied as tf32.  A target that is neither ``ignore_index`` nor a
     vocabulary row counts as ignored and sets ``BT_STATUS_BAD_LABEL`` (see ``check_all_status``)."""
     _check("fused_linear_log_probs", hidden_states, weight, target, chunk_size)
-    return LinearLogProbsFunction.apply(hidden_states, weight, target, int(ignore_index), int(chunk_size))
+    if torch.is_grad_enabled() and (hidden_states.requires_grad or weight.requires_grad):
+        return LinearLogProbsFunction.apply(hidden_states, weight, target, int(ignore_index), int(chunk_size))
+    return _log_probs(hidden_states, weight, target, int(ignore_index), int(chunk_size), False)[0]
 
 
 def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tensor, old_log_probs: Tensor,
@@ -341,6 +295,10 @@ def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tens
         if cu_seqlens.dtype == torch.int64:
             cu_seqlens = cu_seqlens.clamp(-1, (1 << 31) - 1).to(torch.int32)
         cu_seqlens = cu_seqlens.contiguous()
-    return PolicyLoss(*LinearPolicyLossFunction.apply(hidden_states, weight, target, old_log_probs, advantages,
-                                                      ref_log_probs, cu_seqlens, clip_low, clip_high, kl_coef,
-                                                      int(ignore_index), int(chunk_size)))
+    args = (hidden_states, weight, target, old_log_probs, advantages, ref_log_probs, cu_seqlens, clip_low, clip_high,
+            kl_coef, int(ignore_index), int(chunk_size))
+    if torch.is_grad_enabled() and (hidden_states.requires_grad or weight.requires_grad):
+        loss, log_probs, averages = LinearPolicyLossFunction.apply(*args)
+    else:
+        loss, log_probs, averages = _policy(*args, False, False)[0]
+    return PolicyLoss(loss, log_probs, averages[0], averages[1])

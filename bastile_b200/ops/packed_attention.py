@@ -56,38 +56,43 @@ def pack_sequences(cu_seqlens: Tensor, total_tokens: int) -> PackedSequences:
 
 
 def _strides(t: Tensor):
-    return _lib.I64x2(t.stride(0), t.stride(1))
+    return _lib.I64x2(*t.stride()[:2])
 
 
 def _rows(t: Tensor) -> Tensor:
     """``t`` if the kernels can read it where it lies (unit stride along the head, 16-byte rows), else a copy."""
-    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2])))
-    return t if ok else t.contiguous()
+    (n, heads, _), (st, sh, sd) = t.shape, t.stride()
+    if sd == 1 and (n <= 1 or (st > 0 and st % 8 == 0)) and (heads <= 1 or (sh > 0 and sh % 8 == 0)) \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous()
+
+
+def _forward(q, k, v, sequences, scale, keep: bool):
+    """(out, what the backward needs if ``keep``)."""
+    lib = _lib.get_lib()
+    dev = q.device
+    t, hq, d = q.shape
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    lse2 = torch.empty((hq, t), dtype=torch.float32, device=dev) if keep else None
+    if t > 0:
+        st = _lib.status_word(dev)
+        with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
+            rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                 lse2.data_ptr() if keep else None, sequences.plan.data_ptr(), sequences.batch, t, hq,
+                                 k.shape[1], d, _strides(q), _strides(k), _strides(v), _strides(out), scale,
+                                 _lib.dtype_code(q.dtype), st.data_ptr(), _lib.stream_ptr(dev))
+        _lib.check(rc, "bt_attn_fwd")
+    return out, (q, k, v, out, lse2, sequences.plan)
 
 
 class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, sequences, scale):
-        dev = q.device
-        lib = _lib.get_lib()
-        t, hq, d = q.shape
-        hk = k.shape[1]
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-        lse2 = torch.empty((hq, t), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad[:3]) else None
-        if out.numel() > 0:
-            st = _lib.status_word(dev)
-            with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
-                rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                     lse2.data_ptr() if lse2 is not None else None, sequences.plan.data_ptr(),
-                                     sequences.batch, t, hq, hk, d, _strides(q), _strides(k), _strides(v),
-                                     _strides(out), scale, _lib.dtype_code(q.dtype), st.data_ptr(),
-                                     _lib.stream_ptr(dev))
-            _lib.check(rc, "bt_attn_fwd")
-        if lse2 is not None:
-            ctx.save_for_backward(q, k, v, out, lse2, sequences.plan)
-            ctx.meta = (sequences.batch, scale)
+        out, saved = _forward(q, k, v, sequences, scale, True)
+        ctx.save_for_backward(*saved)
+        ctx.meta = (sequences.batch, scale)
         return out
 
     @staticmethod
@@ -142,4 +147,6 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, sequences: PackedSequences
         raise ValueError(f"packed_attention: q has {t} tokens, the packed sequences {sequences.total_tokens}")
     _lib.require_cuda(q, k, v, sequences.plan)
     scale = d ** -0.5 if scale is None else float(scale)
-    return PackedAttentionFunction.apply(q, k, v, sequences, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return PackedAttentionFunction.apply(q, k, v, sequences, scale)
+    return _forward(q, k, v, sequences, scale, False)[0]

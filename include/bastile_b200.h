@@ -481,47 +481,55 @@ int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, c
 /* ---- log-probabilities through the output head and the clipped policy loss (no reference
  * counterpart; the products and chunking are those of the fused cross-entropy) ----
  *
- * A position counts when its label is a vocabulary row other than ignore_index; a label that is neither
- * sets BT_STATUS_BAD_LABEL.  `tile_stats` is rows * bt_lce_num_vtiles(V) pairs of floats.
+ * hidden [rows, H] with row stride ld_hidden, W [V, H] dense, labels [rows]; 16-byte aligned rows.  A
+ * position counts when its label is a vocabulary row other than ignore_index; a label that is neither
+ * sets BT_STATUS_BAD_LABEL.  Rows are worked through `chunk` at a time; a buffer of logits is
+ * [min(chunk, rows), (V + 7) / 8 * 8] in `dtype`.  `masked` is [rows, H] scratch in `dtype`.
  *
- * bt_logp_stats: (max, sum exp) per 128 columns and the target logit of hidden W^T, from the fp32
- * accumulators.  logits may be NULL; otherwise [rows, ld_logits] in `dtype` receives every logit minus
- * the maximum of its 128 columns. */
-int bt_logp_stats(const void* hidden, const void* W, const int64_t* labels, void* logits, float* tile_stats,
-                  float* tgt_logit, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t ld_logits,
-                  int64_t ignore_index, int dtype, int32_t* status, void* stream);
-/* logp[rows] (0 where a position does not count) and, unless NULL, lse[rows]. */
-int bt_logp_rows(const float* tile_stats, const float* tgt_logit, const int64_t* labels, float* logp, float* lse,
-                 int64_t rows, int64_t V, int64_t ignore_index, int32_t* status, void* stream);
-/* coef[n] = dlogp scaled by the power of two that brings the largest of the counted ones into [1/2, 1)
- * (0 where a position does not count); scal[0] = the factor back. */
-int bt_logp_coef(const float* dlogp, const int64_t* labels, int64_t n, int64_t V, int64_t ignore_index, float* coef,
-                 float* scal, void* stream);
-/* dlogits[rows, ld] = coef (onehot(label) - exp(hidden W^T - lse)), logits recomputed. */
-int bt_logp_dlogits(const void* hidden, const void* W, const int64_t* labels, const float* lse, const float* coef,
-                    void* dlogits, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t ld_dlogits,
-                    int dtype, int32_t* status, void* stream);
-/* y[rows, H] dense = x where the position counts, 0 elsewhere. */
-int bt_logp_mask_rows(const void* x, void* y, const int64_t* labels, int64_t rows, int64_t H, int64_t ld, int64_t V,
-                      int64_t ignore_index, int dtype, void* stream);
-/* weights[n_seq]: what one counted token of each sequence weighs in the mean over sequences of token
- * means (cu_seqlens NULL, n_seq 1: the mean over all tokens); scal[0] = largest weight, scal[1] = 1 / it.
- * Offsets are checked as in bt_attn_plan; with bad ones nothing counts. */
-int bt_policy_weights(const int64_t* labels, int64_t n, const int32_t* cu_seqlens, int64_t n_seq, int64_t V,
-                      int64_t ignore_index, float* weights, float* scal, int32_t* status, void* stream);
-/* One chunk of rows (row0 .. row0 + rows of `total`): logp, lse and coef = d loss / d logp / scal[0] per
- * row of the chunk; terms[3][total] = weighted loss, kl and clipped at the rows' places.  labels, logp,
- * lse, coef and tile_stats are the chunk's; old_logp, adv and ref_logp (may be NULL) the whole batch's. */
-int bt_policy_rows(const float* tile_stats, const float* tgt_logit, const int64_t* labels, const float* old_logp,
-                   const float* adv, const float* ref_logp, const int32_t* cu_seqlens, const float* weights,
-                   const float* scal, float* logp, float* lse, float* coef, float* terms, int64_t rows, int64_t row0,
-                   int64_t total, int64_t n_seq, int64_t V, int64_t ignore_index, float clip_low, float clip_high,
-                   float kl_coef, void* stream);
-/* The shifted logits of bt_logp_stats -> coef (onehot - softmax), in place. */
-int bt_policy_dlogits(void* logits, const float* tile_stats, const float* lse, const int64_t* labels,
-                      const float* coef, int64_t rows, int64_t V, int64_t ld_logits, int dtype, void* stream);
-/* out[3] = sums of the three rows of terms. */
-int bt_policy_reduce(const float* terms, int64_t n, float* out, void* stream);
+ * bt_logp_fwd: logp[rows] fp32 (0 where a position does not count) and, unless NULL, lse[rows], from the
+ * fp32 accumulators of the logits product; ws: bt_logp_fwd_ws_floats(chunk, V) floats. */
+int64_t bt_logp_fwd_ws_floats(int64_t chunk, int64_t V);
+int bt_logp_fwd(const void* hidden, const void* W, const int64_t* labels, float* logp, float* lse, float* ws,
+                int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
+                int32_t* status, void* stream);
+/* Gradients for the upstream gradient dlogp[rows]; logits are recomputed.  dhidden [rows, H] in `dtype`
+ * and dweight [V, H] in dweight_dtype may each be NULL; dweight_acc [V, H] fp32 is needed for dweight when
+ * rows > chunk; ws: rows + 1 floats. */
+int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels, const float* lse,
+                void* masked, void* dlogits, void* dhidden, void* dweight, float* dweight_acc, float* ws, int64_t rows,
+                int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
+                int dweight_dtype, int32_t* status, void* stream);
+
+/* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
+ * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
+ * counts).  loss [1], averages [2] = (kl, clipped fraction), logp [rows].  dhidden (fp32 [rows, H], may be
+ * NULL) and the weight gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose
+ * dlogits stay in `logits`) are relative to ws[0], the largest weight of a token: the caller multiplies by
+ * it and the upstream gradient.  masked, logits: needed with either gradient.
+ * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats. */
+typedef struct {
+  const void* hidden;
+  const void* W;
+  const int64_t* labels;
+  const float* old_logp;
+  const float* adv;
+  const float* ref_logp; /* may be NULL: no KL term */
+  const int32_t* cu_seqlens;
+  float* logp;
+  float* loss;
+  float* averages;
+  float* dhidden;
+  float* dweight_acc;
+  void* masked;
+  void* logits;
+  float* ws;
+  int64_t rows, H, V, ld_hidden, chunk, n_seq, ignore_index;
+  float clip_low, clip_high, kl_coef;
+  int32_t want_dweight;
+  int32_t dtype;
+} bt_policy_desc;
+int64_t bt_policy_fwd_ws_floats(int64_t rows, int64_t chunk, int64_t n_seq, int64_t V);
+int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

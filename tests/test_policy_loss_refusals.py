@@ -55,21 +55,37 @@ def test_c_entry_points():
     def err(rc, text):
         assert rc == -1 and text in lib.bt_last_error(), lib.bt_last_error()
 
-    err(lib.bt_logp_stats(None, one, one, None, one, one, 4, 64, 100, 64, 104, -100, b, None, None), b"null")
-    err(lib.bt_logp_stats(one, one, one, one, one, one, 4, 64, 100, 64, 96, -100, b, None, None), b"stride")
-    err(lib.bt_logp_stats(one, one, one, None, one, one, 4, 64, 100, 64, 104, -100, 7, None, None), b"dtype")
-    err(lib.bt_logp_stats(one, one, one, None, one, one, 4, 0, 100, 64, 104, -100, b, None, None), b"extents")
-    err(lib.bt_logp_rows(one, one, one, None, None, 4, 100, -100, None, None), b"null")
-    err(lib.bt_logp_coef(one, one, 4, 100, -100, None, one, None), b"null")
-    err(lib.bt_logp_dlogits(one, one, one, one, None, one, 4, 64, 100, 64, 104, b, None, None), b"null")
-    err(lib.bt_logp_dlogits(one, one, one, one, one, one, 4, 64, 100, 64, 99, b, None, None), b"stride")
-    err(lib.bt_logp_mask_rows(one, one, one, 4, 60, 60, 100, -100, b, None), b"aligned")
-    err(lib.bt_policy_weights(one, 4, None, 2, 100, -100, one, one, None, None), b"sequence count")
-    err(lib.bt_policy_weights(one, 4, one, 2, 100, -100, None, one, None, None), b"null")
-    err(lib.bt_policy_rows(*[one] * 13, 4, 2, 5, 1, 100, -100, 0.2, 0.2, 0.0, None), b"outside")
-    err(lib.bt_policy_rows(None, *[one] * 12, 4, 0, 5, 1, 100, -100, 0.2, 0.2, 0.0, None), b"null")
-    err(lib.bt_policy_dlogits(one, one, one, one, one, 4, 101, 103, b, None), b"aligned")
-    err(lib.bt_policy_reduce(None, 4, one, None), b"bad args")
-    for rc in (lib.bt_logp_rows(None, None, None, None, None, 0, 100, -100, None, None),
-               lib.bt_policy_dlogits(None, None, None, None, None, 0, 100, 104, b, None)):
-        assert rc == 0  # no rows: nothing to do
+    def fwd(hidden=one, w=one, labels=one, logp=one, ws=one, rows=4, h=64, v=100, ld=64, chunk=4, dtype=b):
+        return lib.bt_logp_fwd(hidden, w, labels, logp, None, ws, rows, h, v, ld, chunk, -100, dtype, None, None)
+
+    err(fwd(hidden=None), b"null"), err(fwd(labels=None), b"null"), err(fwd(logp=None), b"null")
+    err(fwd(dtype=7), b"dtype"), err(fwd(h=0), b"extents"), err(fwd(rows=-1), b"extents"), err(fwd(chunk=0), b"chunk")
+    err(fwd(hidden=C.c_void_p(8)), b"aligned"), err(fwd(ld=60), b"aligned"), err(fwd(ld=56), b"aligned")
+    assert fwd(rows=0, hidden=None, labels=None) == 0
+
+    def bwd(dlogp=one, masked=one, dw=one, acc=one, rows=4, chunk=4):
+        return lib.bt_logp_bwd(dlogp, one, one, one, one, masked, one, one, dw, acc, one, rows, 64, 100, 64, chunk,
+                               -100, b, b, None, None)
+
+    err(bwd(dlogp=None), b"null"), err(bwd(masked=None), b"null"), err(bwd(masked=C.c_void_p(24)), b"aligned")
+    err(bwd(acc=None, chunk=2), b"accumulator")
+    assert bwd(rows=0) == 0
+
+    def policy(**kw):
+        d = _lib.PolicyDesc()
+        for n, t in d._fields_:
+            if t is C.c_void_p and n not in ("cu_seqlens", "ref_logp"):
+                setattr(d, n, 16)
+        d.rows, d.H, d.V, d.ld_hidden, d.chunk, d.n_seq, d.ignore_index, d.dtype = 4, 64, 100, 64, 4, 1, -100, b
+        for n, x in kw.items():
+            setattr(d, n, x)
+        return lib.bt_policy_fwd(C.byref(d), None, None)
+
+    err(lib.bt_policy_fwd(None, None, None), b"null descriptor")
+    for kw, text in ((dict(hidden=None), b"null"), (dict(ws=None), b"null"), (dict(adv=None), b"null"),
+                     (dict(masked=None), b"buffers"), (dict(logits=24), b"buffers"), (dict(n_seq=2), b"sequence count"),
+                     (dict(n_seq=-1, cu_seqlens=16), b"sequence count"), (dict(dtype=9), b"dtype"),
+                     (dict(chunk=2, want_dweight=1, dweight_acc=None), b"accumulator"), (dict(ld_hidden=8), b"aligned")):
+        err(policy(**kw), text)
+    assert lib.bt_logp_fwd_ws_floats(3, 100) == 3 * 2 * 2 + 3 and lib.bt_logp_fwd_ws_floats(-1, 100) == 0
+    assert lib.bt_policy_fwd_ws_floats(5, 3, 2, 100) == 28 + 3 * 2 * 2 and lib.bt_policy_fwd_ws_floats(5, 3, 2, 0) == 0
