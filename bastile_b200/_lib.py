@@ -107,7 +107,9 @@ SIGNATURES = {
                     [c_float, c_int, c_void_p, c_void_p]),
     "bt_logp_fwd_ws_floats": (c_int64, [c_int64] * 2),
     "bt_logp_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 6 + [c_int, c_void_p, c_void_p]),
-    "bt_logp_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_void_p]),
+    "bt_dhidden_runs": (c_int64, [c_int64] * 3 + [c_int]),
+    "bt_sum_runs": (c_int, [c_void_p, c_void_p] + [c_int64] * 3 + [c_void_p, c_int, c_void_p]),
+    "bt_logp_bwd": (c_int, [c_void_p] * 12 + [c_int64] * 6 + [c_int, c_int, c_void_p, c_void_p]),
     "bt_policy_fwd_ws_floats": (c_int64, [c_int64] * 4),
     "bt_policy_fwd": (c_int, [POINTER(PolicyDesc), c_void_p, c_void_p]),
     "bt_scale_cast": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p]),

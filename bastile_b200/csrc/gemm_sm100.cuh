@@ -95,6 +95,8 @@ struct Params {
   int a_split;     // A_WHOLE, A_SPLIT_K or A_SPLIT_M
   int m_seg0, m_seg1;  // A_SPLIT_M: rows [0, m_seg0) come from A0, the next m_seg1 from A1, the rest from A2
   int tiles_m, tiles_n, num_tiles;
+  int splits, kb_split;   // > 1: the contraction is cut into `splits` runs of kb_split k-blocks, each a tile of its
+  int64_t split_stride;   // own whose fp32 result goes to out + run * split_stride (plain epilogue, fp32 only)
   int group_m;     // rasterisation: row-tiles walked per column-tile before moving on
   int a_kmajor, b_kmajor, dual_b;
   uint32_t idesc;
@@ -145,6 +147,23 @@ __device__ __forceinline__ void tile_coords(const Params& p, int tile, int* m_id
   const int r = tile - g * per_group;
   *m_idx = first_m + r % gs;
   *n_idx = r / gs;
+}
+
+// The k-blocks of a tile and, with a cut contraction, which run they are; reduces `tile` to its place
+// in the result.
+struct KRun {
+  int begin, end, run;
+};
+__device__ __forceinline__ KRun k_run(const Params& p, int* tile, int nkb) {
+  KRun r{0, nkb, 0};
+  if (p.splits > 1) {
+    const int per = p.tiles_m * p.tiles_n;
+    r.run = *tile / per;
+    *tile -= r.run * per;
+    r.begin = r.run * p.kb_split;
+    r.end = min(nkb, r.begin + p.kb_split);
+  }
+  return r;
 }
 
 template <typename T>
@@ -255,14 +274,14 @@ __device__ __forceinline__ void stage_store32(OutStage& st, const CUtensorMap* t
 
 // ------------------------------------------------------------------ epilogues
 template <typename T>
-__device__ __forceinline__ void epi_plain(const Params& p, uint32_t taddr, int64_t row, int n0,
+__device__ __forceinline__ void epi_plain(const Params& p, uint32_t taddr, int64_t row, int n0, int run,
                                           int half, OutStage& stg, const CUtensorMap* tmO0,
                                           const CUtensorMap* tmO1, const CUtensorMap* tmO2, int lane) {
   const float alpha = p.alpha != nullptr ? __ldg(p.alpha) : 1.0f;
   const bool row_ok = row < p.M;
   const int row0 = static_cast<int>(row) - lane;  // first row of this warp's 32
   // where this tile's columns live: one result tensor, or one of three side by side
-  void* out = p.out;
+  void* out = run == 0 ? p.out : static_cast<float*>(p.out) + run * p.split_stride;
   int64_t ldo = p.ldo;
   int col_shift = 0, n_end = p.N;
   const CUtensorMap* tmo = tmO0;
@@ -731,11 +750,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+        int place = tile;
         int m_idx, n_idx;
-        tile_coords(p, tile, &m_idx, &n_idx);
+        const KRun kr = k_run(p, &place, nkb);
+        tile_coords(p, place, &m_idx, &n_idx);
         const int m0 = m_idx * BM;
         const int n0 = n_idx * (p.dual_b ? BN / 2 : BN);
-        for (int kb = 0; kb < nkb; ++kb) {
+        for (int kb = kr.begin; kb < kr.end; ++kb) {
           if (!ptx::mbar_wait(&empty[stage], phase ^ 1u, cta_abort, p.status, ST_PRODUCER)) {
             ok = false;
             break;
@@ -785,10 +806,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+        int place = tile;
+        const KRun kr = k_run(p, &place, nkb);
         if (!ptx::mbar_wait(&tempty[acc], acc_phase ^ 1u, cta_abort, p.status, ST_MMA_ACC)) break;
         ptx::tcgen05_fence_after_sync();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = 0; kb < nkb; ++kb) {
+        for (int kb = kr.begin; kb < kr.end; ++kb) {
           if (!ptx::mbar_wait(&full[stage], phase, cta_abort, p.status, ST_MMA_FULL)) {
             ok = false;
             break;
@@ -802,11 +825,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
             if constexpr (sizeof(T) == 4)
               ptx::umma_tf32(d_tmem, a_desc + static_cast<uint64_t>(kk * p.a_kstep),
                              b_desc + static_cast<uint64_t>(kk * p.b_kstep), p.idesc,
-                             (kb | kk) != 0 ? 1u : 0u);
+                             (kb != kr.begin || kk != 0) ? 1u : 0u);
             else
               ptx::umma_f16(d_tmem, a_desc + static_cast<uint64_t>(kk * p.a_kstep),
                             b_desc + static_cast<uint64_t>(kk * p.b_kstep), p.idesc,
-                            (kb | kk) != 0 ? 1u : 0u);
+                            (kb != kr.begin || kk != 0) ? 1u : 0u);
           }
           ptx::umma_commit(&empty[stage]);  // frees the smem stage when these MMAs retire
           if (++stage == kStages) {
@@ -832,8 +855,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
                          : 0u;
     stg.count = 0;
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x) {
+      int place = tile;
       int m_idx, n_idx;
-      tile_coords(p, tile, &m_idx, &n_idx);
+      const KRun kr = k_run(p, &place, nkb);
+      tile_coords(p, place, &m_idx, &n_idx);
       // all 32 lanes leave together: what follows is warp-synchronous (tcgen05.ld.sync.aligned)
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], acc_phase, cta_abort, p.status, ST_EPILOGUE)))
         break;
@@ -841,7 +866,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CU
       const uint32_t taddr =
           tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
       const int64_t row = static_cast<int64_t>(m_idx) * BM + quarter * 32 + lane;
-      if (EPI == EPI_PLAIN) epi_plain<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, &tmO2, lane);
+      if (EPI == EPI_PLAIN)
+        epi_plain<T>(p, taddr, row, n_idx * BN, kr.run, half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_FWD)
         epi_swiglu_fwd<T>(p, taddr, row, n_idx * (BN / 2), half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_BWD) epi_swiglu_bwd<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, lane);
@@ -1020,11 +1046,13 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
           tile = sched_wait(p, pair, npairs, it, cta_abort, ST_PRODUCER);
         }
         if (tile < 0) break;
+        int place = tile;
         int m_idx, n_idx;
-        tile_coords(p, tile, &m_idx, &n_idx);
+        const KRun kr = k_run(p, &place, nkb);
+        tile_coords(p, place, &m_idx, &n_idx);
         const int m0 = m_idx * (2 * BM) + static_cast<int>(rank) * BM;
         const int n0 = p.dual_b ? n_idx * (BN / 2) : n_idx * BN + static_cast<int>(rank) * (BN / 2);
-        for (int kb = 0; kb < nkb; ++kb) {
+        for (int kb = kr.begin; kb < kr.end; ++kb) {
           if (!ptx::mbar_wait(&empty[stage], phase ^ 1u, cta_abort, p.status, ST_PRODUCER)) {
             ok = false;
             break;
@@ -1071,11 +1099,13 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int it = 0; ok; ++it) {
-        if (sched_wait(p, pair, npairs, it, cta_abort, ST_MMA_ACC) < 0) break;
+        int place = sched_wait(p, pair, npairs, it, cta_abort, ST_MMA_ACC);
+        if (place < 0) break;
+        const KRun kr = k_run(p, &place, nkb);
         if (!ptx::mbar_wait(&tempty[acc], acc_phase ^ 1u, cta_abort, p.status, ST_MMA_ACC)) break;
         ptx::tcgen05_fence_after_sync();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = 0; kb < nkb; ++kb) {
+        for (int kb = kr.begin; kb < kr.end; ++kb) {
           if (!ptx::mbar_wait(&full[stage], phase, cta_abort, p.status, ST_MMA_FULL)) {
             ok = false;
             break;
@@ -1089,11 +1119,11 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
             if constexpr (sizeof(T) == 4)
               ptx::umma_tf32_pair(d_tmem, a_desc + static_cast<uint64_t>(kk * p.a_kstep),
                                   b_desc + static_cast<uint64_t>(kk * p.b_kstep), p.idesc,
-                                  (kb | kk) != 0 ? 1u : 0u);
+                                  (kb != kr.begin || kk != 0) ? 1u : 0u);
             else
               ptx::umma_f16_pair(d_tmem, a_desc + static_cast<uint64_t>(kk * p.a_kstep),
                                  b_desc + static_cast<uint64_t>(kk * p.b_kstep), p.idesc,
-                                 (kb | kk) != 0 ? 1u : 0u);
+                                 (kb != kr.begin || kk != 0) ? 1u : 0u);
           }
           ptx::umma_commit_pair(&empty[stage]);
           if (++stage == kStages2) {
@@ -1123,8 +1153,10 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
       if (lane == 0) tile = sched_wait(p, pair, npairs, it, cta_abort, ST_EPILOGUE);
       tile = __shfl_sync(0xffffffffu, tile, 0);
       if (tile < 0) break;
+      int place = tile;
       int m_idx, n_idx;
-      tile_coords(p, tile, &m_idx, &n_idx);
+      const KRun kr = k_run(p, &place, nkb);
+      tile_coords(p, place, &m_idx, &n_idx);
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], acc_phase, cta_abort, p.status, ST_EPILOGUE)))
         break;
       ptx::tcgen05_fence_after_sync();
@@ -1132,7 +1164,8 @@ gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
           tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
       const int64_t row =
           static_cast<int64_t>(m_idx) * (2 * BM) + static_cast<int64_t>(rank) * BM + quarter * 32 + lane;
-      if (EPI == EPI_PLAIN) epi_plain<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, &tmO2, lane);
+      if (EPI == EPI_PLAIN)
+        epi_plain<T>(p, taddr, row, n_idx * BN, kr.run, half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_FWD)
         epi_swiglu_fwd<T>(p, taddr, row, n_idx * (BN / 2), half, stg, &tmO0, &tmO1, &tmO2, lane);
       if (EPI == EPI_SWIGLU_BWD) epi_swiglu_bwd<T>(p, taddr, row, n_idx * BN, half, stg, &tmO0, &tmO1, lane);
@@ -1510,6 +1543,18 @@ int launch(Launch& L, cudaStream_t s) {
     return BT_ERR_ARG;
   }
   p.num_tiles = static_cast<int>(nt);
+  if (p.splits > 1) {
+    const int kbk = kRowBytes / (L.dtype == BT_FP32 ? 4 : 2);
+    const int64_t blocks = ceil_div(p.K0, kbk);
+    p.kb_split = static_cast<int>(ceil_div(blocks, p.splits));
+    if (EPI != EPI_PLAIN || !p.out_fp32 || p.K1 != 0 || p.K2 != 0 || L.dual_b || ceil_div(blocks, p.kb_split) != p.splits ||
+        nt * p.splits > 0x7fffffff || p.addend != nullptr || p.addend_t != nullptr || p.n_seg0 > 0) {
+      set_error("gemm: a cut contraction needs a plain fp32 result and no empty run (%d runs of %d k-blocks)", p.splits,
+                p.kb_split);
+      return BT_ERR_ARG;
+    }
+    p.num_tiles *= p.splits;
+  }
   // Rasterisation: CTAs that run at the same time share operand tiles through L2.  With a short
   // contraction the A panel of 16 row tiles (16 x 256 rows x K) stays in L2 while the walk
   // crosses all column tiles, so B is fetched once per 16 row tiles.  With a long contraction

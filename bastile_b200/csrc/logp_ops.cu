@@ -348,11 +348,90 @@ int mask_rows(const Head& h, const void* x, void* y, const int64_t* labels, int6
   return BT_OK;
 }
 
-// d hidden[rows, H] = alpha dlogits[rows, V] W[V, H]
-int dhidden(const Head& h, const void* dlogits, void* out, int64_t rows, int out_dtype, const float* alpha) {
-  return bt_gemm(dlogits, h.W, out, rows, h.H, h.V, h.ld_logits, h.H, h.H, 1, 0, h.dtype, out_dtype, nullptr, 0, alpha,
-                 h.status, h.s);
+// Runs into which the contraction of d hidden is cut.  The result has few tiles (rows x H) against a long
+// contraction (V): 517 x 1024 from V = 32000 is 12 tiles for 74 CTA pairs, 2048 x 4096 is 1.7 waves.
+// The fewest runs that come within 3% of the least estimated time: waves of tiles at the sustained
+// product rate, and 8 bytes an element and run for the partial sums.  Measured, both gradient products
+// together: 517 x 1024 x 32000 in 1 / 2 / 4 / 6 / 8 runs 201 / 126 / 90 / 78 / 94 us (6 taken);
+// 4096 x 4096 x 151936 in 1 / 2 / 4 runs 8.05 / 7.59 / 7.69 ms (2 taken).
+int dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype) {
+  const int64_t pairs = sm_count() / 2, tiles = ceil_div(rows, 256) * ceil_div(H, 256);
+  const int64_t blocks = ceil_div(V, 128 / esize(dtype));
+  const double tile_s = 2.0 * 256 * 256 * V / (1.4e15 / 74);
+  double least = 0.0, cost[17] = {};
+  for (int s = 1; s <= 16; ++s) {
+    const int64_t per = ceil_div(blocks, s);
+    if (s > 1 && (per < 16 || ceil_div(blocks, per) != s)) continue;
+    cost[s] = static_cast<double>(ceil_div(tiles * s, pairs)) * tile_s * per / blocks +
+              (s > 1 ? s * rows * H * 8.0 / 6.5e12 + 2e-6 : 0.0);
+    if (s == 1 || cost[s] < least) least = cost[s];
+  }
+  for (int s = 1; s <= 16; ++s)
+    if (cost[s] > 0.0 && cost[s] <= 1.03 * least) return s;
+  return 1;
 }
+
+// parts[run][rows, H] (fp32, runs `stride` elements apart) of dlogits[rows, V] W[V, H]
+int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows, int64_t stride, int runs) {
+  gemm::Launch L;
+  L.dtype = h.dtype;
+  L.a0.ptr = dlogits, L.a0.kmajor = 1, L.a0.mn = rows, L.a0.k = h.V, L.a0.ld = h.ld_logits;
+  L.b0.ptr = h.W, L.b0.kmajor = 0, L.b0.mn = h.H, L.b0.k = h.V, L.b0.ld = h.H;
+  L.p.M = static_cast<int>(rows);
+  L.p.N = static_cast<int>(h.H);
+  L.p.status = h.status;
+  L.p.out = parts;
+  L.p.ldo = h.H;
+  L.p.out_fp32 = 1;
+  L.p.vec_ok = rows_aligned(parts, h.H, 4) && stride % 4 == 0;
+  L.p.splits = runs;
+  L.p.split_stride = stride;
+  return gemm::launch<gemm::EPI_PLAIN>(L, h.s);
+}
+
+// out = T(alpha * sum over runs), in the runs' order; four elements per thread and step.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+sum_runs_kernel(const float* __restrict__ parts, T* __restrict__ out, int64_t n4, int runs, int64_t stride4,
+                const float* __restrict__ alpha) {
+  grid_dependency_wait();
+  const float a = __ldg(alpha);
+  const float4* in = reinterpret_cast<const float4*>(parts);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n4; i += step) {
+    float4 v = __ldcs(in + i);
+    for (int r = 1; r < runs; ++r) {
+      const float4 u = __ldcs(in + r * stride4 + i);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    v.x *= a, v.y *= a, v.z *= a, v.w *= a;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(out)[i] = v;
+    } else {
+      T o[4] = {Cvt<T>::from_f(v.x), Cvt<T>::from_f(v.y), Cvt<T>::from_f(v.z), Cvt<T>::from_f(v.w)};
+      reinterpret_cast<uint2*>(out)[i] = *reinterpret_cast<const uint2*>(o);
+    }
+  }
+}
+
+int sum_runs(const float* parts, void* out, int64_t n, int runs, int64_t stride, const float* alpha, int dtype,
+             cudaStream_t s) {
+  const int64_t n4 = n / 4;  // rows are whole 16-byte vectors
+  const dim3 grid(grid_for(ceil_div(n4, kThreads), 16)), block(kThreads);
+  cudaError_t e;
+  if (dtype == BT_BF16)
+    e = launch_dependent(sum_runs_kernel<__nv_bfloat16>, grid, block, 0, s, parts, static_cast<__nv_bfloat16*>(out), n4,
+                         runs, stride / 4, alpha);
+  else if (dtype == BT_FP16)
+    e = launch_dependent(sum_runs_kernel<__half>, grid, block, 0, s, parts, static_cast<__half*>(out), n4, runs,
+                         stride / 4, alpha);
+  else
+    e = launch_dependent(sum_runs_kernel<float>, grid, block, 0, s, parts, static_cast<float*>(out), n4, runs,
+                         stride / 4, alpha);
+  BT_CHECK_LAUNCHED(e, "logp: sum of d hidden");
+  return BT_OK;
+}
+
 // out[V, H] = alpha (dlogits^T x + addend), x dense
 int dweight(const Head& h, const void* dlogits, const void* x, void* out, int64_t rows, int out_dtype,
             const float* addend, const float* alpha) {
@@ -445,8 +524,8 @@ extern "C" int bt_logp_fwd(const void* hidden, const void* W, const int64_t* lab
 }
 
 extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels,
-                           const float* lse, void* masked, void* dlogits, void* dhidden_out, void* dweight_out,
-                           float* dweight_acc, float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
+                           const float* lse, void* masked, void* dlogits, void* dhidden, float* dhidden_parts_,
+                           void* dweight_out, float* dweight_acc, float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
                            int64_t chunk, int64_t ignore_index, int dtype, int dweight_dtype, int32_t* status,
                            void* stream) {
   using namespace bt;
@@ -456,8 +535,12 @@ extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W
   if (rows == 0) return BT_OK;
   BT_CHECK_ARG(dlogp && labels && lse && masked && dlogits && ws, "logp_bwd: null pointer");
   BT_CHECK_ARG(aligned16(masked) && aligned16(dlogits), "logp_bwd: buffers must be 16-byte aligned");
+  BT_CHECK_ARG(dhidden == nullptr || (dhidden_parts_ != nullptr && aligned16(dhidden) && aligned16(dhidden_parts_)),
+               "logp_bwd: the gradient of hidden needs 16-byte aligned buffers for itself and its parts");
   BT_CHECK_ARG(dweight_out == nullptr || rows <= chunk || dweight_acc != nullptr,
                "logp_bwd: more than one chunk needs an accumulator for the weight gradient");
+  if (chunk > rows) chunk = rows;
+  const int runs = dhidden_runs(chunk, H, V, dtype);
   float* scal = ws;  // [1 + rows]: scale back, coefficients
   float* coef = ws + 1;
   BT_CHECK_LAUNCHED(launch_dependent(logp_coef_kernel, dim3(1), dim3(1024), 0, h.s, dlogp, labels, rows, ignore_index,
@@ -474,8 +557,11 @@ extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W
     L.p.ldo = h.ld_logits;
     L.p.vec_ok = rows_aligned(dlogits, h.ld_logits, esize(dtype));
     if (int rc = gemm::launch<gemm::EPI_DLOGITS>(L, h.s)) return rc;
-    if (dhidden_out != nullptr) {
-      if (int rc = dhidden(h, dlogits, const_cast<char*>(row_ptr(dhidden_out, r, H, dtype)), n, dtype, scal)) return rc;
+    if (dhidden != nullptr) {
+      if (int rc = dhidden_parts(h, dlogits, dhidden_parts_, n, chunk * H, runs)) return rc;
+      if (int rc = sum_runs(dhidden_parts_, const_cast<char*>(row_ptr(dhidden, r, H, dtype)), n * H, runs, chunk * H,
+                            scal, dtype, h.s))
+        return rc;
     }
     if (dweight_out != nullptr) {
       const bool last = r + n == rows;
@@ -485,6 +571,23 @@ extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W
     }
   }
   return BT_OK;
+}
+
+extern "C" int64_t bt_dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype) {
+  using namespace bt;
+  return rows > 0 && H > 0 && V > 0 && known(dtype) ? dhidden_runs(rows, H, V, dtype) : 1;
+}
+
+extern "C" int bt_sum_runs(const float* parts, void* out, int64_t n, int64_t runs, int64_t stride, const float* alpha,
+                           int dtype, void* stream) {
+  using namespace bt;
+  BT_CHECK_ARG(known(dtype), "sum_runs: unknown dtype %d", dtype);
+  BT_CHECK_ARG(n >= 0 && n % 4 == 0 && runs >= 1 && runs <= 1024 && (runs == 1 || (stride >= n && stride % 4 == 0)),
+               "sum_runs: bad sizes");
+  if (n == 0) return BT_OK;
+  BT_CHECK_ARG(parts && out && alpha, "sum_runs: null pointer");
+  BT_CHECK_ARG(aligned16(parts) && aligned16(out), "sum_runs: buffers must be 16-byte aligned");
+  return sum_runs(parts, out, n, static_cast<int>(runs), stride, alpha, dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t bt_policy_fwd_ws_floats(int64_t rows, int64_t chunk, int64_t n_seq, int64_t V) {
@@ -510,6 +613,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     BT_CHECK_ARG(!d->want_dweight || d->rows <= d->chunk || d->dweight_acc != nullptr,
                  "policy_fwd: more than one chunk needs an accumulator for the weight gradient");
   }
+  const int runs = d->rows > 0 ? dhidden_runs(d->chunk < d->rows ? d->chunk : d->rows, d->H, d->V, d->dtype) : 1;
   float* scal = d->ws;
   float* weights = scal + 2;
   float* terms = weights + d->n_seq;
@@ -545,7 +649,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     if (!grad) continue;
     if (int rc = policy_dlogits(h, d->logits, tile_stats, lse, d->labels + r, coef, n)) return rc;
     if (d->dhidden != nullptr) {
-      if (int rc = dhidden(h, d->logits, d->dhidden + r * d->H, n, BT_FP32, nullptr)) return rc;
+      if (int rc = dhidden_parts(h, d->logits, d->dhidden + r * d->H, n, d->rows * d->H, runs)) return rc;
     }
     if (d->want_dweight && r + n < d->rows) {  // the last chunk's product waits for the upstream gradient
       if (int rc = dweight(h, d->logits, xc, d->dweight_acc, n, BT_FP32, r > 0 ? d->dweight_acc : nullptr, nullptr))

@@ -151,15 +151,17 @@ class LinearLogProbsFunction(torch.autograd.Function):
         n_chunks = -(-rows // step)
         dlogits = torch.empty((step, ld), dtype=x.dtype, device=dev)
         masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev)
+        code = _lib.dtype_code(x.dtype)
+        parts = _f32(dev, int(lib.bt_dhidden_runs(step, hdim, vocab, code)), step, hdim) if need_x else None
         acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
         ws = _f32(dev, rows + 1)
         st = _lib.status_word(dev)
-        with _lib.device_of(dev), _lib.timed("logp_bwd", 2 + n_chunks * (1 + int(need_x) + int(need_w)), dev):
+        with _lib.device_of(dev), _lib.timed("logp_bwd", 2 + n_chunks * (1 + 2 * int(need_x) + int(need_w)), dev):
             rc = lib.bt_logp_bwd(g.data_ptr(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(),
                                  masked.data_ptr(), dlogits.data_ptr(), dx.data_ptr() if need_x else None,
-                                 dw.data_ptr() if need_w else None, acc.data_ptr() if acc is not None else None,
-                                 ws.data_ptr(), rows, hdim, vocab, _ld(x), step, ignore_index,
-                                 _lib.dtype_code(x.dtype), _lib.dtype_code(dw.dtype) if need_w else 0, st.data_ptr(),
+                                 parts.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                                 acc.data_ptr() if acc is not None else None, ws.data_ptr(), rows, hdim, vocab,
+                                 _ld(x), step, ignore_index, code, _lib.dtype_code(dw.dtype) if need_w else 0, st.data_ptr(),
                                  _lib.stream_ptr(dev))
         _lib.check(rc, "bt_logp_bwd")
         return (dx.view(shape) if need_x else None, dw.to(w_dtype) if need_w else None, None, None, None)
@@ -183,13 +185,14 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
     ws = _f32(dev, int(lib.bt_policy_fwd_ws_floats(rows, step, n_seq, vocab)))
     logits = torch.empty((step, ld), dtype=x.dtype, device=dev) if grad else None
     masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
+    code = _lib.dtype_code(x.dtype)
     # fp32 until the upstream gradient is known: one rounding to the hidden states' type
-    dx = _f32(dev, rows, hdim) if need_x else None
+    dx = _f32(dev, int(lib.bt_dhidden_runs(step, hdim, vocab, code)), rows, hdim) if need_x else None
     acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     d = _lib.PolicyDesc(ptr(x), ptr(w), ptr(labels), ptr(old), ptr(adv), ptr(ref), ptr(cu), ptr(logp), ptr(loss),
                         ptr(averages), ptr(dx), ptr(acc), ptr(masked), ptr(logits), ptr(ws), rows, hdim, vocab, _ld(x),
-                        step, n_seq, ignore_index, clip_low, clip_high, kl_coef, int(need_w), _lib.dtype_code(x.dtype))
+                        step, n_seq, ignore_index, clip_low, clip_high, kl_coef, int(need_w), code)
     st = _lib.status_word(dev)
     with _lib.device_of(dev), _lib.timed("policy_fwd", 2 + int(grad) + n_chunks *
                                          (2 + int(grad) + int(need_x) + int(need_w)) - int(need_w), dev):
@@ -227,8 +230,9 @@ class LinearPolicyLossFunction(torch.autograd.Function):
         with _lib.device_of(dev), _lib.timed("policy_bwd", int(need_x) + int(need_w and x_last is not None), dev):
             if need_x:
                 dx_out = torch.empty(shape, dtype=x_dtype, device=dev)
-                _lib.check(lib.bt_scale_cast(dx.data_ptr(), dx_out.data_ptr(), dx.numel(), alpha.data_ptr(),
-                                             _lib.BT_FP32, code, stream), "bt_scale_cast(dhidden)")
+                n = dx_out.numel()
+                _lib.check(lib.bt_sum_runs(dx.data_ptr(), dx_out.data_ptr(), n, dx.shape[0], n, alpha.data_ptr(), code,
+                                           stream), "bt_sum_runs(dhidden)")
             if need_w:
                 dw = _dweight_out(w, w_dtype)
                 if x_last is None:

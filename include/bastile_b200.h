@@ -492,18 +492,24 @@ int64_t bt_logp_fwd_ws_floats(int64_t chunk, int64_t V);
 int bt_logp_fwd(const void* hidden, const void* W, const int64_t* labels, float* logp, float* lse, float* ws,
                 int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
                 int32_t* status, void* stream);
+/* The gradient of hidden has few result tiles against a contraction over the vocabulary, which is therefore
+ * cut into bt_dhidden_runs(min(chunk, rows), H, V, dtype) runs with an fp32 result each. */
+int64_t bt_dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype);
+/* out[n] = alpha * (sum of the runs' parts[n], `stride` elements apart), in `dtype`; n a multiple of 4. */
+int bt_sum_runs(const float* parts, void* out, int64_t n, int64_t runs, int64_t stride, const float* alpha, int dtype,
+                void* stream);
 /* Gradients for the upstream gradient dlogp[rows]; logits are recomputed.  dhidden [rows, H] in `dtype`
- * and dweight [V, H] in dweight_dtype may each be NULL; dweight_acc [V, H] fp32 is needed for dweight when
+ * (with dhidden_parts [runs, min(chunk, rows), H] fp32) and dweight [V, H] in dweight_dtype may each be NULL; dweight_acc [V, H] fp32 is needed for dweight when
  * rows > chunk; ws: rows + 1 floats. */
 int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels, const float* lse,
-                void* masked, void* dlogits, void* dhidden, void* dweight, float* dweight_acc, float* ws, int64_t rows,
-                int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
+                void* masked, void* dlogits, void* dhidden, float* dhidden_parts, void* dweight, float* dweight_acc,
+                float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
                 int dweight_dtype, int32_t* status, void* stream);
 
 /* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
  * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
- * counts).  loss [1], averages [2] = (kl, clipped fraction), logp [rows].  dhidden (fp32 [rows, H], may be
- * NULL) and the weight gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose
+ * counts).  loss [1], averages [2] = (kl, clipped fraction), logp [rows].  dhidden (fp32 [runs, rows, H], may
+ * be NULL) and the weight gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose
  * dlogits stay in `logits`) are relative to ws[0], the largest weight of a token: the caller multiplies by
  * it and the upstream gradient.  masked, logits: needed with either gradient.
  * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats. */

@@ -63,13 +63,18 @@ def test_c_entry_points():
     err(fwd(hidden=C.c_void_p(8)), b"aligned"), err(fwd(ld=60), b"aligned"), err(fwd(ld=56), b"aligned")
     assert fwd(rows=0, hidden=None, labels=None) == 0
 
-    def bwd(dlogp=one, masked=one, dw=one, acc=one, rows=4, chunk=4):
-        return lib.bt_logp_bwd(dlogp, one, one, one, one, masked, one, one, dw, acc, one, rows, 64, 100, 64, chunk,
+    def bwd(dlogp=one, masked=one, parts=one, dw=one, acc=one, rows=4, chunk=4):
+        return lib.bt_logp_bwd(dlogp, one, one, one, one, masked, one, one, parts, dw, acc, one, rows, 64, 100, 64, chunk,
                                -100, b, b, None, None)
 
     err(bwd(dlogp=None), b"null"), err(bwd(masked=None), b"null"), err(bwd(masked=C.c_void_p(24)), b"aligned")
     err(bwd(acc=None, chunk=2), b"accumulator")
+    err(bwd(parts=None), b"parts")
     assert bwd(rows=0) == 0
+    err(lib.bt_sum_runs(one, one, 6, 1, 6, one, b, None), b"sizes"), err(lib.bt_sum_runs(one, one, 8, 2, 4, one, b, None), b"sizes")
+    err(lib.bt_sum_runs(one, None, 8, 1, 8, one, b, None), b"null"), err(lib.bt_sum_runs(one, one, 8, 1, 8, one, 5, None), b"dtype")
+    assert lib.bt_dhidden_runs(517, 1024, 32000, b) > 1 and lib.bt_dhidden_runs(8192, 4096, 4096, b) == 1
+    assert lib.bt_dhidden_runs(0, 64, 100, b) == 1
 
     def policy(**kw):
         d = _lib.PolicyDesc()
