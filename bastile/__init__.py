@@ -15,7 +15,7 @@ from bastile_b200 import *  # noqa: F401,F403
 from bastile_b200 import __all__, __version__  # noqa: F401
 
 for _name in ("autotune", "core", "registry", "ops", "ops.utils", "ops.rms_norm", "ops.rope", "ops.swiglu",
-              "ops.fused_linear_cross_entropy"):
+              "ops.fused_linear_cross_entropy", "ops.fused_linear_policy_loss", "ops.packed_attention"):
     _mod = _importlib.import_module("bastile_b200." + _name)
     _sys.modules[__name__ + "." + _name] = _mod
     if "." not in _name:

@@ -314,7 +314,8 @@ def _describe_status(v: int) -> str:
         parts.append("fused_linear_cross_entropy got a label that is neither ignore_index nor a vocabulary row "
                      "(or fused_linear_log_probs / fused_linear_policy_loss such a target)")
     if v & STATUS_BAD_SEQUENCES:
-        parts.append("sequence offsets do not start at 0, fall, or run past the packed tokens")
+        parts.append("sequence offsets do not start at 0, fall, or run past the packed tokens (or a padding "
+                     "mask has holes, or position ids restart inside a sequence)")
     return "; ".join(parts) or f"status {v:#x}"
 
 

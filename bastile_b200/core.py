@@ -25,6 +25,12 @@ input gradient (``gemm_projections="acc"``, the default; ``"off"`` leaves
 product, or the stacked q|k|v product to the library's own GEMM); the names
 ``"decoder_layer_qwen3"`` and ``"attention_qwen3"`` are then appended to the
 returned list, and ``reset()`` restores both methods.
+
+Another, off by default: ``apply(packed_attention=True)`` makes the packed causal
+attention (``ops/packed_attention.py``) known to transformers under the name
+``"bastile_packed"``, which is appended to the returned list; models built with
+``attn_implementation="bastile_packed"`` use it.  Nothing is replaced, so there is
+nothing for ``reset()`` to undo.
 """
 
 from __future__ import annotations
@@ -122,6 +128,14 @@ def apply(rms_norm: bool = True, swiglu: bool = True, rope: bool = True,
                                                 projections=kwargs.get("gemm_projections", "acc")))
         except Exception as exc:  # patch failures are reported, not raised
             log.warning("Could not apply the fused decoder-layer forwards: %s", exc)
+
+    if kwargs.get("packed_attention", False):
+        try:
+            from .ops.packed_attention import register_with_transformers
+
+            applied.append(register_with_transformers())
+        except Exception as exc:  # patch failures are reported, not raised
+            log.warning("Could not register the packed attention: %s", exc)
 
     if fused_linear_cross_entropy:
         try:

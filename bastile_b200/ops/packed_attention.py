@@ -150,3 +150,78 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, sequences: PackedSequences
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return PackedAttentionFunction.apply(q, k, v, sequences, scale)
     return _forward(q, k, v, sequences, scale, False)[0]
+
+
+# ------------------------------------------------------------------ as an attention of HF transformers
+#: ``attn_implementation`` under which ``apply(packed_attention=True)`` makes the op known to transformers.
+HF_NAME = "bastile_packed"
+
+
+def _padded_offsets(mask: Tensor) -> Tensor:
+    """Offsets of a padded batch: every row of the [B, T] mask is up to three sequences, the padding in
+    front, the tokens, the padding behind (each attends to itself only).  Tokens that are not one run
+    are reported like bad offsets."""
+    b, t = mask.shape
+    m = mask != 0
+    lead = m.to(torch.int32).argmax(dim=1)
+    count = m.sum(dim=1)
+    lead = torch.where(count > 0, lead, torch.zeros_like(lead))
+    start = torch.arange(b, device=mask.device) * t
+    cu = torch.stack((start, start + lead, start + lead + count), dim=1).reshape(-1)
+    pos = torch.arange(t, device=mask.device)
+    holes = (m != ((pos >= lead[:, None]) & (pos < (lead + count)[:, None]))).any()
+    _report(holes)
+    return torch.nn.functional.pad(cu, (0, 1), value=b * t).to(torch.int32)
+
+
+def _report(bad: Tensor) -> None:
+    """Set BT_STATUS_BAD_SEQUENCES in the stream's status word where ``bad`` - without waiting for it."""
+    _lib.status_word(bad.device).bitwise_or_(bad.to(torch.int32) * _lib.STATUS_BAD_SEQUENCES)
+
+
+def hf_packed_mask(batch_size, q_length, kv_length, *args, attention_mask=None, **kwargs):
+    """The mask that transformers prepares once per forward: nothing, or for a padded batch its offsets."""
+    if attention_mask is None:
+        return None
+    if attention_mask.dim() != 2 or attention_mask.shape[1] != q_length or kv_length != q_length:
+        raise ValueError(f"{HF_NAME}: takes [batch, tokens] padding masks and no cached tokens, got a mask of "
+                         f"{tuple(attention_mask.shape)} for {q_length} queries and {kv_length} keys")
+    return _padded_offsets(attention_mask)
+
+
+def hf_packed_attention(module, query, key, value, attention_mask, dropout: float = 0.0, scaling: float | None = None,
+                        sliding_window=None, is_causal=None, cu_seq_lens_q=None, position_ids=None, **kwargs):
+    """``packed_attention`` with the signature of ``ALL_ATTENTION_FUNCTIONS``: query [B, Hq, T, D], key and
+    value [B, Hk, T, D] -> ([B, T, Hq, D], None).  A packed row (B = 1) brings its offsets as
+    ``cu_seq_lens_q`` (transformers' ``DataCollatorWithFlattening(return_flash_attn_kwargs=True)``);
+    otherwise each batch row is a sequence, or what its padding mask leaves of it.  Position ids that
+    restart inside a sequence are reported through the status word."""
+    b, hq, t, d = query.shape
+    if dropout:
+        raise ValueError(f"{HF_NAME}: attention dropout is not supported")
+    if sliding_window is not None or kwargs.get("softcap") is not None or is_causal is False:
+        raise ValueError(f"{HF_NAME}: full causal attention only")
+    if key.shape[2] != t:
+        raise ValueError(f"{HF_NAME}: {t} queries against {key.shape[2]} keys: a cache is not supported, use 'sdpa'")
+    if cu_seq_lens_q is not None:
+        if b != 1:
+            raise ValueError(f"{HF_NAME}: cu_seq_lens_q describes one packed row, got a batch of {b}")
+        cu = cu_seq_lens_q
+    elif attention_mask is not None:
+        cu = attention_mask
+    else:
+        cu = torch.arange(0, (b + 1) * t, max(t, 1), dtype=torch.int32, device=query.device)[:b + 1]
+        if position_ids is not None and t > 1 and getattr(module, "layer_idx", 0) == 0:
+            _report((position_ids[..., 1:] <= position_ids[..., :-1]).any())
+    seqs = pack_sequences(cu, b * t)
+    rows = [x.transpose(1, 2).reshape(b * t, x.shape[1], d) for x in (query, key, value)]
+    return packed_attention(*rows, seqs, scale=scaling).view(b, t, hq, d), None
+
+
+def register_with_transformers() -> str:
+    """Make ``attn_implementation="bastile_packed"`` known to transformers; returns the name."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+
+    AttentionInterface.register(HF_NAME, hf_packed_attention)
+    AttentionMaskInterface.register(HF_NAME, hf_packed_mask)
+    return HF_NAME

@@ -616,7 +616,7 @@ class _LigerPatches:
 
 def train_run(*, dev, rank, world, local, patches="bastile", parallel="single", optimizer="bastile", seq=SEQ_LEN,
               layers=36, intermediate=12288, steps=5, warmup=3, fused_layers=True, gemm_projections="acc",
-              overlap_opt=True, tiles="auto", grad_checkpoint=False, measure_e2e=True, sample_clocks=False,
+              attention="sdpa", overlap_opt=True, tiles="auto", grad_checkpoint=False, measure_e2e=True, sample_clocks=False,
               master_weights=False, sweep=(), bucket_mb=1024, last_bucket_mb=None):
     """Build the model under the given patches / parallel wrapper / optimizer, run `warmup` untimed
     and `steps` timed steps (and, optionally, the same loop fed from pinned host memory), then the
@@ -637,9 +637,11 @@ def train_run(*, dev, rank, world, local, patches="bastile", parallel="single", 
     applied = []
     if patches == "bastile":
         _lib.get_lib().bt_set_gemm_dynamic_tiles(1 if dynamic_tiles else 0)
-        applied = bastile_b200.apply(fused_layers=fused_layers, gemm_projections=gemm_projections)
+        applied = bastile_b200.apply(fused_layers=fused_layers, gemm_projections=gemm_projections,
+                                     packed_attention=attention == "bastile_packed")
         expected = ["rms_norm_qwen3", "rope_qwen3", "swiglu_qwen3"]
         expected += ["decoder_layer_qwen3", "attention_qwen3"] if fused_layers else []
+        expected += [attention] if attention != "sdpa" else []
         assert applied == expected + ["fused_linear_cross_entropy"], applied
     else:
         bastile_b200.reset()
@@ -650,7 +652,7 @@ def train_run(*, dev, rank, world, local, patches="bastile", parallel="single", 
     import transformers.models.qwen3.modeling_qwen3 as q3
 
     cfg = Qwen3Config(**{**QWEN3_8B, "num_hidden_layers": layers, "intermediate_size": intermediate})
-    cfg._attn_implementation = "sdpa"
+    cfg._attn_implementation = attention if patches == "bastile" else "sdpa"
     torch.manual_seed(1234)  # same initial weights on every rank
     prev = torch.get_default_dtype()
     # under FSDP "fp32 master" means fp32 shards that FSDP casts to bf16 for every layer's compute
@@ -925,6 +927,9 @@ def main():
                          "afterwards; dx = their shared input "
                          "gradient from two bt_gemm_ex launches; all = every product of theirs on bt_gemm_ex; qkv = "
                          "q/k/v weights stacked in memory and the three projections run as one product each way")
+    ap.add_argument("--attention", default="sdpa", choices=["sdpa", "bastile_packed"],
+                    help="attention of the patched model: torch's own (what the reference's loop uses) or the "
+                         "library's packed causal attention")
     ap.add_argument("--no-overlap-optimizer", action="store_true",
                     help="single GPU: run the whole AdamW step after the backward pass instead of updating each "
                          "large parameter underneath it as soon as its gradient is complete")
@@ -1002,7 +1007,7 @@ def main():
     fused_layers = not args.no_fused_layers
     grad_checkpoint = args.grad_checkpoint or args.seq >= 32768
     common = dict(dev=dev, rank=rank, world=world, local=local, layers=args.layers, fused_layers=fused_layers,
-                  gemm_projections=args.gemm_projections, tiles=args.tiles)
+                  gemm_projections=args.gemm_projections, attention=args.attention, tiles=args.tiles)
     extras = not args.no_extras and args.layers == QWEN3_8B["num_hidden_layers"]
 
     sweep = []
@@ -1054,7 +1059,7 @@ def main():
                                    "batch 1 fwd+bwd+AdamW, random init",
                        "global_batch_tokens": seq * world, "seq_len": seq,
                        "parallelism": main_run["parallelism"],
-                       "attention": "torch SDPA", "activation_checkpointing": bool(grad_checkpoint),
+                       "attention": "torch SDPA" if args.attention == "sdpa" else args.attention, "activation_checkpointing": bool(grad_checkpoint),
                        "gemm_tiles": main_run["gemm_tiles"], "fused_layers": fused_layers,
                        "gemm_projections": args.gemm_projections if fused_layers else "off",
                        "optimizer": main_run["optimizer_name"],
