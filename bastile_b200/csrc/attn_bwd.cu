@@ -52,50 +52,6 @@ struct BwdGeo {
   static constexpr int kSmem = 7 * kTileBytes + kVecBytes + 512;
 };
 
-template <typename T>
-__host__ __device__ constexpr uint32_t mma_fmt() {
-  return std::is_same<T, __half>::value ? 0u : 1u;
-}
-
-// One tile through the ring slot `dst`: rows from `valid` on are cleared before the consumers see it.
-// Called by the whole load warp; returns false when a wait ran out.
-template <int DT>
-__device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, int head, int token, int valid,
-                                          uint64_t* full, uint64_t* empty, uint32_t empty_parity, uint64_t* fix,
-                                          uint32_t* fix_phase, int lane, volatile int* cta_abort, int32_t* status) {
-  bool ok = true;
-  const bool ragged = valid < kTile;
-  if (lane == 0) {
-    ok = ptx::mbar_wait(empty, empty_parity, cta_abort, status, ST_LOAD);
-    if (ok) {
-      uint64_t* bar = ragged ? fix : full;
-      ptx::mbar_arrive_expect_tx(bar, (DT / 64) * kBoxBytes);
-      load_tile<DT>(dst, tm, head, token, bar);
-      if (ragged) ok = ptx::mbar_wait(fix, *fix_phase, cta_abort, status, ST_LOAD);
-    }
-  }
-  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-  if (ok && ragged) {
-    *fix_phase ^= 1u;
-    zero_rows<DT>(dst, valid, lane);
-    if (lane == 0) ptx::mbar_arrive(full);
-  }
-  return ok;
-}
-
-// The tiles need a 1024-byte start, which is where dynamic shared memory begins when a kernel has no
-// other; should that ever change, the call reports itself as failed instead of reading wrong tiles.
-__device__ __forceinline__ bool aligned_start(const uint8_t* smem, int32_t* status) {
-  const bool ok = (ptx::smem_u32(smem) & 1023u) == 0;
-  if (!ok && threadIdx.x == 0 && status != nullptr) atomicOr(status, ST_LOAD);
-  return ok;
-}
-
-__device__ __forceinline__ void drain_copies() {
-  const uint64_t t0 = ptx::globaltimer_ns();
-  while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-}
-
 // 32 accumulator columns of one row, scaled and stored.
 template <typename T>
 __device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, int col0, int d, float scale, bool row_ok) {

@@ -2,14 +2,16 @@
 //
 //   O_i = sum_{j <= i} P_ij V_j,   P_ij = exp(scale q_i.k_j - lse_i),   i, j in the same sequence
 //
-// One CTA per (two consecutive query tiles of 128 packed rows, key/value head): 384 threads,
-//   warps 0..3 / 4..7  softmax of tile 0 / tile 1, one row per thread, then the tile's epilogue
-//   warp 8             issues tcgen05.mma:  S_t = Q_t K_j^T,  O_t += P_t V_j
-//   warp 9             TMA loads: Q once, then K_0, V_0, K_1, ... through one ring
-// (warps 10, 11 complete the warpgroup that hands its registers to the softmax warps).
-// Tensor memory (512 columns): S_0, S_1 (fp32, 128 columns each; P_t in 16 bits replaces the first
-// half of S_t and is the A operand of the second product), O_0, O_1 (fp32).  While the softmax of one
-// tile runs, the tensor pipe works on the other tile.
+// One CTA per (query tile of 128 packed rows, key/value head), two CTAs on an SM: 256 threads,
+//   warps 0..3  softmax, one row per thread, and the epilogue
+//   warp 4      issues tcgen05.mma:  S = Q K_j^T,  O += P_j V_j
+//   warp 5      TMA loads: Q once, then K_0, V_0, K_1, ... (one tile of each at a time)
+// (warps 6, 7 complete the warpgroup that hands its registers to the softmax warps).
+// Tensor memory (256 columns): S (fp32, 128 columns; the 16-bit P replaces the first half and is the A
+// operand of the second product) and O.  A key block takes a CTA about 3600 cycles - scores, softmax,
+// second product - of which its products are 1050 and its exponentials 1024: the other CTA's products
+// and exponentials run meanwhile, and under its start and its end as well, which no second tile inside
+// one CTA can do (measured: see attn_fwd_kernel).
 #include <mutex>
 
 #include "attn_sm100.cuh"
@@ -82,13 +84,12 @@ attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* 
 }
 
 // --------------------------------------------------------------- the forward
-constexpr int kFwdThreads = 384;
+constexpr int kFwdThreads = 256;
 
 template <int DT>
 struct FwdGeo {
   static constexpr int kTileBytes = (DT / 64) * kBoxBytes;
-  static constexpr int kStages = DT == 128 ? 5 : 8;
-  static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024 + 1024;
+  static constexpr int kSmem = 3 * kTileBytes + 512;  // Q, K, V and the barriers: two CTAs fit an SM
 };
 
 // Rescaling the output accumulator is put off until a row's maximum has grown by more than this many
@@ -96,37 +97,32 @@ struct FwdGeo {
 constexpr float kLazyMax = 8.0f;
 
 template <typename T, int DT>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const Params p) {
   using G = FwdGeo<DT>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  const uint32_t sQ = ptx::smem_u32(smem);
-  const uint32_t sRing = sQ + 2 * G::kTileBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + (2 + G::kStages) * G::kTileBytes);  // [2]
-  uint64_t* full = q_full + 2;
-  uint64_t* empty = full + G::kStages;
-  uint64_t* s_full = empty + G::kStages;  // [2]
-  uint64_t* p_ready = s_full + 2;         // [2]
-  uint64_t* pv_done = p_ready + 2;        // [2]
-  uint64_t* fix = pv_done + 2;
+  constexpr int TB = G::kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (!aligned_start(smem, p.status)) return;
+  const uint32_t sQ = ptx::smem_u32(smem), sK = sQ + TB, sV = sK + TB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + 3 * TB);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* v_full = k_full + 1;
+  uint64_t* s_full = v_full + 1;   // phase j: scores j are there, and K_j may be replaced
+  uint64_t* p_ready = s_full + 1;
+  uint64_t* pv_done = p_ready + 1; // phase j: block j is in O, and V_j may be replaced
+  uint64_t* fix = pv_done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(&q_full[i], 1);
-      ptx::mbar_init(&s_full[i], 1);
-      ptx::mbar_init(&p_ready[i], 4);
-      ptx::mbar_init(&pv_done[i], 1);
-    }
-    for (int i = 0; i < G::kStages; ++i) {
-      ptx::mbar_init(&full[i], 1);
-      ptx::mbar_init(&empty[i], 1);
-    }
+    ptx::mbar_init(q_full, 1);
+    ptx::mbar_init(k_full, 1);
+    ptx::mbar_init(v_full, 1);
+    ptx::mbar_init(s_full, 1);
+    ptx::mbar_init(p_ready, 4);
+    ptx::mbar_init(pv_done, 1);
     ptx::mbar_init(fix, 1);
     *cta_abort = 0;
     ptx::fence_mbar_init();
@@ -134,242 +130,167 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     ptx::prefetch_tensormap(&tmK);
     ptx::prefetch_tensormap(&tmV);
   }
-  if (warp == 8) {
-    ptx::tmem_alloc(tmem_slot, 512);
+  if (warp == 4) {
+    ptx::tmem_alloc(tmem_slot, 256);
     ptx::tmem_relinquish_alloc_permit();
   }
-  ptx::tcgen05_fence_before_sync();
-  __syncthreads();
-  ptx::tcgen05_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
-
   const int groups = p.hk * p.nsub;
   const int hs = static_cast<int>(blockIdx.x) % groups;
   Item it{};
   const bool live = plan_item(p.plan, p.gran, static_cast<int>(blockIdx.x) / groups, lane, &it);
-  const int span = 2 * p.tq;  // tokens of the two tiles
-  const bool behind = live && it.entry == p.plan.n - 1;
-  const int first = live ? (behind ? it.tile : (it.len + span - 1) / span - 1 - it.tile) * span : 0;
-  const int kv_end = live ? min(it.len, first + span) : 0;
-  const int nblk = (live && !behind) ? (kv_end + kTile - 1) / kTile : 0;
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
 
-  // 384 x 168 registers at launch = 2 x 128 x 208 + 128 x 88
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 9 && nblk > 0) {
-      // ------------------------------------------------------------------ loads
-      bool ok = true;
+  const bool behind = live && it.entry == p.plan.n - 1;
+  const int first = live ? (behind ? it.tile : (it.len + p.tq - 1) / p.tq - 1 - it.tile) * p.tq : 0;
+  const int n = (live && !behind) ? (min(it.len, first + p.tq) + kTile - 1) / kTile : 0;  // key blocks
+
+  // 256 x 128 registers at launch = 128 x 192 + 128 x 64
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 5 && n > 0) {
+      // ---------------------------------------------------------------- loads
       if (lane == 0) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ptx::mbar_arrive_expect_tx(&q_full[t], G::kTileBytes);
-          load_tile<DT>(sQ + t * G::kTileBytes, &tmQ, hs * p.gp, it.start + first + t * p.tq, &q_full[t]);
-        }
+        ptx::mbar_arrive_expect_tx(q_full, TB);
+        load_tile<DT>(sQ, &tmQ, hs * p.gp, it.start + first, q_full);
       }
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int i = 0; i < 2 * nblk; ++i) {
-        const int kv0 = (i >> 1) * kTile;
-        const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
-        const uint32_t dst = sRing + stage * G::kTileBytes;
+      uint32_t fix_phase = 0;
+      bool ok = true;
+      for (int j = 0; ok && j < n; ++j) {
+        const uint32_t par = (j & 1) ^ 1u;
         // rows of V behind the sequence meet P = 0, which is only harmless if they are finite: they are
         // cleared before the product reads them (rows of K give columns that the mask overwrites)
-        const bool ragged = (i & 1) && kv0 + kTile > it.len;
-        if (lane == 0) {
-          ok = ptx::mbar_wait(&empty[stage], phase ^ 1u, cta_abort, p.status, ST_LOAD);
-          if (ok) {
-            uint64_t* bar = ragged ? fix : &full[stage];
-            ptx::mbar_arrive_expect_tx(bar, G::kTileBytes);
-            load_tile<DT>(dst, tm, hs / p.nsub, it.start + kv0, bar);
-            if (ragged) ok = ptx::mbar_wait(fix, 0, cta_abort, p.status, ST_LOAD);
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        ok = ring_load<DT>(sK, &tmK, hs / p.nsub, it.start + j * kTile, kTile, k_full, s_full, par, fix, &fix_phase,
+                           lane, cta_abort, p.status) &&
+             ring_load<DT>(sV, &tmV, hs / p.nsub, it.start + j * kTile, min(kTile, it.len - j * kTile), v_full,
+                           pv_done, par, fix, &fix_phase, lane, cta_abort, p.status);
+      }
+      if (!ok || *cta_abort != 0) drain_copies();
+    } else if (warp == 4 && n > 0) {
+      // ----------------------------------------------------------- MMA issuer
+      constexpr uint32_t id_s = ptx::make_idesc(mma_fmt<T>(), false, false, 128, 128);
+      constexpr uint32_t id_o = ptx::make_idesc(mma_fmt<T>(), false, true, 128, DT);
+      bool ok = warp_wait(q_full, 0, cta_abort, p.status, ST_ISSUE) &&
+                warp_wait(k_full, 0, cta_abort, p.status, ST_ISSUE);
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        mma_abt<DT>(tmem, sQ, sK, id_s);
+        mma_commit(s_full);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        ok = warp_wait(v_full, j & 1, cta_abort, p.status, ST_ISSUE) &&
+             warp_wait(p_ready, j & 1, cta_abort, p.status, ST_ISSUE2);
         if (!ok) break;
-        if (ragged) {
-          zero_rows<DT>(dst, it.len - kv0, lane);
-          if (lane == 0) ptx::mbar_arrive(&full[stage]);
-        }
-        if (++stage == G::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!ok || *cta_abort != 0) {  // copies in flight land before the shared memory is handed on
-        const uint64_t t0 = ptx::globaltimer_ns();
-        while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-      }
-    } else if (warp == 8 && nblk > 0) {
-      // ------------------------------------------------------------- MMA issuer
-      {
-        constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0u : 1u;
-        constexpr uint32_t id_s = ptx::make_idesc(fmt, false, false, 128, 128);
-        constexpr uint32_t id_o = ptx::make_idesc(fmt, false, true, 128, DT);
-        const uint32_t o0 = tmem + 256;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = warp_wait(&full[0], 0, cta_abort, p.status, ST_ISSUE);
-        for (int t = 0; ok && t < 2; ++t) {
-          ok = warp_wait(&q_full[t], 0, cta_abort, p.status, ST_ISSUE);
+        ptx::tcgen05_fence_after_sync();
+        mma_pb<DT>(tmem + 128, tmem, tmem + 32, sV, id_o, j > 0);
+        mma_commit(pv_done);
+        if (j + 1 < n) {
+          ok = warp_wait(k_full, (j + 1) & 1, cta_abort, p.status, ST_ISSUE);
           if (!ok) break;
           ptx::tcgen05_fence_after_sync();
-          mma_abt<DT>(tmem + t * 128, sQ + t * G::kTileBytes, sRing, id_s);
-          mma_commit(&s_full[t]);
-        }
-        if (ok) mma_commit(&empty[0]);
-        stage = 1;
-        for (int j = 0; ok && j < nblk; ++j) {
-          const int v_stage = stage;
-          ok = warp_wait(&full[v_stage], phase, cta_abort, p.status, ST_ISSUE);
-          if (!ok) break;
-          if (++stage == G::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          const int k_stage = stage;
-          const bool more = j + 1 < nblk;
-          const uint32_t k_phase = phase;
-          if (more && ++stage == G::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            ok = warp_wait(&p_ready[t], j & 1, cta_abort, p.status, ST_ISSUE2);
-            if (!ok) break;
-            ptx::tcgen05_fence_after_sync();
-            const uint32_t pt = tmem + t * 128;
-            mma_pb<DT>(o0 + t * DT, pt, pt + 32, sRing + v_stage * G::kTileBytes, id_o, j > 0);
-            mma_commit(&pv_done[t]);
-            if (more) {
-              if (t == 0) {
-                ok = warp_wait(&full[k_stage], k_phase, cta_abort, p.status, ST_ISSUE);
-                if (!ok) break;
-                ptx::tcgen05_fence_after_sync();
-              }
-              mma_abt<DT>(pt, sQ + t * G::kTileBytes, sRing + k_stage * G::kTileBytes, id_s);
-              mma_commit(&s_full[t]);
-            }
-          }
-          if (!ok) break;
-          mma_commit(&empty[v_stage]);
-          if (more) mma_commit(&empty[k_stage]);
+          mma_abt<DT>(tmem, sQ, sK, id_s);
+          mma_commit(s_full);
         }
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------- softmax and epilogue
-    if (live) {
-      const int t = warp >> 2;
-      const int row = (warp & 3) * 32 + lane;
-      const int tok = first + t * p.tq + (row >> p.gp_shift);
-      const int head = hs * p.gp + (row & (p.gp - 1));
-      const int64_t token = static_cast<int64_t>(it.start) + tok;
-      const bool row_ok = tok < it.len;
-      T* out = static_cast<T*>(p.o.ptr) + token * p.o.st + head * p.o.sh;
-      if (behind) {
-        if (row_ok)
-          for (int c = 0; c < p.d; c += 8) st_global_v4(out + c, make_uint4(0, 0, 0, 0));
-      } else {
-        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lane_base + t * 128;
-        const uint32_t to = tmem + lane_base + 256 + t * DT;
-        const int lim = min(tok, it.len - 1);  // last key this row sees
-        const int safe = min(first + t * p.tq, it.len - 1);  // last key that every row of the tile sees
-        const float c = p.scale_log2;
-        float m = 0.f, l = 0.f;
-        bool ok = true;
-        for (int j = 0; j < nblk; ++j) {
-          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], j & 1, cta_abort, p.status, ST_MATH));
-          if (!ok) break;
-          ptx::tcgen05_fence_after_sync();
-          float s[128];
+    const int row = warp * 32 + lane;
+    const int tok = first + (row >> p.gp_shift);
+    const int head = hs * p.gp + (row & (p.gp - 1));
+    const int64_t token = static_cast<int64_t>(it.start) + tok;
+    const bool row_ok = live && tok < it.len;
+    T* out = static_cast<T*>(p.o.ptr) + token * p.o.st + head * p.o.sh;
+    if (behind && row_ok)
+      for (int c = 0; c < p.d; c += 8) st_global_v4(out + c, make_uint4(0, 0, 0, 0));
+    if (n > 0) {
+      const uint32_t ts = tmem + (static_cast<uint32_t>(warp * 32) << 16), to = ts + 128;
+      const int lim = min(tok, it.len - 1);     // last key this row sees
+      const int safe = min(first, it.len - 1);  // last key that every row of the tile sees
+      const float c = p.scale_log2;
+      float m = 0.f, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        ok = warp_wait(s_full, j & 1, cta_abort, p.status, ST_MATH);
+        if (!ok) break;
+        ptx::tcgen05_fence_after_sync();
+        float s[128];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) tmem_ld32(ts + q * 32, s + q * 32);
-          tmem_wait_ld();
-          if (j * kTile + kTile - 1 > safe) {
-            const int last = lim - j * kTile;
+        for (int q = 0; q < 4; ++q) tmem_ld32(ts + q * 32, s + q * 32);
+        tmem_wait_ld();
+        if (j * kTile + kTile - 1 > safe) {
+          const int last = lim - j * kTile;
 #pragma unroll
-            for (int e = 0; e < 128; ++e) s[e] = e <= last ? s[e] : -INFINITY;
-          }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int e = 4; e < 128; e += 8) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (e + 4 + q < 128) mx[q] = fmaxf(mx[q], fmaxf(s[e + q], s[e + 4 + q]));
-              else mx[q] = fmaxf(mx[q], s[e + q]);
-            }
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (j == 0) {
-            m = fmaxf(top, -1e30f);  // finite, should a whole block score -inf
-          } else {
-            const bool grow = (top - m) * c > kLazyMax;
-            if (__any_sync(0xffffffffu, grow)) {
-              // the tile's previous product has to be in O before O is rescaled
-              ok = __all_sync(0xffffffffu,
-                              ptx::mbar_wait(&pv_done[t], (j - 1) & 1, cta_abort, p.status, ST_MATH));
-              if (!ok) break;
-              ptx::tcgen05_fence_after_sync();
-              const float nm = fmaxf(m, top);
-              const float alpha = ex2((m - nm) * c);
-              m = nm;
-              l *= alpha;
-#pragma unroll 1
-              for (int q = 0; q < DT / 32; ++q) {
-                float o[32];
-                tmem_ld32(to + q * 32, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= alpha;
-                tmem_st32(to + q * 32, o);
-              }
-              tmem_wait_st();
-            }
-          }
-          const f32x2 c2 = pair(c, c), mc2 = pair(-m * c, -m * c);
-          f32x2 sum2 = pair(0.f, 0.f);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const f32x2 x = fma2(pair(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), c2, mc2);
-              const float a = ex2(lo_of(x)), b = ex2(hi_of(x));
-              sum2 = add2(sum2, pair(a, b));
-              pk[e] = pack2<T>(a, b);  // the product's operand type; the sum keeps fp32
-            }
-            tmem_st16(ts + q * 16, pk);
-          }
-          l += lo_of(sum2) + hi_of(sum2);
-          tmem_wait_st();
-          ptx::tcgen05_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&p_ready[t]);
+          for (int e = 0; e < 128; ++e) s[e] = e <= last ? s[e] : -INFINITY;
         }
-        if (ok)
-          ok = __all_sync(0xffffffffu,
-                          ptx::mbar_wait(&pv_done[t], (nblk - 1) & 1, cta_abort, p.status, ST_MATH));
-        if (ok) {
-          ptx::tcgen05_fence_after_sync();
-          const float inv = 1.0f / l;
-          if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int e = 4; e < 124; e += 8) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(s[e + q], s[e + 4 + q]));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[124 + q]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (j == 0) {
+          m = fmaxf(top, -1e30f);  // finite, should a whole block score -inf
+        } else if (__any_sync(0xffffffffu, (top - m) * c > kLazyMax)) {
+          // (the blocks before are in O: scores j were computed behind them)
+          const float nm = fmaxf(m, top);
+          const float alpha = ex2((m - nm) * c);
+          m = nm;
+          l *= alpha;
 #pragma unroll 1
           for (int q = 0; q < DT / 32; ++q) {
             float o[32];
             tmem_ld32(to + q * 32, o);
             tmem_wait_ld();
-            if (row_ok) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t w[4];
+            for (int e = 0; e < 32; ++e) o[e] *= alpha;
+            tmem_st32(to + q * 32, o);
+          }
+        }
+        const f32x2 c2 = pair(c, c), mc2 = pair(-m * c, -m * c);
+        f32x2 sum2 = pair(0.f, 0.f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = pack2<T>(o[v * 8 + 2 * e] * inv, o[v * 8 + 2 * e + 1] * inv);
-                if (q * 32 + v * 8 < p.d) st_global_v4(out + q * 32 + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
-              }
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const f32x2 x = fma2(pair(s[q * 32 + 2 * e], s[q * 32 + 2 * e + 1]), c2, mc2);
+            const float a = ex2(lo_of(x)), b = ex2(hi_of(x));
+            sum2 = add2(sum2, pair(a, b));
+            pk[e] = pack2<T>(a, b);  // the product's operand type; the sum keeps fp32
+          }
+          tmem_st16(ts + q * 16, pk);
+        }
+        tmem_wait_st();
+        ptx::tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready);
+        l += lo_of(sum2) + hi_of(sum2);
+      }
+      ok = ok && warp_wait(pv_done, (n - 1) & 1, cta_abort, p.status, ST_MATH);
+      if (ok) {
+        ptx::tcgen05_fence_after_sync();
+        const float inv = 1.0f / l;
+        if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
+#pragma unroll 1
+        for (int q = 0; q < DT / 32; ++q) {
+          float o[32];
+          tmem_ld32(to + q * 32, o);
+          tmem_wait_ld();
+          if (row_ok) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack2<T>(o[v * 8 + 2 * e] * inv, o[v * 8 + 2 * e + 1] * inv);
+              if (q * 32 + v * 8 < p.d) st_global_v4(out + q * 32 + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
             }
           }
         }
@@ -378,9 +299,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   }
   ptx::tcgen05_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4) {
     ptx::tcgen05_fence_after_sync();
-    ptx::tmem_dealloc(tmem, 512);
+    ptx::tmem_dealloc(tmem, 256);
   }
 }
 
@@ -390,7 +311,7 @@ int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
   auto* kern = attn_fwd_kernel<T, DT>;
   static std::atomic<uint64_t> reserved{0};
   BT_CHECK_LAUNCHED(reserve_smem(kern, FwdGeo<DT>::kSmem, &reserved), "attn_fwd: shared memory");
-  const int64_t grid = max_items(p.total, batch, 2 * p.tq) * p.hk * p.nsub;
+  const int64_t grid = max_items(p.total, batch, p.tq) * p.hk * p.nsub;
   BT_CHECK_ARG(grid <= 0x7fffffffll, "attn_fwd: too many tiles (%lld)", (long long)grid);
   BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdGeo<DT>::kSmem, s,
                                      q, k, v, p),
@@ -462,6 +383,7 @@ int fill_params(Params* p, const char* what, const int32_t* plan, int64_t batch,
                what);
   BT_CHECK_ARG(d >= 8 && d <= 128 && d % 8 == 0, "%s: head_dim must be a multiple of 8, at most 128 (got %lld)", what,
                (long long)d);
+  BT_CHECK_ARG(scale >= 0.f && scale <= 1e30f, "%s: scale must be finite and not negative (got %g)", what, scale);
   p->plan.words = plan;
   p->plan.n = static_cast<int>(batch) + 1;
   p->hq = static_cast<int>(hq);
@@ -516,7 +438,7 @@ extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* ou
   if (int rc = check_view("attn_fwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;
   if (int rc = check_view("attn_fwd v", v, v_strides[0], v_strides[1], nk, total)) return rc;
   if (int rc = check_view("attn_fwd out", out, o_strides[0], o_strides[1], nq, total)) return rc;
-  p.gran = gran_index(2 * p.tq);
+  p.gran = gran_index(p.tq);
   p.lse2 = lse2;
   p.o = View{out, o_strides[0], o_strides[1]};
   p.status = status;

@@ -29,7 +29,7 @@ enum : int { ST_LOAD = 1, ST_ISSUE = 2, ST_ISSUE2 = 4, ST_MATH = 8 };
 // int32 words written once per batch by bt_attn_plan: start[n], len[n] of the n = batch + 1 entries
 // (the sequences, longest first when there are at most kPlanSort of them, then the rows behind the
 // last sequence), then for each tile height kGran[g] the n + 1 running tile counts.
-constexpr int kGrans = 6;
+constexpr int kGrans = 5;
 constexpr int kPlanSort = 1024;
 __host__ __device__ constexpr int gran_of(int g) { return 8 << g; }
 __host__ __device__ inline int gran_index(int tokens) {
@@ -48,12 +48,14 @@ struct Item {
   int start, len, tile, entry;  // entry == n - 1: rows behind the last sequence
 };
 
-// The item-th tile of height kGran[g] (one warp; all lanes get the answer); false: no such tile.
+// The item-th tile of height gran_of(g) (one warp; all lanes get the answer); false: no such tile.
+// Every CTA waits for this before its first load, so the reads of a round do not wait for one another:
+// up to 32 entries take one round, up to 1024 two.
 __device__ __forceinline__ bool plan_item(const Plan& p, int g, int item, int lane, Item* it) {
   const int32_t* pre = p.words + 2 * p.n + g * (p.n + 1);
+  const int total = __ldg(pre + p.n);
   int lo = 0, hi = p.n;
-  if (item >= __ldg(pre + hi)) return false;
-  while (hi - lo > 1) {  // invariant: pre[lo] <= item < pre[hi]; 32 probes a round
+  while (hi - lo > 32) {  // invariant: pre[lo] <= item < pre[hi]; 32 probes a round
     const int step = (hi - lo + 31) / 32;
     const int at = lo + (lane + 1) * step;
     const bool le = at < hi && __ldg(pre + at) <= item;
@@ -62,10 +64,14 @@ __device__ __forceinline__ bool plan_item(const Plan& p, int g, int item, int la
     lo = base + c * step;
     hi = min(base + (c + 1) * step, hi);
   }
-  it->entry = lo;
-  it->start = __ldg(p.words + lo);
-  it->len = __ldg(p.words + p.n + lo);
-  it->tile = item - __ldg(pre + lo);
+  const int at = min(lo + lane, p.n - 1);
+  const int first = __ldg(pre + at), start = __ldg(p.words + at), len = __ldg(p.words + p.n + at);
+  if (item >= total) return false;
+  const int src = __popc(__ballot_sync(0xffffffffu, lo + lane < hi && first <= item)) - 1;
+  it->entry = lo + src;
+  it->start = __shfl_sync(0xffffffffu, start, src);
+  it->len = __shfl_sync(0xffffffffu, len, src);
+  it->tile = item - __shfl_sync(0xffffffffu, first, src);
   return true;
 }
 
@@ -219,6 +225,50 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int first, int lane) {
       ptx::st_shared_v4(tile + j * kBoxBytes + i * 16, make_uint4(0, 0, 0, 0));
   ptx::fence_proxy_async_smem();
   __syncwarp();
+}
+
+// The tiles need a 1024-byte start, which is where dynamic shared memory begins when a kernel has no
+// other; should that ever change, the call reports itself as failed instead of reading wrong tiles.
+__device__ __forceinline__ bool aligned_start(const uint8_t* smem, int32_t* status) {
+  const bool ok = (ptx::smem_u32(smem) & 1023u) == 0;
+  if (!ok && threadIdx.x == 0 && status != nullptr) atomicOr(status, ST_LOAD);
+  return ok;
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t mma_fmt() {
+  return std::is_same<T, __half>::value ? 0u : 1u;
+}
+
+// One tile through the ring slot `dst`: rows from `valid` on are cleared before the consumers see it.
+// Called by the whole load warp; returns false when a wait ran out.
+template <int DT>
+__device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, int head, int token, int valid,
+                                          uint64_t* full, uint64_t* empty, uint32_t empty_parity, uint64_t* fix,
+                                          uint32_t* fix_phase, int lane, volatile int* cta_abort, int32_t* status) {
+  bool ok = true;
+  const bool ragged = valid < kTile;
+  if (lane == 0) {
+    ok = ptx::mbar_wait(empty, empty_parity, cta_abort, status, ST_LOAD);
+    if (ok) {
+      uint64_t* bar = ragged ? fix : full;
+      ptx::mbar_arrive_expect_tx(bar, (DT / 64) * kBoxBytes);
+      load_tile<DT>(dst, tm, head, token, bar);
+      if (ragged) ok = ptx::mbar_wait(fix, *fix_phase, cta_abort, status, ST_LOAD);
+    }
+  }
+  ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  if (ok && ragged) {
+    *fix_phase ^= 1u;
+    zero_rows<DT>(dst, valid, lane);
+    if (lane == 0) ptx::mbar_arrive(full);
+  }
+  return ok;
+}
+
+__device__ __forceinline__ void drain_copies() {
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
 }
 
 // What every kernel is told about one [tokens, heads, head_dim] tensor besides its tile map.

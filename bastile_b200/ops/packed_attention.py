@@ -145,8 +145,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, sequences: PackedSequences
         raise TypeError(f"packed_attention: q, k and v must share bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
     if t != sequences.total_tokens:
         raise ValueError(f"packed_attention: q has {t} tokens, the packed sequences {sequences.total_tokens}")
-    _lib.require_cuda(q, k, v, sequences.plan)
     scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= scale <= 1e30:
+        raise ValueError(f"packed_attention: scale must be finite and not negative, got {scale}")
+    _lib.require_cuda(q, k, v, sequences.plan)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return PackedAttentionFunction.apply(q, k, v, sequences, scale)
     return _forward(q, k, v, sequences, scale, False)[0]

@@ -40,6 +40,9 @@ def test_mismatched_tensors_and_plans():
         packed_attention(q[0], k, v, _seqs(4))
     with pytest.raises(TypeError, match="share"):
         packed_attention(q, k.half(), v, _seqs(4))
+    for scale in (-0.1, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            packed_attention(q, k, v, _seqs(4), scale=scale)
     with pytest.raises(RuntimeError, match="CUDA"):
         packed_attention(q, k, v, _seqs(4))
     with pytest.raises(ValueError, match="batch"):
@@ -61,14 +64,14 @@ def test_c_entry_points():
     one = C.c_void_p(16)  # never dereferenced: validation fails before any launch
     good, bad = _lib.I64x2(256, 64), _lib.I64x2(250, 64)
 
-    def fwd(q=one, batch=1, total=4, hq=4, hk=2, d=64, qs=good, dtype=_lib.BT_BF16, plan=one):
-        return lib.bt_attn_fwd(q, one, one, one, None, plan, batch, total, hq, hk, d, qs, good, good, good, 0.1, dtype,
-                               None, None)
+    def fwd(q=one, batch=1, total=4, hq=4, hk=2, d=64, qs=good, dtype=_lib.BT_BF16, plan=one, scale=0.1):
+        return lib.bt_attn_fwd(q, one, one, one, None, plan, batch, total, hq, hk, d, qs, good, good, good, scale,
+                               dtype, None, None)
 
     for kw, text in ((dict(q=None), b"null"), (dict(plan=None), b"null plan"), (dict(hq=3), b"multiple"),
                      (dict(d=68), b"head_dim"), (dict(d=256), b"head_dim"), (dict(dtype=_lib.BT_FP32), b"dtype"),
                      (dict(qs=bad), b"strides"), (dict(q=C.c_void_p(8)), b"aligned"), (dict(total=0), b"token count"),
-                     (dict(total=1 << 30), b"token count"), (dict(batch=-1), b"batch")):
+                     (dict(total=1 << 30), b"token count"), (dict(batch=-1), b"batch"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale")):
         assert fwd(**kw) == -1 and text in lib.bt_last_error(), (kw, lib.bt_last_error())
 
     def bwd(dk=one, dv=one, lse=one):
@@ -80,4 +83,4 @@ def test_c_entry_points():
     assert bwd() == -1 and b"dv" in lib.bt_last_error()
     assert lib.bt_attn_plan(None, 1, 4, one, None, None) == -1 and b"null" in lib.bt_last_error()
     assert lib.bt_attn_plan(one, -1, 4, one, None, None) == -1
-    assert lib.bt_attn_plan_words(-1) == 0 and lib.bt_attn_plan_words(3) == 4 * 2 + 6 * 5
+    assert lib.bt_attn_plan_words(-1) == 0 and lib.bt_attn_plan_words(3) == 4 * 2 + 5 * 5
