@@ -17,29 +17,47 @@ namespace {
 constexpr int kBwdThreads = 384;
 
 // ------------------------------------------------------------------ D = dO . O
-// Half a warp per (token, head) row, 16 bytes of each tensor per lane.
+// Half a warp per (token, head) row, 16 bytes of each tensor per lane, four rows in flight.  Bound by
+// memory.
 template <typename T>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* __restrict__ delta, int64_t rows,
                   int heads, int64_t total, int d, int64_t o_st, int64_t o_sh, int64_t g_st, int64_t g_sh) {
   grid_dependency_wait();
+  constexpr int kRows = 4;
   const int sub = threadIdx.x & 15;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 16;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16; r0 < rows; r0 += step) {
-    const int64_t r = r0 + (threadIdx.x >> 4);
-    float acc = 0.f;
-    const int64_t tok = r / heads;
-    const int head = static_cast<int>(r - tok * heads);
-    if (r < rows && sub * 8 < d) {
-      float a[8], b[8];
-      Cvt<T>::unpack(ld_stream_v4(out + tok * o_st + head * o_sh + sub * 8), a);
-      Cvt<T>::unpack(ld_global_v4(dout + tok * g_st + head * g_sh + sub * 8), b);
+  const bool live = sub * 8 < d;
+  const bool small = rows <= 0xffffffffll;  // a 64-bit division costs more than the row's arithmetic
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 16 * kRows;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16 * kRows; r0 < rows; r0 += step) {
+    uint4 a[kRows], b[kRows];
+    int64_t at[kRows];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc = fmaf(a[e], b[e], acc);
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
+      a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      at[i] = -1;
+      if (r < rows) {
+        const int64_t tok = small ? static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(heads)) : r / heads;
+        const int64_t head = r - tok * heads;
+        at[i] = head * total + tok;
+        if (live) {
+          a[i] = ld_stream_v4(out + tok * o_st + head * o_sh + sub * 8);
+          b[i] = ld_global_v4(dout + tok * g_st + head * g_sh + sub * 8);
+        }
+      }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (r < rows && sub == 0) delta[head * total + tok] = acc;
+    for (int i = 0; i < kRows; ++i) {
+      float x[8], y[8], acc = 0.f;
+      Cvt<T>::unpack(a[i], x);
+      Cvt<T>::unpack(b[i], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc = fmaf(x[e], y[e], acc);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      if (at[i] >= 0 && sub == 0) delta[at[i]] = acc;
+    }
   }
 }
 
@@ -653,7 +671,7 @@ template <typename T>
 int run_delta(const void* out, const void* dout, float* delta, int64_t total, int64_t hq, int64_t d,
               const int64_t* os, const int64_t* gs, cudaStream_t s) {
   const int64_t rows = total * hq;
-  const int64_t want = ceil_div(rows, 16), cap = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t want = ceil_div(rows, 64), cap = static_cast<int64_t>(sm_count()) * 8;
   BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(static_cast<unsigned>(want < cap ? want : cap)),
                                      dim3(256), 0, s, static_cast<const T*>(out), static_cast<const T*>(dout), delta,
                                      rows, static_cast<int>(hq), total, static_cast<int>(d), os[0], os[1], gs[0],
