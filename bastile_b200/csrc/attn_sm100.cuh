@@ -10,7 +10,6 @@
 // 128 rows x 128 bytes with the 128-byte TMA swizzle.  A head_dim below DT is zero-filled by TMA.
 #pragma once
 
-#include <atomic>
 #include <type_traits>
 
 #include "bt_common.cuh"
@@ -294,19 +293,6 @@ struct Params {
 inline void bind_context() {
   int dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
-}
-
-// Reserve a kernel's dynamic shared memory, once per device (the attribute belongs to the device's copy
-// of the kernel; setting it twice does no harm).
-template <typename K>
-inline cudaError_t reserve_smem(K* kern, int bytes, std::atomic<uint64_t>* done) {
-  int dev = 0;
-  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
-  if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-  done->fetch_or(bit, std::memory_order_release);
-  return cudaSuccess;
 }
 
 // Host side (attn_fwd.cu)

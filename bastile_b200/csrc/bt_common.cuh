@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -218,6 +219,19 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Reserve a kernel's dynamic shared memory, once per device (the attribute belongs to the device's copy
+// of the kernel; setting it twice does no harm).
+template <typename K>
+inline cudaError_t reserve_smem(K* kern, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  done->fetch_or(bit, std::memory_order_release);
+  return cudaSuccess;
+}
 
 // Programmatic dependent launch: a kernel launched through launch_dependent() may be set up on
 // the SMs (its CTAs scheduled, their prologues run) while the previous kernel of the stream is

@@ -1340,12 +1340,9 @@ template <int EPI, typename T>
 int launch_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
              const CUtensorMap& b1, const CUtensorMap& a2, const CUtensorMap (&o)[3], const Params& p,
              cudaStream_t s) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
+  static std::atomic<uint64_t> reserved{0};
   auto* kern = gemm_kernel<EPI, T>;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  });
+  const cudaError_t attr_err = reserve_smem(kern, kSmemBytes, &reserved);
   if (attr_err != cudaSuccess) {
     set_error("gemm: cannot reserve %d bytes of shared memory: %s", kSmemBytes,
               cudaGetErrorString(attr_err));
@@ -1413,12 +1410,9 @@ template <int EPI, typename T>
 int launch_pair_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
                   const CUtensorMap& b1, const CUtensorMap& a2, const CUtensorMap (&o)[3],
                   const Params& p, cudaStream_t s) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
+  static std::atomic<uint64_t> reserved{0};
   auto* kern = gemm_kernel_pair<EPI, T>;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes2);
-  });
+  const cudaError_t attr_err = reserve_smem(kern, kSmemBytes2, &reserved);
   if (attr_err != cudaSuccess) {
     set_error("gemm: cannot reserve %d bytes of shared memory: %s", kSmemBytes2,
               cudaGetErrorString(attr_err));

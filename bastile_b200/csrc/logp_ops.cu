@@ -592,7 +592,7 @@ extern "C" int bt_sum_runs(const float* parts, void* out, int64_t n, int64_t run
 
 extern "C" int64_t bt_policy_fwd_ws_floats(int64_t rows, int64_t chunk, int64_t n_seq, int64_t V) {
   if (rows < 0 || chunk < 0 || n_seq < 0 || V <= 0) return 0;
-  return bt::even(2 + n_seq + 3 * rows + 3 * chunk) + chunk * bt_lce_num_vtiles(V) * 2;
+  return bt::even(n_seq + 3 * rows + 3 * chunk) + chunk * bt_lce_num_vtiles(V) * 2;
 }
 
 extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* stream) {
@@ -614,13 +614,13 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
                  "policy_fwd: more than one chunk needs an accumulator for the weight gradient");
   }
   const int runs = d->rows > 0 ? dhidden_runs(d->chunk < d->rows ? d->chunk : d->rows, d->H, d->V, d->dtype) : 1;
-  float* scal = d->ws;
-  float* weights = scal + 2;
+  float* scal = d->averages + 2;
+  float* weights = d->ws;
   float* terms = weights + d->n_seq;
   float* lse = terms + 3 * d->rows;
   float* coef = lse + d->chunk;
   float* tgt = coef + d->chunk;
-  float* tile_stats = d->ws + even(2 + d->n_seq + 3 * d->rows + 3 * d->chunk);
+  float* tile_stats = d->ws + even(d->n_seq + 3 * d->rows + 3 * d->chunk);
   BT_CHECK_LAUNCHED(launch_dependent(policy_weights_kernel, dim3(1), dim3(1024), 0, h.s, d->labels, d->rows,
                                      d->cu_seqlens, static_cast<int>(d->n_seq), d->ignore_index, d->V, weights, scal,
                                      status),

@@ -24,6 +24,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .fused_linear_cross_entropy import _GEMM_DTYPES, AUTO_CHUNK_BYTES, AUTO_CHUNK_ROWS, DEFAULT_CHUNK
@@ -134,6 +135,7 @@ class LinearLogProbsFunction(torch.autograd.Function):
         return logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dlogp):
         lib = _lib.get_lib()
         x, w, labels, lse = ctx.saved_tensors
@@ -181,7 +183,7 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
     ld = _ld_logits(vocab)
     step = _chunk_rows(chunk_size, rows, ld)
     n_chunks = -(-rows // step)
-    loss, averages, logp = _f32(dev), _f32(dev, 2), _f32(dev, rows)
+    loss, averages, logp = _f32(dev), _f32(dev, 4), _f32(dev, rows)
     ws = _f32(dev, int(lib.bt_policy_fwd_ws_floats(rows, step, n_seq, vocab)))
     logits = torch.empty((step, ld), dtype=x.dtype, device=dev) if grad else None
     masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
@@ -199,7 +201,7 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
         rc = lib.bt_policy_fwd(ctypes.byref(d), st.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "bt_policy_fwd")
     last = masked[(n_chunks - 1) * step:] if need_w and n_chunks else None
-    return (loss, logp.view(target.shape), averages), (w, ws[:2], dx, logits if need_w else None, last, acc)
+    return (loss, logp.view(target.shape), averages), (w, averages, dx, logits if need_w else None, last, acc)
 
 
 class LinearPolicyLossFunction(torch.autograd.Function):
@@ -213,19 +215,20 @@ class LinearPolicyLossFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, *_):
         none = (None,) * 10
         if dloss is None:
             return (None, None, *none)
         lib = _lib.get_lib()
-        w, scal, dx, dlogits, x_last, acc = ctx.saved_tensors
+        w, averages, dx, dlogits, x_last, acc = ctx.saved_tensors
         shape, x_dtype, w_dtype = ctx.meta
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         dev = w.device
         vocab, hdim = w.shape
         stream, code = _lib.stream_ptr(dev), _lib.dtype_code(x_dtype)
-        # the coefficients were stored relative to the largest token weight (scal[0])
-        alpha = dloss.detach().to(torch.float32) * scal[0]
+        # the coefficients were stored relative to the largest token weight
+        alpha = dloss.detach().to(torch.float32) * averages[2]
         dx_out = dw = None
         with _lib.device_of(dev), _lib.timed("policy_bwd", int(need_x) + int(need_w and x_last is not None), dev):
             if need_x:

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -96,6 +97,7 @@ class PackedAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse2, plan = ctx.saved_tensors
         batch, scale = ctx.meta

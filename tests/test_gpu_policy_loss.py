@@ -402,3 +402,47 @@ def test_captured_step_replays_and_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(res, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("switch,value", [("bt_set_gemm_cta_pairs", 0), ("bt_set_gemm_dynamic_tiles", 1),
+                                          ("bt_set_gemm_tile_stores", 0), ("bt_set_dependent_launch", 0)])
+def test_other_ways_to_run_the_products(switch, value):
+    """The process-wide switches of the products: the contraction over the vocabulary in several runs
+    (40 rows x 128 from 9000), several chunks, an odd vocabulary."""
+    from bastile_b200 import _lib
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_log_probs, fused_linear_policy_loss
+
+    lib = _lib.get_lib()
+    assert lib.bt_dhidden_runs(40, 128, 9001, _lib.BT_BF16) > 1
+    x, w, t, up, g = make(100, 128, 9001, torch.bfloat16, seed=10)
+    o = Oracle(x, w, t)
+    old, adv, ref = policy_inputs(o, g)
+    want, *_ = policy_oracle(o, old, adv, ref, 0.2, 0.28, 0.1, None)
+    x.requires_grad_(True), w.requires_grad_(True)
+    prev = getattr(lib, switch)(value)
+    try:
+        lp = fused_linear_log_probs(x, w, t, chunk_size=40)
+        a = torch.autograd.grad(lp, (x, w), up)
+        pl = fused_linear_policy_loss(x, w, t, old, adv, ref, 0.2, 0.28, 0.1, chunk_size=40)
+        b = torch.autograd.grad(pl.loss, (x, w))
+        torch.cuda.synchronize()
+    finally:
+        getattr(lib, switch)(prev)
+    close(lp.detach(), o.logp, o.e_logp, "logp")
+    close(pl.loss.detach(), want["loss"], want["e_loss"], "loss")
+    ref_a = o.grads(up.double(), torch.zeros_like(o.e), shifted=False)
+    ref_b = o.grads(want["coef"], want["e_coef"], shifted=True)
+    for i, name in enumerate(("dhidden", "dweight")):
+        close(a[i], *ref_a[name], name)
+        close(b[i], *ref_b[name], name)
+    _lib.check_all_status()
+
+
+def test_second_derivatives_are_refused():
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_log_probs
+
+    x, w, t, up, _ = make(10, 64, 50, torch.bfloat16, seed=11)
+    x.requires_grad_(True)
+    (g,) = torch.autograd.grad(fused_linear_log_probs(x, w, t), x, up.requires_grad_(True), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()

@@ -93,4 +93,4 @@ def test_c_entry_points():
                      (dict(chunk=2, want_dweight=1, dweight_acc=None), b"accumulator"), (dict(ld_hidden=8), b"aligned")):
         err(policy(**kw), text)
     assert lib.bt_logp_fwd_ws_floats(3, 100) == 3 * 2 * 2 + 3 and lib.bt_logp_fwd_ws_floats(-1, 100) == 0
-    assert lib.bt_policy_fwd_ws_floats(5, 3, 2, 100) == 28 + 3 * 2 * 2 and lib.bt_policy_fwd_ws_floats(5, 3, 2, 0) == 0
+    assert lib.bt_policy_fwd_ws_floats(5, 3, 2, 100) == 26 + 3 * 2 * 2 and lib.bt_policy_fwd_ws_floats(5, 3, 2, 0) == 0
