@@ -60,7 +60,7 @@ def _check(what: str, hidden: Tensor, weight: Tensor, target: Tensor, chunk_size
 
 def _rows_of(x: Tensor) -> Tensor:
     """[..., H] -> [rows, H] with unit inner stride and 16-byte rows."""
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     vec = 16 // x2.element_size()
     if x2.stride(-1) != 1 or x2.data_ptr() % 16 != 0 or (x2.shape[0] > 1 and
                                                          (x2.stride(0) % vec != 0 or x2.stride(0) < x2.shape[1])):
@@ -69,14 +69,17 @@ def _rows_of(x: Tensor) -> Tensor:
 
 
 def _head_weight(weight: Tensor, dtype) -> Tensor:
+    if weight.dtype == dtype and weight.is_contiguous() and weight.data_ptr() % 16 == 0:
+        return weight
     w = weight.detach()
     w = w if w.dtype == dtype else w.to(dtype)
     w = w.contiguous()
     return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
-def _labels(target: Tensor) -> Tensor:
-    return target.reshape(-1).to(torch.int64).contiguous()
+def _flat(t: Tensor, dtype) -> Tensor:
+    """``t``'s values one behind the other in ``dtype`` (itself if they lie that way)."""
+    return t if t.dtype == dtype and t.is_contiguous() else t.detach().to(dtype).contiguous()
 
 
 def _ld(x2: Tensor) -> int:
@@ -109,7 +112,7 @@ def _dweight_out(w: Tensor, w_dtype) -> Tensor:
 def _log_probs(hidden, weight, target, ignore_index: int, chunk_size: int, keep: bool):
     """(log-probabilities, what the backward needs if ``keep``)."""
     lib = _lib.get_lib()
-    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
+    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _flat(target, torch.int64)
     dev, rows = x.device, x.shape[0]
     vocab, hdim = w.shape
     logp = _f32(dev, rows)
@@ -147,7 +150,7 @@ class LinearLogProbsFunction(torch.autograd.Function):
         dw = _dweight_out(w, w_dtype) if need_w else None
         if rows == 0:
             return (dx.view(shape) if need_x else None, dw.zero_().to(w_dtype) if need_w else None, None, None, None)
-        g = dlogp.reshape(-1).to(torch.float32).contiguous()
+        g = _flat(dlogp, torch.float32)
         ld = _ld_logits(vocab)
         step = _chunk_rows(chunk_size, rows, ld)
         n_chunks = -(-rows // step)
@@ -173,12 +176,11 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
             need_w):
     """((loss, log-probabilities, averages), what the backward needs)."""
     lib = _lib.get_lib()
-    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _labels(target)
+    x, w, labels = _rows_of(hidden), _head_weight(weight, hidden.dtype), _flat(target, torch.int64)
     dev, rows = x.device, x.shape[0]
     vocab, hdim = w.shape
     grad = need_x or need_w
-    old, adv, ref = (t if t is None else t.detach().reshape(-1).to(torch.float32).contiguous()
-                     for t in (old, adv, ref))
+    old, adv, ref = (None if t is None else _flat(t, torch.float32) for t in (old, adv, ref))
     n_seq = 1 if cu is None else cu.numel() - 1
     ld = _ld_logits(vocab)
     step = _chunk_rows(chunk_size, rows, ld)
