@@ -99,7 +99,7 @@ constexpr float kLazyMax = 8.0f;
 template <typename T, int DT>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const Params p) {
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Params p) {
   using G = FwdGeo<DT>;
   constexpr int TB = G::kTileBytes;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -111,7 +111,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   uint64_t* s_full = v_full + 1;   // phase j: scores j are there, and K_j may be replaced
   uint64_t* p_ready = s_full + 1;
   uint64_t* pv_done = p_ready + 1; // phase j: block j is in O, and V_j may be replaced
-  uint64_t* fix = pv_done + 1;
+  uint64_t* staged = pv_done + 1;
+  uint64_t* fix = staged + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fix + 1);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -123,6 +124,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     ptx::mbar_init(s_full, 1);
     ptx::mbar_init(p_ready, 4);
     ptx::mbar_init(pv_done, 1);
+    ptx::mbar_init(staged, 4);
     ptx::mbar_init(fix, 1);
     *cta_abort = 0;
     ptx::fence_mbar_init();
@@ -279,20 +281,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         ptx::tcgen05_fence_after_sync();
         const float inv = 1.0f / l;
         if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
+        if (first + p.tq <= it.len) {  // into Q's place
 #pragma unroll 1
-        for (int q = 0; q < DT / 32; ++q) {
-          float o[32];
-          tmem_ld32(to + q * 32, o);
-          tmem_wait_ld();
-          if (row_ok) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack2<T>(o[v * 8 + 2 * e] * inv, o[v * 8 + 2 * e + 1] * inv);
-              if (q * 32 + v * 8 < p.d) st_global_v4(out + q * 32 + v * 8, make_uint4(w[0], w[1], w[2], w[3]));
-            }
-          }
+          for (int c = 0; c < DT; c += 32) stage_cols<T>(to + c, sQ, row, c, inv);
+          store_tile<DT>(warp == 0 && lane == 0, staged, 0, sQ, &tmO, hs * p.gp, it.start + first, lane, cta_abort,
+                         p.status);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < DT; c += 32) store_cols<T>(to + c, out, c, p.d, inv, row_ok);
         }
       }
     }
@@ -306,15 +302,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 }
 
 template <typename T, int DT>
-int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p, int64_t batch,
-               cudaStream_t s) {
+int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const Params& p,
+               int64_t batch, cudaStream_t s) {
   auto* kern = attn_fwd_kernel<T, DT>;
   static std::atomic<uint64_t> reserved{0};
   BT_CHECK_LAUNCHED(reserve_smem(kern, FwdGeo<DT>::kSmem, &reserved), "attn_fwd: shared memory");
   const int64_t grid = max_items(p.total, batch, p.tq) * p.hk * p.nsub;
   BT_CHECK_ARG(grid <= 0x7fffffffll, "attn_fwd: too many tiles (%lld)", (long long)grid);
   BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdGeo<DT>::kSmem, s,
-                                     q, k, v, p),
+                                     q, k, v, o, p),
                     "attn_fwd");
   return BT_OK;
 }
@@ -443,13 +439,16 @@ extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* ou
   p.o = View{out, o_strides[0], o_strides[1]};
   p.status = status;
   bind_context();
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   if (int rc = encode_rows(&tq, q, dtype, nd, nq, total, q_strides[1], q_strides[0], p.gp, p.tq, "attn_fwd q")) return rc;
   if (int rc = encode_rows(&tk, k, dtype, nd, nk, total, k_strides[1], k_strides[0], 1, kTile, "attn_fwd k")) return rc;
   if (int rc = encode_rows(&tv, v, dtype, nd, nk, total, v_strides[1], v_strides[0], 1, kTile, "attn_fwd v")) return rc;
+  if (int rc = encode_rows(&to, out, dtype, nd, nq, total, o_strides[1], o_strides[0], p.gp, p.tq, "attn_fwd out"))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BT_BF16)
-    return d <= 64 ? launch_fwd<__nv_bfloat16, 64>(tq, tk, tv, p, batch, s)
-                   : launch_fwd<__nv_bfloat16, 128>(tq, tk, tv, p, batch, s);
-  return d <= 64 ? launch_fwd<__half, 64>(tq, tk, tv, p, batch, s) : launch_fwd<__half, 128>(tq, tk, tv, p, batch, s);
+    return d <= 64 ? launch_fwd<__nv_bfloat16, 64>(tq, tk, tv, to, p, batch, s)
+                   : launch_fwd<__nv_bfloat16, 128>(tq, tk, tv, to, p, batch, s);
+  return d <= 64 ? launch_fwd<__half, 64>(tq, tk, tv, to, p, batch, s)
+                 : launch_fwd<__half, 128>(tq, tk, tv, to, p, batch, s);
 }

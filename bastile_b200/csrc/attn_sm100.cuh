@@ -88,6 +88,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(ptx::smem_u32(bar))
       : "memory");
 }
+// Tile store, the way back: one box of a staged tile (rows / columns outside the tensor are clipped).
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tm, uint32_t smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                   reinterpret_cast<uint64_t>(tm)),
+               "r"(x), "r"(y), "r"(z), "r"(smem_src)
+               : "memory");
+}
 // One operand tile: DT / 64 boxes.
 template <int DT>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* tm, int head, int token, uint64_t* bar) {
@@ -268,6 +275,55 @@ __device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, i
 __device__ __forceinline__ void drain_copies() {
   const uint64_t t0 = ptx::globaltimer_ns();
   while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
+// Results leave the accumulator 32 columns of a row per thread.  A thread's own stores would touch 32
+// rows per instruction, about 2000 cycles a tile; a tile that lies inside its sequence goes to shared
+// memory instead, where the operands were, and from there as one tile store.  (A tile that reaches past
+// its sequence must not write there: its rows are stored one by one.)
+template <typename T>
+__device__ __forceinline__ void stage_cols(uint32_t taddr, uint32_t tile, int row, int col0, float scale) {
+  float v[32];
+  tmem_ld32(taddr, v);
+  tmem_wait_ld();
+  const uint32_t at = tile + (col0 / 64) * kBoxBytes + row * 128;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[g * 8 + 2 * e] * scale, v[g * 8 + 2 * e + 1] * scale);
+    const uint32_t chunk = static_cast<uint32_t>((col0 % 64) / 8 + g) ^ (static_cast<uint32_t>(row) & 7u);
+    ptx::st_shared_v4(at + (chunk << 4), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, int col0, int d, float scale, bool row_ok) {
+  float v[32];
+  tmem_ld32(taddr, v);
+  tmem_wait_ld();
+  if (!row_ok) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[g * 8 + 2 * e] * scale, v[g * 8 + 2 * e + 1] * scale);
+    if (col0 + g * 8 < d) st_global_v4(dst + col0 + g * 8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+// After a warp has staged its part: say so, and (the one thread) wait for all and store the tile.
+template <int DT>
+__device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32_t parity, uint32_t tile,
+                                           const CUtensorMap* tm, int head, int token, int lane,
+                                           volatile int* cta_abort, int32_t* status) {
+  ptx::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) ptx::mbar_arrive(staged);
+  if (issuer && ptx::mbar_wait(staged, parity, cta_abort, status, ST_MATH)) {
+#pragma unroll
+    for (int j = 0; j < DT / 64; ++j) tma_store_3d(tm, tile + j * kBoxBytes, j * 64, head, token);
+    ptx::bulk_commit_group();
+    ptx::bulk_wait_group<0>();
+  }
 }
 
 // What every kernel is told about one [tokens, heads, head_dim] tensor besides its tile map.
