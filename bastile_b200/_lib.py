@@ -101,9 +101,9 @@ SIGNATURES = {
                                      c_void_p]),
     "bt_attn_plan_words": (c_int64, [c_int64]),
     "bt_attn_plan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
-    "bt_attn_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 5 + [POINTER(c_int64)] * 4 +
+    "bt_attn_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 5 + [POINTER(c_int64)] * 4 +
                     [c_float, c_int, c_void_p, c_void_p]),
-    "bt_attn_bwd": (c_int, [c_void_p] * 11 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
+    "bt_attn_bwd": (c_int, [c_void_p] * 12 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
                     [c_float, c_int, c_void_p, c_void_p]),
     "bt_logp_fwd_ws_floats": (c_int64, [c_int64] * 2),
     "bt_logp_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 6 + [c_int, c_void_p, c_void_p]),

@@ -18,11 +18,14 @@ constexpr int kBwdThreads = 384;
 
 // ------------------------------------------------------------------ D = dO . O
 // Half a warp per (token, head) row, 16 bytes of each tensor per lane, four rows in flight.  Bound by
-// memory.
+// memory.  O comes as its 16-bit values and what their rounding cut off: with the rounded O alone, D is
+// off by dO . (that), which is as much in dQ and dK as the rounding of dS (2-norm of the error of dQ at
+// bf16: 2.7e-3 instead of 2.4e-3; 1.7e-3 is the rounding of the result).
 template <typename T>
 __global__ void __launch_bounds__(256)
-attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* __restrict__ delta, int64_t rows,
-                  int heads, int64_t total, int d, int64_t o_st, int64_t o_sh, int64_t g_st, int64_t g_sh) {
+attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ out_lo, const T* __restrict__ dout,
+                  float* __restrict__ delta, int64_t rows, int heads, int64_t total, int d, int64_t o_st, int64_t o_sh,
+                  int64_t g_st, int64_t g_sh) {
   grid_dependency_wait();
   constexpr int kRows = 4;
   const int sub = threadIdx.x & 15;
@@ -30,12 +33,12 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* 
   const bool small = rows <= 0xffffffffll;  // a 64-bit division costs more than the row's arithmetic
   const int64_t step = static_cast<int64_t>(gridDim.x) * 16 * kRows;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16 * kRows; r0 < rows; r0 += step) {
-    uint4 a[kRows], b[kRows];
+    uint4 a[kRows], b[kRows], c[kRows];
     int64_t at[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
-      a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      a[i] = b[i] = c[i] = make_uint4(0, 0, 0, 0);
       at[i] = -1;
       if (r < rows) {
         const int64_t tok = small ? static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(heads)) : r / heads;
@@ -43,17 +46,19 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout, float* 
         at[i] = head * total + tok;
         if (live) {
           a[i] = ld_stream_v4(out + tok * o_st + head * o_sh + sub * 8);
+          if (out_lo != nullptr) c[i] = ld_stream_v4(out_lo + tok * o_st + head * o_sh + sub * 8);
           b[i] = ld_global_v4(dout + tok * g_st + head * g_sh + sub * 8);
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      float x[8], y[8], acc = 0.f;
+      float x[8], y[8], z[8], acc = 0.f;
       Cvt<T>::unpack(a[i], x);
       Cvt<T>::unpack(b[i], y);
+      Cvt<T>::unpack(c[i], z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc = fmaf(x[e], y[e], acc);
+      for (int e = 0; e < 8; ++e) acc = fmaf(x[e] + z[e], y[e], acc);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
       if (at[i] >= 0 && sub == 0) delta[at[i]] = acc;
@@ -360,8 +365,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         // (one store per tile and output here: a staged tile store measured 1% slower)
 #pragma unroll 1
         for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
-          store_cols<T>(tmem + lane_base + 256 + c, dv, c, p.d, 1.0f, row_ok);
-          store_cols<T>(tmem + lane_base + 256 + DT + c, dk, c, p.d, p.scale, row_ok);
+          store_cols<T>(tmem + lane_base + 256 + c, dv, nullptr, c, p.d, 1.0f, row_ok);
+          store_cols<T>(tmem + lane_base + 256 + DT + c, dk, nullptr, c, p.d, p.scale, row_ok);
         }
       }
     }
@@ -618,13 +623,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         const uint32_t ta = tmem + lane_base + 384;
         if (first + p.tq <= it.len) {  // into Q's place
 #pragma unroll 1
-          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) stage_cols<T>(ta + c, sQ, row, c, p.scale);
-          store_tile<DT>(warp == 0 && lane == 0, staged, 0, sQ, &tmD, hs * p.gp, it.start + first, lane, cta_abort,
-                         p.status);
+          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) stage_cols<T>(ta + c, sQ, 0, row, c, p.scale);
+          store_tile<DT>(warp == 0 && lane == 0, staged, sQ, &tmD, 0, &tmD, hs * p.gp, it.start + first, lane,
+                         cta_abort, p.status);
         } else {
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
-            store_cols<T>(ta + c, dq, c, p.d, p.scale, row_ok);
+            store_cols<T>(ta + c, dq, nullptr, c, p.d, p.scale, row_ok);
         }
       }
     }
@@ -671,12 +676,13 @@ int run_bwd(const Maps& m, Params p, int64_t batch, cudaStream_t s) {
 }
 
 template <typename T>
-int run_delta(const void* out, const void* dout, float* delta, int64_t total, int64_t hq, int64_t d,
+int run_delta(const void* out, const void* out_lo, const void* dout, float* delta, int64_t total, int64_t hq, int64_t d,
               const int64_t* os, const int64_t* gs, cudaStream_t s) {
   const int64_t rows = total * hq;
   const int64_t want = ceil_div(rows, 64), cap = static_cast<int64_t>(sm_count()) * 8;
   BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(static_cast<unsigned>(want < cap ? want : cap)),
-                                     dim3(256), 0, s, static_cast<const T*>(out), static_cast<const T*>(dout), delta,
+                                     dim3(256), 0, s, static_cast<const T*>(out),
+                                     static_cast<const T*>(out_lo), static_cast<const T*>(dout), delta,
                                      rows, static_cast<int>(hq), total, static_cast<int>(d), os[0], os[1], gs[0],
                                      gs[1]),
                     "attn_bwd delta");
@@ -692,7 +698,7 @@ int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns) {
 }
 
 extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
-                           const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan,
+                           const void* out_lo, const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan,
                            int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides,
                            const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                            const int64_t* o_strides, const int64_t* dq_strides, const int64_t* dk_strides,
@@ -703,6 +709,7 @@ extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const
   if (int rc = fill_params(&p, "attn_bwd", plan, batch, total, hq, hk, d, scale, dtype)) return rc;
   const int nq = static_cast<int>(hq), nk = static_cast<int>(hk), nd = static_cast<int>(d);
   BT_CHECK_ARG(lse2 != nullptr && delta != nullptr, "attn_bwd: null pointer");
+  BT_CHECK_ARG(aligned16(out_lo), "attn_bwd out_lo: must be 16-byte aligned");
   BT_CHECK_ARG((dk == nullptr) == (dv == nullptr), "attn_bwd: dk and dv are computed together");
   if (int rc = check_view("attn_bwd dout", dout, g_strides[0], g_strides[1], nq, total)) return rc;
   if (int rc = check_view("attn_bwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
@@ -736,9 +743,9 @@ extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const
   if (int rc = rows(&m.dq, dq, dq_strides, true, "attn_bwd dq")) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BT_BF16) {
-    if (int rc = run_delta<__nv_bfloat16>(out, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+    if (int rc = run_delta<__nv_bfloat16>(out, out_lo, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
     return d <= 64 ? run_bwd<__nv_bfloat16, 64>(m, p, batch, s) : run_bwd<__nv_bfloat16, 128>(m, p, batch, s);
   }
-  if (int rc = run_delta<__half>(out, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+  if (int rc = run_delta<__half>(out, out_lo, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
   return d <= 64 ? run_bwd<__half, 64>(m, p, batch, s) : run_bwd<__half, 128>(m, p, batch, s);
 }

@@ -99,7 +99,8 @@ constexpr float kLazyMax = 8.0f;
 template <typename T, int DT>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Params p) {
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ CUtensorMap tmL, const Params p) {
   using G = FwdGeo<DT>;
   constexpr int TB = G::kTileBytes;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -206,8 +207,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const int head = hs * p.gp + (row & (p.gp - 1));
     const int64_t token = static_cast<int64_t>(it.start) + tok;
     const bool row_ok = live && tok < it.len;
-    T* out = static_cast<T*>(p.o.ptr) + token * p.o.st + head * p.o.sh;
-    if (behind && row_ok)
+    const int64_t out_at = token * p.o.st + head * p.o.sh;
+    T* out = static_cast<T*>(p.o.ptr) + out_at;
+    if (behind && row_ok)  // (the gradients of these rows are zeros whatever the residual holds)
       for (int c = 0; c < p.d; c += 8) st_global_v4(out + c, make_uint4(0, 0, 0, 0));
     if (n > 0) {
       const uint32_t ts = tmem + (static_cast<uint32_t>(warp * 32) << 16), to = ts + 128;
@@ -281,14 +283,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         ptx::tcgen05_fence_after_sync();
         const float inv = 1.0f / l;
         if (row_ok && p.lse2 != nullptr) p.lse2[static_cast<int64_t>(head) * p.total + token] = m * c + log2f(l);
-        if (first + p.tq <= it.len) {  // into Q's place
+        if (first + p.tq <= it.len) {  // into Q's place, the residual into K's
+          const uint32_t lo_tile = p.o_lo != nullptr ? sK : 0u;
 #pragma unroll 1
-          for (int c = 0; c < DT; c += 32) stage_cols<T>(to + c, sQ, row, c, inv);
-          store_tile<DT>(warp == 0 && lane == 0, staged, 0, sQ, &tmO, hs * p.gp, it.start + first, lane, cta_abort,
-                         p.status);
+          for (int c = 0; c < DT; c += 32) stage_cols<T>(to + c, sQ, lo_tile, row, c, inv);
+          store_tile<DT>(warp == 0 && lane == 0, staged, sQ, &tmO, lo_tile, &tmL, hs * p.gp, it.start + first, lane,
+                         cta_abort, p.status);
         } else {
+          T* lo = p.o_lo != nullptr ? static_cast<T*>(p.o_lo) + out_at : nullptr;
 #pragma unroll 1
-          for (int c = 0; c < DT; c += 32) store_cols<T>(to + c, out, c, p.d, inv, row_ok);
+          for (int c = 0; c < DT; c += 32) store_cols<T>(to + c, out, lo, c, p.d, inv, row_ok);
         }
       }
     }
@@ -302,15 +306,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 }
 
 template <typename T, int DT>
-int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const Params& p,
-               int64_t batch, cudaStream_t s) {
+int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& o, const CUtensorMap& l,
+               const Params& p, int64_t batch, cudaStream_t s) {
   auto* kern = attn_fwd_kernel<T, DT>;
   static std::atomic<uint64_t> reserved{0};
   BT_CHECK_LAUNCHED(reserve_smem(kern, FwdGeo<DT>::kSmem, &reserved), "attn_fwd: shared memory");
   const int64_t grid = max_items(p.total, batch, p.tq) * p.hk * p.nsub;
   BT_CHECK_ARG(grid <= 0x7fffffffll, "attn_fwd: too many tiles (%lld)", (long long)grid);
   BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdGeo<DT>::kSmem, s,
-                                     q, k, v, o, p),
+                                     q, k, v, o, l, p),
                     "attn_fwd");
   return BT_OK;
 }
@@ -421,7 +425,8 @@ extern "C" int bt_attn_plan(const int32_t* cu_seqlens, int64_t batch, int64_t to
   return BT_OK;
 }
 
-extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse2, const int32_t* plan,
+extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse2,
+                           const int32_t* plan,
                            int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
                            const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale,
                            int dtype, int32_t* status, void* stream) {
@@ -434,21 +439,28 @@ extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* ou
   if (int rc = check_view("attn_fwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;
   if (int rc = check_view("attn_fwd v", v, v_strides[0], v_strides[1], nk, total)) return rc;
   if (int rc = check_view("attn_fwd out", out, o_strides[0], o_strides[1], nq, total)) return rc;
+  BT_CHECK_ARG(aligned16(out_lo), "attn_fwd out_lo: must be 16-byte aligned");
   p.gran = gran_index(p.tq);
+  p.o_lo = out_lo;
   p.lse2 = lse2;
   p.o = View{out, o_strides[0], o_strides[1]};
   p.status = status;
   bind_context();
-  CUtensorMap tq, tk, tv, to;
+  CUtensorMap tq, tk, tv, to, tl;
   if (int rc = encode_rows(&tq, q, dtype, nd, nq, total, q_strides[1], q_strides[0], p.gp, p.tq, "attn_fwd q")) return rc;
   if (int rc = encode_rows(&tk, k, dtype, nd, nk, total, k_strides[1], k_strides[0], 1, kTile, "attn_fwd k")) return rc;
   if (int rc = encode_rows(&tv, v, dtype, nd, nk, total, v_strides[1], v_strides[0], 1, kTile, "attn_fwd v")) return rc;
   if (int rc = encode_rows(&to, out, dtype, nd, nq, total, o_strides[1], o_strides[0], p.gp, p.tq, "attn_fwd out"))
     return rc;
+  tl = to;
+  if (out_lo != nullptr) {
+    if (int rc = encode_rows(&tl, out_lo, dtype, nd, nq, total, o_strides[1], o_strides[0], p.gp, p.tq, "attn_fwd out_lo"))
+      return rc;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BT_BF16)
-    return d <= 64 ? launch_fwd<__nv_bfloat16, 64>(tq, tk, tv, to, p, batch, s)
-                   : launch_fwd<__nv_bfloat16, 128>(tq, tk, tv, to, p, batch, s);
-  return d <= 64 ? launch_fwd<__half, 64>(tq, tk, tv, to, p, batch, s)
-                 : launch_fwd<__half, 128>(tq, tk, tv, to, p, batch, s);
+    return d <= 64 ? launch_fwd<__nv_bfloat16, 64>(tq, tk, tv, to, tl, p, batch, s)
+                   : launch_fwd<__nv_bfloat16, 128>(tq, tk, tv, to, tl, p, batch, s);
+  return d <= 64 ? launch_fwd<__half, 64>(tq, tk, tv, to, tl, p, batch, s)
+                 : launch_fwd<__half, 128>(tq, tk, tv, to, tl, p, batch, s);
 }

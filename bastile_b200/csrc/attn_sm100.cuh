@@ -281,46 +281,66 @@ __device__ __forceinline__ void drain_copies() {
 // rows per instruction, about 2000 cycles a tile; a tile that lies inside its sequence goes to shared
 // memory instead, where the operands were, and from there as one tile store.  (A tile that reaches past
 // its sequence must not write there: its rows are stored one by one.)
+// `lo_tile` / `lo_dst` (0 / null: none) take what rounding to 16 bits cut off, rounded in its turn.
 template <typename T>
-__device__ __forceinline__ void stage_cols(uint32_t taddr, uint32_t tile, int row, int col0, float scale) {
+__device__ __forceinline__ void round_cols(const float (&v)[32], int g, float scale, uint4* hi, uint4* lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float a = v[g * 8 + 2 * e] * scale, b = v[g * 8 + 2 * e + 1] * scale;
+    h[e] = pack2<T>(a, b);
+    const T* r = reinterpret_cast<const T*>(&h[e]);
+    l[e] = pack2<T>(a - Cvt<T>::to_f(r[0]), b - Cvt<T>::to_f(r[1]));
+  }
+  *hi = make_uint4(h[0], h[1], h[2], h[3]);
+  *lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+template <typename T>
+__device__ __forceinline__ void stage_cols(uint32_t taddr, uint32_t tile, uint32_t lo_tile, int row, int col0,
+                                           float scale) {
   float v[32];
   tmem_ld32(taddr, v);
   tmem_wait_ld();
-  const uint32_t at = tile + (col0 / 64) * kBoxBytes + row * 128;
+  const uint32_t at = (col0 / 64) * kBoxBytes + row * 128;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[g * 8 + 2 * e] * scale, v[g * 8 + 2 * e + 1] * scale);
+    uint4 hi, lo;
+    round_cols<T>(v, g, scale, &hi, &lo);
     const uint32_t chunk = static_cast<uint32_t>((col0 % 64) / 8 + g) ^ (static_cast<uint32_t>(row) & 7u);
-    ptx::st_shared_v4(at + (chunk << 4), make_uint4(w[0], w[1], w[2], w[3]));
+    ptx::st_shared_v4(tile + at + (chunk << 4), hi);
+    if (lo_tile != 0) ptx::st_shared_v4(lo_tile + at + (chunk << 4), lo);
   }
 }
 template <typename T>
-__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, int col0, int d, float scale, bool row_ok) {
+__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, T* lo_dst, int col0, int d, float scale, bool row_ok) {
   float v[32];
   tmem_ld32(taddr, v);
   tmem_wait_ld();
   if (!row_ok) return;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack2<T>(v[g * 8 + 2 * e] * scale, v[g * 8 + 2 * e + 1] * scale);
-    if (col0 + g * 8 < d) st_global_v4(dst + col0 + g * 8, make_uint4(w[0], w[1], w[2], w[3]));
+    uint4 hi, lo;
+    round_cols<T>(v, g, scale, &hi, &lo);
+    if (col0 + g * 8 >= d) continue;
+    st_global_v4(dst + col0 + g * 8, hi);
+    if (lo_dst != nullptr) st_global_v4(lo_dst + col0 + g * 8, lo);
   }
 }
-// After a warp has staged its part: say so, and (the one thread) wait for all and store the tile.
+// After a warp has staged its part: say so, and (the one thread) wait for all and store the tile, and the
+// second one unless lo_tile is 0.
 template <int DT>
-__device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32_t parity, uint32_t tile,
-                                           const CUtensorMap* tm, int head, int token, int lane,
+__device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32_t tile, const CUtensorMap* tm,
+                                           uint32_t lo_tile, const CUtensorMap* lo_tm, int head, int token, int lane,
                                            volatile int* cta_abort, int32_t* status) {
   ptx::fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) ptx::mbar_arrive(staged);
-  if (issuer && ptx::mbar_wait(staged, parity, cta_abort, status, ST_MATH)) {
+  if (issuer && ptx::mbar_wait(staged, 0, cta_abort, status, ST_MATH)) {
 #pragma unroll
-    for (int j = 0; j < DT / 64; ++j) tma_store_3d(tm, tile + j * kBoxBytes, j * 64, head, token);
+    for (int j = 0; j < DT / 64; ++j) {
+      tma_store_3d(tm, tile + j * kBoxBytes, j * 64, head, token);
+      if (lo_tile != 0) tma_store_3d(lo_tm, lo_tile + j * kBoxBytes, j * 64, head, token);
+    }
     ptx::bulk_commit_group();
     ptx::bulk_wait_group<0>();
   }
@@ -341,6 +361,7 @@ struct Params {
   float* lse2;   // [hq][total] base-2 log-sum-exp of the scaled scores
   float* delta;  // [hq][total] dot(dO, O)
   View o, dq, dk, dv;
+  void* o_lo;  // laid out as o
   int32_t* status;
 };
 

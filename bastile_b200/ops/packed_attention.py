@@ -77,15 +77,16 @@ def _forward(q, k, v, sequences, scale, keep: bool):
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
     lse2 = torch.empty((hq, t), dtype=torch.float32, device=dev) if keep else None
+    lo = torch.empty_like(out) if keep else None  # what rounding cut off: dout . out is formed from both
     if t > 0:
         st = _lib.status_word(dev)
         with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
             rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                 lse2.data_ptr() if keep else None, sequences.plan.data_ptr(), sequences.batch, t, hq,
+                                 lo.data_ptr() if keep else None, lse2.data_ptr() if keep else None, sequences.plan.data_ptr(), sequences.batch, t, hq,
                                  k.shape[1], d, _strides(q), _strides(k), _strides(v), _strides(out), scale,
                                  _lib.dtype_code(q.dtype), st.data_ptr(), _lib.stream_ptr(dev))
         _lib.check(rc, "bt_attn_fwd")
-    return out, (q, k, v, out, lse2, sequences.plan)
+    return out, (q, k, v, out, lo, lse2, sequences.plan)
 
 
 class PackedAttentionFunction(torch.autograd.Function):
@@ -99,7 +100,7 @@ class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse2, plan = ctx.saved_tensors
+        q, k, v, out, lo, lse2, plan = ctx.saved_tensors
         batch, scale = ctx.meta
         dev = q.device
         lib = _lib.get_lib()
@@ -116,7 +117,7 @@ class PackedAttentionFunction(torch.autograd.Function):
             none = _lib.I64x2(0, 0)
             with _lib.device_of(dev), _lib.timed("attn_bwd", 1 + int(need_q) + int(need_kv), dev):
                 rc = lib.bt_attn_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                     lse2.data_ptr(), delta.data_ptr(), dq.data_ptr() if need_q else None,
+                                     lo.data_ptr(), lse2.data_ptr(), delta.data_ptr(), dq.data_ptr() if need_q else None,
                                      dk.data_ptr() if need_kv else None, dv.data_ptr() if need_kv else None,
                                      plan.data_ptr(), batch, t, hq, hk, d, _strides(dout), _strides(q), _strides(k),
                                      _strides(v), _strides(out), _strides(dq) if need_q else none,

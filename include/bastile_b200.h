@@ -461,18 +461,20 @@ int bt_attn_plan(const int32_t* cu_seqlens, int64_t batch, int64_t total, int32_
 /* out[t, h, :] = sum over s <= t of the same sequence of softmax_s(scale q[t,h].k[s,h/(hq/hk)]) v[s].
  * q, out [total, hq, d], k, v [total, hk, d]; BT_BF16 or BT_FP16; *_strides = element strides of
  * (token, head), multiples of 8; unit stride along d; d a multiple of 8, at most 128.  Rows behind the
- * last sequence are written as zeros.  lse2 (may be NULL): [hq, total] fp32, the base-2 log-sum-exp of
- * the scaled scores, written for rows of sequences only. */
-int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse2, const int32_t* plan,
-                int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
+ * last sequence are written as zeros.  out_lo (may be NULL, laid out as out): what rounding to `dtype` cut
+ * off, for bt_attn_bwd; written for rows of sequences only, and so is lse2 (may be NULL): [hq, total] fp32, the base-2
+ * log-sum-exp of the scaled scores. */
+int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse2,
+                const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
                 const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale, int dtype,
                 int32_t* status, void* stream);
 
-/* Gradients of bt_attn_fwd for the upstream gradient `dout` (bt_attn_fwd's out and lse2 come back in).
+/* Gradients of bt_attn_fwd for the upstream gradient `dout` (bt_attn_fwd's out, out_lo - may
+ * be NULL, with the gradients then a little less exact - and lse2 come back in).
  * dq may be NULL, and so may dk and dv together; `delta` is [hq, total] fp32 scratch.  Rows behind the
  * last sequence get zeros.  No atomics: the same inputs give the same bits. */
-int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse2,
-                float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch, int64_t total,
+int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* out_lo,
+                const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch, int64_t total,
                 int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides, const int64_t* q_strides,
                 const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                 const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides, float scale,

@@ -65,7 +65,7 @@ def test_c_entry_points():
     good, bad = _lib.I64x2(256, 64), _lib.I64x2(250, 64)
 
     def fwd(q=one, batch=1, total=4, hq=4, hk=2, d=64, qs=good, dtype=_lib.BT_BF16, plan=one, scale=0.1):
-        return lib.bt_attn_fwd(q, one, one, one, None, plan, batch, total, hq, hk, d, qs, good, good, good, scale,
+        return lib.bt_attn_fwd(q, one, one, one, None, None, plan, batch, total, hq, hk, d, qs, good, good, good, scale,
                                dtype, None, None)
 
     for kw, text in ((dict(q=None), b"null"), (dict(plan=None), b"null plan"), (dict(hq=3), b"multiple"),
@@ -75,7 +75,7 @@ def test_c_entry_points():
         assert fwd(**kw) == -1 and text in lib.bt_last_error(), (kw, lib.bt_last_error())
 
     def bwd(dk=one, dv=one, lse=one):
-        return lib.bt_attn_bwd(one, one, one, one, one, lse, one, one, dk, dv, one, 1, 4, 4, 2, 64, good, good, good,
+        return lib.bt_attn_bwd(one, one, one, one, one, None, lse, one, one, dk, dv, one, 1, 4, 4, 2, 64, good, good, good,
                                good, good, good, good, bad, 0.1, _lib.BT_BF16, None, None)
 
     assert bwd(lse=None) == -1 and b"null" in lib.bt_last_error()
