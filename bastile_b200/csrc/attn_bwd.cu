@@ -8,6 +8,10 @@
 // dQ per query tile.  S and dO V^T are computed by both - seven products where one kernel could do
 // with five - but that one would have to add dQ tiles into memory by atomics, whose order changes
 // the result; here every launch gives the same bits.
+// Measured, 8192 tokens in one sequence, 32 / 8 heads of 128, bf16: dK and dV 783 us, dQ 593 us, which is
+// 1.40 and 1.39 PFLOP/s of the products that they execute (a library product of this length runs at 1.41:
+// the chip's power limit, at 1.4 - 1.5 GHz); D = dO . O 34 us.  At 4096 tokens the matrix pipe is busy in 63%
+// and 60% of the cycles, the exponentials' in 36% and 42%.
 #include "attn_sm100.cuh"
 
 namespace bt {
@@ -41,7 +45,7 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ out_lo, const
       a[i] = b[i] = c[i] = make_uint4(0, 0, 0, 0);
       at[i] = -1;
       if (r < rows) {
-        const int64_t tok = small ? static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(heads)) : r / heads;
+        const int64_t tok = small ? static_cast<uint32_t>(r) / static_cast<uint32_t>(heads) : r / heads;
         const int64_t head = r - tok * heads;
         at[i] = head * total + tok;
         if (live) {
@@ -187,7 +191,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = e * 32 + lane;
-          const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + it.start + tok0 + (r >> p.gp_shift);
+          const int token = it.start + tok0 + (r >> p.gp_shift);
+          const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + token;
           const bool in = r < valid;
           vec[st * 256 + r] = in ? -__ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
           vec[st * 256 + 128 + r] = in ? -__ldg(p.delta + at) : 0.f;
@@ -623,7 +628,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         const uint32_t ta = tmem + lane_base + 384;
         if (first + p.tq <= it.len) {  // into Q's place
 #pragma unroll 1
-          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) stage_cols<T>(ta + c, sQ, 0, row, c, p.scale);
+          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
+            stage_cols<T>(ta + c, sQ, 0, row, c, p.scale);
           store_tile<DT>(warp == 0 && lane == 0, staged, sQ, &tmD, 0, &tmD, hs * p.gp, it.start + first, lane,
                          cta_abort, p.status);
         } else {
@@ -681,10 +687,9 @@ int run_delta(const void* out, const void* out_lo, const void* dout, float* delt
   const int64_t rows = total * hq;
   const int64_t want = ceil_div(rows, 64), cap = static_cast<int64_t>(sm_count()) * 8;
   BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(static_cast<unsigned>(want < cap ? want : cap)),
-                                     dim3(256), 0, s, static_cast<const T*>(out),
-                                     static_cast<const T*>(out_lo), static_cast<const T*>(dout), delta,
-                                     rows, static_cast<int>(hq), total, static_cast<int>(d), os[0], os[1], gs[0],
-                                     gs[1]),
+                                     dim3(256), 0, s, static_cast<const T*>(out), static_cast<const T*>(out_lo),
+                                     static_cast<const T*>(dout), delta, rows, static_cast<int>(hq), total,
+                                     static_cast<int>(d), os[0], os[1], gs[0], gs[1]),
                     "attn_bwd delta");
   return BT_OK;
 }
@@ -698,9 +703,9 @@ int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns) {
 }
 
 extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
-                           const void* out_lo, const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan,
-                           int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides,
-                           const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                           const void* out_lo, const float* lse2, float* delta, void* dq, void* dk, void* dv,
+                           const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d,
+                           const int64_t* g_strides, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                            const int64_t* o_strides, const int64_t* dq_strides, const int64_t* dk_strides,
                            const int64_t* dv_strides, float scale, int dtype, int32_t* status, void* stream) {
   using namespace bt;

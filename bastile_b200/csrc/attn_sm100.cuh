@@ -27,7 +27,7 @@ enum : int { ST_LOAD = 1, ST_ISSUE = 2, ST_ISSUE2 = 4, ST_MATH = 8 };
 // ------------------------------------------------------------------ the plan
 // int32 words written once per batch by bt_attn_plan: start[n], len[n] of the n = batch + 1 entries
 // (the sequences, longest first when there are at most kPlanSort of them, then the rows behind the
-// last sequence), then for each tile height kGran[g] the n + 1 running tile counts.
+// last sequence), then for each tile height gran_of(g) the n + 1 running tile counts.
 constexpr int kGrans = 5;
 constexpr int kPlanSort = 1024;
 __host__ __device__ constexpr int gran_of(int g) { return 8 << g; }
@@ -42,7 +42,6 @@ struct Plan {
   const int32_t* words;
   int n;  // entries
 };
-// a tile of one entry
 struct Item {
   int start, len, tile, entry;  // entry == n - 1: rows behind the last sequence
 };
@@ -312,7 +311,8 @@ __device__ __forceinline__ void stage_cols(uint32_t taddr, uint32_t tile, uint32
   }
 }
 template <typename T>
-__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, T* lo_dst, int col0, int d, float scale, bool row_ok) {
+__device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, T* lo_dst, int col0, int d, float scale,
+                                           bool row_ok) {
   float v[32];
   tmem_ld32(taddr, v);
   tmem_wait_ld();

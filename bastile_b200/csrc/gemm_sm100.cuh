@@ -1541,8 +1541,9 @@ int launch(Launch& L, cudaStream_t s) {
     const int kbk = kRowBytes / (L.dtype == BT_FP32 ? 4 : 2);
     const int64_t blocks = ceil_div(p.K0, kbk);
     p.kb_split = static_cast<int>(ceil_div(blocks, p.splits));
-    if (EPI != EPI_PLAIN || !p.out_fp32 || p.K1 != 0 || p.K2 != 0 || L.dual_b || ceil_div(blocks, p.kb_split) != p.splits ||
-        nt * p.splits > 0x7fffffff || p.addend != nullptr || p.addend_t != nullptr || p.n_seg0 > 0) {
+    if (EPI != EPI_PLAIN || !p.out_fp32 || p.K1 != 0 || p.K2 != 0 || L.dual_b || p.addend != nullptr ||
+        p.addend_t != nullptr || p.n_seg0 > 0 || ceil_div(blocks, p.kb_split) != p.splits ||
+        nt * p.splits > 0x7fffffff) {
       set_error("gemm: a cut contraction needs a plain fp32 result and no empty run (%d runs of %d k-blocks)", p.splits,
                 p.kb_split);
       return BT_ERR_ARG;

@@ -525,9 +525,9 @@ extern "C" int bt_logp_fwd(const void* hidden, const void* W, const int64_t* lab
 
 extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels,
                            const float* lse, void* masked, void* dlogits, void* dhidden, float* dhidden_parts_,
-                           void* dweight_out, float* dweight_acc, float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden,
-                           int64_t chunk, int64_t ignore_index, int dtype, int dweight_dtype, int32_t* status,
-                           void* stream) {
+                           void* dweight_out, float* dweight_acc, float* ws, int64_t rows, int64_t H, int64_t V,
+                           int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype, int dweight_dtype,
+                           int32_t* status, void* stream) {
   using namespace bt;
   Head h;
   if (int rc = fill_head(&h, "logp_bwd", W, rows, H, V, ld_hidden, hidden, chunk, ignore_index, dtype, status, stream))

@@ -102,6 +102,12 @@ def _f32(dev, *shape) -> Tensor:
     return torch.empty(shape, dtype=torch.float32, device=dev)
 
 
+def _runs(dev, rows: int, hdim: int, vocab: int, code: int) -> int:
+    """Partial sums of d hidden that the product of ``rows`` rows writes: counted for ``dev``'s SMs."""
+    with _lib.device_of(dev):
+        return int(_lib.get_lib().bt_dhidden_runs(rows, hdim, vocab, code))
+
+
 def _dweight_out(w: Tensor, w_dtype) -> Tensor:
     """The weight gradient's buffer: a registered destination if there is one."""
     out_dtype = w_dtype if w_dtype in (w.dtype, torch.float32) else w.dtype
@@ -157,7 +163,7 @@ class LinearLogProbsFunction(torch.autograd.Function):
         dlogits = torch.empty((step, ld), dtype=x.dtype, device=dev)
         masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev)
         code = _lib.dtype_code(x.dtype)
-        parts = _f32(dev, int(lib.bt_dhidden_runs(step, hdim, vocab, code)), step, hdim) if need_x else None
+        parts = _f32(dev, _runs(dev, step, hdim, vocab, code), step, hdim) if need_x else None
         acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
         ws = _f32(dev, rows + 1)
         st = _lib.status_word(dev)
@@ -166,8 +172,8 @@ class LinearLogProbsFunction(torch.autograd.Function):
                                  masked.data_ptr(), dlogits.data_ptr(), dx.data_ptr() if need_x else None,
                                  parts.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
                                  acc.data_ptr() if acc is not None else None, ws.data_ptr(), rows, hdim, vocab,
-                                 _ld(x), step, ignore_index, code, _lib.dtype_code(dw.dtype) if need_w else 0, st.data_ptr(),
-                                 _lib.stream_ptr(dev))
+                                 _ld(x), step, ignore_index, code, _lib.dtype_code(dw.dtype) if need_w else 0,
+                                 st.data_ptr(), _lib.stream_ptr(dev))
         _lib.check(rc, "bt_logp_bwd")
         return (dx.view(shape) if need_x else None, dw.to(w_dtype) if need_w else None, None, None, None)
 
@@ -191,7 +197,7 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
     masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
     code = _lib.dtype_code(x.dtype)
     # fp32 until the upstream gradient is known: one rounding to the hidden states' type
-    dx = _f32(dev, int(lib.bt_dhidden_runs(step, hdim, vocab, code)), rows, hdim) if need_x else None
+    dx = _f32(dev, _runs(dev, step, hdim, vocab, code), rows, hdim) if need_x else None
     acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     d = _lib.PolicyDesc(ptr(x), ptr(w), ptr(labels), ptr(old), ptr(adv), ptr(ref), ptr(cu), ptr(logp), ptr(loss),
@@ -277,14 +283,16 @@ def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tens
     mean over tokens whose target is not ``ignore_index``, or with ``cu_seqlens`` [sequences + 1] (packed
     offsets as for ``pack_sequences``) the mean over sequences of their tokens' means - sequences
     without a counted token are left out, tokens behind the last sequence count as ignored.
-    ``old_log_probs``, ``advantages`` and ``ref_log_probs`` have the target's shape and get no gradients."""
+    ``old_log_probs``, ``advantages`` and ``ref_log_probs`` have the target's shape and get no gradients.
+    Gradients of logits are formed in the hidden states' type relative to the largest token weight: with
+    fp16 those below 6e-8 of it vanish, so scale tiny advantages up (and ``loss`` down) there."""
     what = "fused_linear_policy_loss"
     for name, t in (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs)):
         if t is None and name == "ref_log_probs":
             continue
         if t.shape != target.shape or not t.dtype.is_floating_point:
-            raise ValueError(f"{what}: {name} must be floating-point values in the target's shape {tuple(target.shape)}, "
-                             f"got {t.dtype} {tuple(t.shape)}")
+            raise ValueError(f"{what}: {name} must be floating-point values in the target's shape "
+                             f"{tuple(target.shape)}, got {t.dtype} {tuple(t.shape)}")
     clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
         raise ValueError(f"{what}: need 0 <= clip_low <= 1 and clip_high >= 0, got {clip_low} and {clip_high}")

@@ -82,8 +82,8 @@ def _forward(q, k, v, sequences, scale, keep: bool):
         st = _lib.status_word(dev)
         with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
             rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                 lo.data_ptr() if keep else None, lse2.data_ptr() if keep else None, sequences.plan.data_ptr(), sequences.batch, t, hq,
-                                 k.shape[1], d, _strides(q), _strides(k), _strides(v), _strides(out), scale,
+                                 lo.data_ptr() if keep else None, lse2.data_ptr() if keep else None,
+                                 sequences.plan.data_ptr(), sequences.batch, t, hq, k.shape[1], d, _strides(q), _strides(k), _strides(v), _strides(out), scale,
                                  _lib.dtype_code(q.dtype), st.data_ptr(), _lib.stream_ptr(dev))
         _lib.check(rc, "bt_attn_fwd")
     return out, (q, k, v, out, lo, lse2, sequences.plan)
@@ -117,8 +117,8 @@ class PackedAttentionFunction(torch.autograd.Function):
             none = _lib.I64x2(0, 0)
             with _lib.device_of(dev), _lib.timed("attn_bwd", 1 + int(need_q) + int(need_kv), dev):
                 rc = lib.bt_attn_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                     lo.data_ptr(), lse2.data_ptr(), delta.data_ptr(), dq.data_ptr() if need_q else None,
-                                     dk.data_ptr() if need_kv else None, dv.data_ptr() if need_kv else None,
+                                     lo.data_ptr(), lse2.data_ptr(), delta.data_ptr(),
+                                     dq.data_ptr() if need_q else None, dk.data_ptr() if need_kv else None, dv.data_ptr() if need_kv else None,
                                      plan.data_ptr(), batch, t, hq, hk, d, _strides(dout), _strides(q), _strides(k),
                                      _strides(v), _strides(out), _strides(dq) if need_q else none,
                                      _strides(dk) if need_kv else none, _strides(dv) if need_kv else none, scale,
@@ -149,8 +149,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, sequences: PackedSequences
     if t != sequences.total_tokens:
         raise ValueError(f"packed_attention: q has {t} tokens, the packed sequences {sequences.total_tokens}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 <= scale <= 1e30:
-        raise ValueError(f"packed_attention: scale must be finite and not negative, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"packed_attention: scale must be between 1e-30 and 1e30, got {scale}")
     _lib.require_cuda(q, k, v, sequences.plan)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return PackedAttentionFunction.apply(q, k, v, sequences, scale)

@@ -462,21 +462,21 @@ int bt_attn_plan(const int32_t* cu_seqlens, int64_t batch, int64_t total, int32_
  * q, out [total, hq, d], k, v [total, hk, d]; BT_BF16 or BT_FP16; *_strides = element strides of
  * (token, head), multiples of 8; unit stride along d; d a multiple of 8, at most 128.  Rows behind the
  * last sequence are written as zeros.  out_lo (may be NULL, laid out as out): what rounding to `dtype` cut
- * off, for bt_attn_bwd; written for rows of sequences only, and so is lse2 (may be NULL): [hq, total] fp32, the base-2
- * log-sum-exp of the scaled scores. */
+ * off, for bt_attn_bwd; written for rows of sequences only, and so is lse2 (may be NULL): [hq, total]
+ * fp32, the base-2 log-sum-exp of the scaled scores.  scale is between 1e-30 and 1e30. */
 int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse2,
-                const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* q_strides,
-                const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale, int dtype,
-                int32_t* status, void* stream);
+                const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d,
+                const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                const int64_t* o_strides, float scale, int dtype, int32_t* status, void* stream);
 
 /* Gradients of bt_attn_fwd for the upstream gradient `dout` (bt_attn_fwd's out, out_lo - may
  * be NULL, with the gradients then a little less exact - and lse2 come back in).
  * dq may be NULL, and so may dk and dv together; `delta` is [hq, total] fp32 scratch.  Rows behind the
  * last sequence get zeros.  No atomics: the same inputs give the same bits. */
 int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* out_lo,
-                const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch, int64_t total,
-                int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides, const int64_t* q_strides,
-                const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch,
+                int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides,
+                const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                 const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides, float scale,
                 int dtype, int32_t* status, void* stream);
 
@@ -501,19 +501,20 @@ int64_t bt_dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype);
 int bt_sum_runs(const float* parts, void* out, int64_t n, int64_t runs, int64_t stride, const float* alpha, int dtype,
                 void* stream);
 /* Gradients for the upstream gradient dlogp[rows]; logits are recomputed.  dhidden [rows, H] in `dtype`
- * (with dhidden_parts [runs, min(chunk, rows), H] fp32) and dweight [V, H] in dweight_dtype may each be NULL; dweight_acc [V, H] fp32 is needed for dweight when
- * rows > chunk; ws: rows + 1 floats. */
+ * (with dhidden_parts [runs, min(chunk, rows), H] fp32) and dweight [V, H] in dweight_dtype may each be
+ * NULL; dweight_acc [V, H] fp32 is needed for dweight when rows > chunk; ws: rows + 1 floats. */
 int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels, const float* lse,
                 void* masked, void* dlogits, void* dhidden, float* dhidden_parts, void* dweight, float* dweight_acc,
-                float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
-                int dweight_dtype, int32_t* status, void* stream);
+                float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk,
+                int64_t ignore_index, int dtype, int dweight_dtype, int32_t* status, void* stream);
 
 /* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
  * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
- * counts).  loss [1], averages [4] = (kl, clipped fraction, largest weight of a token, 1 / it), logp [rows].  dhidden (fp32 [runs, rows, H], may
- * be NULL) and the weight gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose
- * dlogits stay in `logits`) are relative to averages[2]: the caller multiplies by it and the upstream
- * gradient.  masked, logits: needed with either gradient.
+ * counts).  loss [1], averages [4] = (kl, clipped fraction, largest weight of a token, 1 / it),
+ * logp [rows].  dhidden (fp32 [runs, rows, H] with runs as from bt_dhidden_runs, may be NULL) and the weight
+ * gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in
+ * `logits`) are relative to averages[2]: the caller multiplies by it and the upstream gradient.
+ * masked, logits: needed with either gradient.
  * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats. */
 typedef struct {
   const void* hidden;

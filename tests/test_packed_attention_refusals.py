@@ -40,7 +40,7 @@ def test_mismatched_tensors_and_plans():
         packed_attention(q[0], k, v, _seqs(4))
     with pytest.raises(TypeError, match="share"):
         packed_attention(q, k.half(), v, _seqs(4))
-    for scale in (-0.1, float("inf"), float("nan")):
+    for scale in (-0.1, 0.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="scale"):
             packed_attention(q, k, v, _seqs(4), scale=scale)
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -71,7 +71,8 @@ def test_c_entry_points():
     for kw, text in ((dict(q=None), b"null"), (dict(plan=None), b"null plan"), (dict(hq=3), b"multiple"),
                      (dict(d=68), b"head_dim"), (dict(d=256), b"head_dim"), (dict(dtype=_lib.BT_FP32), b"dtype"),
                      (dict(qs=bad), b"strides"), (dict(q=C.c_void_p(8)), b"aligned"), (dict(total=0), b"token count"),
-                     (dict(total=1 << 30), b"token count"), (dict(batch=-1), b"batch"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale")):
+                     (dict(total=1 << 30), b"token count"), (dict(batch=-1), b"batch"), (dict(scale=-1.0), b"scale"),
+                     (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale")):
         assert fwd(**kw) == -1 and text in lib.bt_last_error(), (kw, lib.bt_last_error())
 
     def bwd(dk=one, dv=one, lse=one):
