@@ -1479,6 +1479,7 @@ struct Launch {
   bool two_pairs = false; // (a1, b1) is a second contraction into the same accumulator
   int a_split = A_WHOLE;  // A_SPLIT_K / A_SPLIT_M: A is (a0, a1, a2), B is b0 alone
   int dtype = BT_BF16;    // storage of the operands: BT_BF16, BT_FP16 or BT_FP32 (tf32 math)
+  bool single = false;    // 128-row tiles even where CTA pairs are on (the same bits)
   Params p{};
 };
 
@@ -1497,7 +1498,7 @@ template <int EPI>
 int launch(Launch& L, cudaStream_t s) {
   bind_context_once();
   Params& p = L.p;
-  const bool pair = pair_mode() != 0;
+  const bool pair = pair_mode() != 0 && !L.single;
   const int n_tile = L.dual_b ? BN / 2 : BN;
   p.K0 = static_cast<int>(L.a0.k);
   p.K1 = L.two_pairs ? static_cast<int>(L.a1.k) : 0;

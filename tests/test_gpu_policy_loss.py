@@ -446,3 +446,18 @@ def test_second_derivatives_are_refused():
     (g,) = torch.autograd.grad(fused_linear_log_probs(x, w, t), x, up.requires_grad_(True), create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_log_probs_do_not_depend_on_the_rows_beside_them(dtype):
+    """Few rows, and an odd number of 128-row tiles, take another tile shape than full pairs of them: the
+    same sums in the same order, so that a policy's ratio to itself is 1 whatever it was batched with."""
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_log_probs, fused_linear_policy_loss
+
+    x, w, t, _, _ = make(512, 264, 4099, dtype, seed=11)
+    with torch.no_grad():
+        full = fused_linear_log_probs(x, w, t)
+        for n in (1, 61, 128, 129, 300):
+            assert torch.equal(fused_linear_log_probs(x[:n], w, t[:n]), full[:n])
+        pl = fused_linear_policy_loss(x, w, t, full, torch.ones_like(full), chunk_size=100)
+        assert torch.equal(pl.log_probs, full) and pl.clip_fraction.item() == 0.0
