@@ -88,7 +88,17 @@ struct BwdGeo {
 // a warp writes both into the 64 columns that it has just read, P^T in the first 32.  S^T is free as
 // soon as it is in registers, and S^T of the next tile is computed under this tile's dS phase; the
 // exponentials of the next tile then run under dV, dK and dP^T.
-template <typename T, int DT>
+//
+// PAIR: clusters of two CTAs.  The first key tile of a sequence has all its query tiles to go through,
+// 1.75 us each, while the rest of a short batch is long done.  Where that is more than twice the time of
+// an even deal (L / TQ of the longest sequence against the sum of L (L + 128) / (256 TQ) over all, heads
+// times, on all SMs) both CTAs of a cluster take half of a key tile's query tiles, and each gets one of the
+// other's two sums through distributed shared memory; else they take a key tile each.  Twice, because the
+// 5 us that a CTA needs besides its query tiles are paid twice.  Measured, alone / shared, us (key/value
+// heads x tokens, 4 query heads each, d = 128, bf16; the even deal as a part of the longest): 8 x 1024
+// (0.24) 56 / 35, 2 x 8192 (0.44) 380 / 204, 8 x 2048 (0.46) 106 / 67, a ragged batch of 8 x 4096 (0.66)
+// 79 / 95, 2 x 16384 (0.87) 809 / 766, 8 x 4096 (0.89) 207 / 217, 8 x two of 2048 (0.92) 113 / 134.
+template <typename T, int DT, bool PAIR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const Params p) {
@@ -152,14 +162,21 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
-  const int hk = static_cast<int>(blockIdx.x) % p.hk;
+  const bool shared_tiles = PAIR && p.plan.area() < p.share * static_cast<float>(p.plan.longest());
+  const int unit = static_cast<int>(shared_tiles ? blockIdx.x / 2 : blockIdx.x);
+  const int hk = unit % p.hk;
   Item it{};
-  const bool live = plan_item(p.plan, p.gran, static_cast<int>(blockIdx.x) / p.hk, lane, &it);
+  const bool live = plan_item(p.plan, p.gran, unit / p.hk, lane, &it);
   const bool behind = live && it.entry == p.plan.n - 1;
   const int kv0 = live ? it.tile * kTile : 0;
   const int i0 = kv0 / p.tq;                                     // first query tile that sees a key of this one
   const int per = live ? (it.len + p.tq - 1) / p.tq - i0 : 0;    // query tiles of one packed group
-  const int n = (live && !behind) ? per * p.nsub : 0;
+  const int all = (live && !behind) ? per * p.nsub : 0;
+  // this CTA's query tiles are `all` of them from x0 on, n of them; with few, the first CTA takes all
+  const int rank = shared_tiles ? static_cast<int>(blockIdx.x & 1) : 0;
+  const bool sharing = shared_tiles && all >= 4;
+  const int x0 = sharing && rank != 0 ? (all + 1) / 2 : 0;
+  const int n = sharing ? (rank != 0 ? all / 2 : (all + 1) / 2) : (rank != 0 ? 0 : all);
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -173,7 +190,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
       uint32_t fix_phase = 0;
       bool ok = true;
-      int sub = 0, i = i0;
+      int sub = x0 / per, i = i0 + x0 % per;
       int qs = 0;
       uint32_t q_par = 1;
       for (int x = 0; ok && x < n; ++x) {
@@ -272,13 +289,18 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
       if (ok) mma_commit(done);
     }
+    if (PAIR && sharing) {
+      __syncwarp();
+      ptx::cluster_sync_all();
+      ptx::cluster_sync_all();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // --------------------------------------------------------- P^T, dS^T, stores
     const int half = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const int kv = kv0 + row;
-    if (behind && kv < it.len) {
+    if (behind && rank == 0 && kv < it.len) {
       const int64_t token = static_cast<int64_t>(it.start) + kv;
       T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
       T* dv = static_cast<T*>(p.dv.ptr) + token * p.dv.st + hk * p.dv.sh;
@@ -292,7 +314,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const uint32_t ts = tmem + lane_base + half * 64, tp = ts + 128;
       const f32x2 c2 = pair(p.scale_log2, p.scale_log2);
       bool ok = true;
-      int i = i0;
+      int i = i0 + x0 % per;
       for (int x = 0; x < n; ++x) {
         const int st = x & 1;
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&vec_full[st], (x >> 1) & 1, cta_abort, p.status, ST_MATH) &&
@@ -361,10 +383,30 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (++i == i0 + per) i = i0;
       }
       if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(done, 0, cta_abort, p.status, ST_MATH));
-      if (ok) {
-        ptx::tcgen05_fence_after_sync();
-        const bool row_ok = kv < it.len;
-        const int64_t token = static_cast<int64_t>(it.start) + kv;
+      if (ok) ptx::tcgen05_fence_after_sync();
+      const bool row_ok = kv < it.len;
+      const int64_t token = static_cast<int64_t>(it.start) + kv;
+      if (PAIR && sharing) {
+        // the first CTA of the two ends with dV, the second with dK; whatever goes wrong in one of them, both
+        // come through both barriers
+        const uint32_t mine = tmem + lane_base + 256 + (rank != 0 ? DT : 0);
+        const uint32_t theirs = tmem + lane_base + 256 + (rank != 0 ? 0 : DT);
+        const View& view = rank != 0 ? p.dk : p.dv;
+        T* dst = static_cast<T*>(view.ptr) + token * view.st + hk * view.sh;
+        __syncwarp();
+        ptx::cluster_sync_all();  // the products of both are done: the tiles of Q may be overwritten
+        if (ok)
+#pragma unroll 1
+          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
+            send_cols(theirs + c, sQ + (c / 4 * 128 + row) * 16, static_cast<uint32_t>(rank ^ 1));
+        __syncwarp();
+        ptx::cluster_sync_all();
+        if (ok)
+#pragma unroll 1
+          for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
+            store_sum_cols<T>(mine + c, sQ + (c / 4 * 128 + row) * 16, dst, c, p.d, rank != 0 ? p.scale : 1.0f,
+                              row_ok);
+      } else if (ok) {
         T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
         T* dv = static_cast<T*>(p.dv.ptr) + token * p.dv.st + hk * p.dv.sh;
         // (one store per tile and output here: a staged tile store measured 1% slower)
@@ -652,30 +694,40 @@ struct Maps {
   CUtensorMap q, k, v, g, dq;
 };
 
+// Key tiles are shared where the even deal, area * hk / (2 kTile * SMs), is below half of the longest
+// sequence.  With sequences of one length that takes a total below this bound, which the host can see.
+float share_bound(int hk) { return kTile * static_cast<float>(sm_count()) / static_cast<float>(hk); }
+
 template <typename K, typename... A>
-int launch_bwd(K* kern, int smem, std::atomic<uint64_t>* reserved, int64_t grid, const char* what, cudaStream_t s,
-               const A&... args) {
+int launch_bwd(K* kern, int smem, std::atomic<uint64_t>* reserved, int64_t grid, int cluster, const char* what,
+               cudaStream_t s, const A&... args) {
   BT_CHECK_LAUNCHED(reserve_smem(kern, smem, reserved), what);
   BT_CHECK_ARG(grid <= 0x7fffffffll, "%s: too many tiles (%lld)", what, (long long)grid);
-  BT_CHECK_LAUNCHED(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(kBwdThreads), smem, s, args...),
+  BT_CHECK_LAUNCHED(launch_dependent_clusters(kern, dim3(static_cast<unsigned>(grid)), dim3(kBwdThreads), smem, cluster,
+                                              s, args...),
                     what);
   return BT_OK;
 }
 
 template <typename T, int DT>
 int run_bwd(const Maps& m, Params p, int64_t batch, cudaStream_t s) {
-  static std::atomic<uint64_t> reserved[2];
+  static std::atomic<uint64_t> reserved[3];
   if (p.dk.ptr != nullptr) {
     p.gran = gran_index(kTile);
-    if (int rc = launch_bwd(attn_dkv_kernel<T, DT>, BwdGeo<DT>::kSmem, &reserved[0],
-                            max_items(p.total, batch, kTile) * p.hk, "attn_bwd dk, dv", s, m.q, m.k, m.v, m.g, p))
-      return rc;
+    p.share = share_bound(p.hk);
+    const int64_t items = max_items(p.total, batch, kTile) * p.hk;
+    const int rc = static_cast<float>(p.total) < p.share
+                       ? launch_bwd(attn_dkv_kernel<T, DT, true>, BwdGeo<DT>::kSmem, &reserved[2], 2 * items, 2,
+                                    "attn_bwd dk, dv", s, m.q, m.k, m.v, m.g, p)
+                       : launch_bwd(attn_dkv_kernel<T, DT, false>, BwdGeo<DT>::kSmem, &reserved[0], items, 1,
+                                    "attn_bwd dk, dv", s, m.q, m.k, m.v, m.g, p);
+    if (rc) return rc;
   }
   if (p.dq.ptr != nullptr) {
     p.gran = gran_index(p.tq);
     if (int rc = launch_bwd(attn_dq_kernel<T, DT>, BwdGeo<DT>::kSmem, &reserved[1],
-                            max_items(p.total, batch, p.tq) * p.hk * p.nsub, "attn_bwd dq", s, m.q, m.k, m.v, m.g, m.dq,
-                            p))
+                            max_items(p.total, batch, p.tq) * p.hk * p.nsub, 1, "attn_bwd dq", s, m.q, m.k, m.v, m.g,
+                            m.dq, p))
       return rc;
   }
   return BT_OK;

@@ -33,6 +33,8 @@ attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* 
                  int32_t* __restrict__ status) {
   grid_dependency_wait();
   __shared__ int s_len[kPlanSort];
+  __shared__ unsigned long long s_area;  // below 2^61: the lengths sum to less than 2^30
+  __shared__ int s_longest;
   const int tid = threadIdx.x;
   const int n = batch + 1;
   int32_t* start = words;
@@ -46,6 +48,14 @@ attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* 
   }
   bad = __syncthreads_or(bad);
   if (bad && tid == 0 && status != nullptr) atomicOr(status, BT_STATUS_BAD_SEQUENCES);
+  if (tid == 0) s_area = 0, s_longest = 0;
+  __syncthreads();
+  if (!bad)
+    for (int i = tid; i < batch; i += kPlanThreads) {
+      const int l = cu[i + 1] - cu[i];
+      atomicAdd(&s_area, static_cast<unsigned long long>(l) * (l + kTile));
+      atomicMax(&s_longest, l);
+    }
   if (batch <= kPlanSort) {
     // longest first: the tiles of a launch are started in plan order, so the last ones are small
     if (tid < batch) s_len[tid] = bad ? 0 : cu[tid + 1] - cu[tid];
@@ -69,6 +79,10 @@ attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* 
     len[batch] = total - covered;
   }
   __syncthreads();
+  if (tid == 0) {
+    words[2 * n + kGrans * (n + 1)] = __float_as_int(static_cast<float>(s_area));
+    words[2 * n + kGrans * (n + 1) + 1] = s_longest;
+  }
   const int g = tid >> 5, lane = tid & 31;
   if (g < kGrans) {  // one warp per tile height: running tile counts
     int32_t* pre = words + 2 * n + g * (n + 1);

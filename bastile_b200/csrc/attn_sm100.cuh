@@ -27,7 +27,9 @@ enum : int { ST_LOAD = 1, ST_ISSUE = 2, ST_ISSUE2 = 4, ST_MATH = 8 };
 // ------------------------------------------------------------------ the plan
 // int32 words written once per batch by bt_attn_plan: start[n], len[n] of the n = batch + 1 entries
 // (the sequences, longest first when there are at most kPlanSort of them, then the rows behind the
-// last sequence), then for each tile height gran_of(g) the n + 1 running tile counts.
+// last sequence), then for each tile height gran_of(g) the n + 1 running tile counts, then the sum over
+// sequences of len (len + kTile) (fp32) - twice the tokens that a step through all tiles covers, times
+// kTile - and the greatest length.
 constexpr int kGrans = 5;
 constexpr int kPlanSort = 1024;
 __host__ __device__ constexpr int gran_of(int g) { return 8 << g; }
@@ -36,11 +38,15 @@ __host__ __device__ inline int gran_index(int tokens) {
   while (gran_of(g) < tokens) ++g;
   return g;
 }
-inline int64_t plan_words(int64_t batch) { return (batch + 1) * 2 + kGrans * (batch + 2); }
+inline int64_t plan_words(int64_t batch) { return (batch + 1) * 2 + kGrans * (batch + 2) + 2; }
 
 struct Plan {
   const int32_t* words;
   int n;  // entries
+  __device__ __forceinline__ float area() const {
+    return __int_as_float(__ldg(words + 2 * n + kGrans * (n + 1)));
+  }
+  __device__ __forceinline__ int longest() const { return __ldg(words + 2 * n + kGrans * (n + 1) + 1); }
 };
 struct Item {
   int start, len, tile, entry;  // entry == n - 1: rows behind the last sequence
@@ -326,6 +332,43 @@ __device__ __forceinline__ void store_cols(uint32_t taddr, T* dst, T* lo_dst, in
     if (lo_dst != nullptr) st_global_v4(lo_dst + col0 + g * 8, lo);
   }
 }
+// 32 fp32 columns of a row to the same place of the CTA `peer` of the cluster, and those received added to
+// this CTA's own.  The 16 bytes of neighbouring rows lie side by side.
+__device__ __forceinline__ void send_cols(uint32_t taddr, uint32_t place, uint32_t peer) {
+  float v[32];
+  tmem_ld32(taddr, v);
+  tmem_wait_ld();
+  uint32_t there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(place), "r"(peer));
+#pragma unroll
+  for (int g = 0; g < 8; ++g)
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + g * 128 * 16), "f"(v[4 * g]),
+                 "f"(v[4 * g + 1]), "f"(v[4 * g + 2]), "f"(v[4 * g + 3])
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void store_sum_cols(uint32_t taddr, uint32_t place, T* dst, int col0, int d, float scale,
+                                               bool row_ok) {
+  float v[32];
+  tmem_ld32(taddr, v);
+  tmem_wait_ld();
+  if (!row_ok) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float r[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(r[4 * h]), "=f"(r[4 * h + 1]), "=f"(r[4 * h + 2]), "=f"(r[4 * h + 3])
+                   : "r"(place + (2 * g + h) * 128 * 16)
+                   : "memory");
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = pack2<T>((v[g * 8 + 2 * e] + r[2 * e]) * scale, (v[g * 8 + 2 * e + 1] + r[2 * e + 1]) * scale);
+    if (col0 + g * 8 < d) st_global_v4(dst + col0 + g * 8, make_uint4(o[0], o[1], o[2], o[3]));
+  }
+}
 // After a warp has staged its part: say so, and (the one thread) wait for all and store the tile, and the
 // second one unless lo_tile is 0.
 template <int DT>
@@ -357,6 +400,7 @@ struct Params {
   int hq, hk, d, total;
   int gp, gp_shift, tq, nsub;  // packed heads, log2, tokens per tile, packed groups per kv head
   int gran;                    // index of the tile height that this kernel's items have
+  float share;                 // dK, dV: plan's area per token of the longest below which key tiles are shared
   float scale, scale_log2;
   float* lse2;   // [hq][total] base-2 log-sum-exp of the scaled scores
   float* delta;  // [hq][total] dot(dO, O)

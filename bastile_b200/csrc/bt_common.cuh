@@ -243,20 +243,29 @@ __device__ __forceinline__ void grid_dependency_wait() {
 }
 int dependent_launch_mode();  // 1 (default): kernels are launched as programmatic dependents (c_api.cu)
 
+// In clusters of `cluster` CTAs along x (1: ordinary CTAs).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_dependent(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                                    cudaStream_t s, Args... args) {
+inline cudaError_t launch_dependent_clusters(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster,
+                                             cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = dependent_launch_mode() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_dependent(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                    cudaStream_t s, Args... args) {
+  return launch_dependent_clusters(kern, grid, block, smem, 1, s, args...);
 }
 
 #define BT_CHECK_LAUNCHED(err, what)                                         \

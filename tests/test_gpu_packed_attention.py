@@ -123,6 +123,20 @@ def test_long_and_many(lens, hq, hk, d):
         close(got[n], want[n], n)
 
 
+@pytest.mark.parametrize("lens,hq,hk,d", [([500, 30, 11], 64, 16, 64), ([100] * 4, 80, 40, 64),
+                                           ([700, 100], 64, 64, 72)])
+def test_key_tiles_of_one_cta_or_two(lens, hq, hk, d):
+    """dK and dV of the longest sequence's key tiles by two CTAs each while an even deal would take half their
+    time, by one each with sequences of one length or more heads."""
+    q, k, v, cu, dout = inputs(lens, hq, hk, d, torch.bfloat16, seed=6, tail=5)
+    want = oracle(q, k, v, cu, d ** -0.5, dout)
+    got = attend(q, k, v, cu, dout)
+    for n in got:
+        close(got[n], want[n], n)
+    again = attend(q, k, v, cu, dout)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
 def test_more_sequences_than_are_sorted():
     lens = [(i * 7) % 5 for i in range(1500)]
     q, k, v, cu, dout = inputs(lens, 2, 1, 64, torch.float16, seed=4, tail=11)

@@ -84,4 +84,4 @@ def test_c_entry_points():
     assert bwd() == -1 and b"dv" in lib.bt_last_error()
     assert lib.bt_attn_plan(None, 1, 4, one, None, None) == -1 and b"null" in lib.bt_last_error()
     assert lib.bt_attn_plan(one, -1, 4, one, None, None) == -1
-    assert lib.bt_attn_plan_words(-1) == 0 and lib.bt_attn_plan_words(3) == 4 * 2 + 5 * 5
+    assert lib.bt_attn_plan_words(-1) == 0 and lib.bt_attn_plan_words(3) == 4 * 2 + 5 * 5 + 2
