@@ -42,20 +42,29 @@ attn_plan_kernel(const int32_t* __restrict__ cu, int batch, int total, int32_t* 
   // offsets have to start at 0, never fall, and end within the tensor; anything else is reported and
   // read as "no sequence at all", so that no kernel that follows the plan can leave the tensors
   bool bad = false;
+  unsigned long long area = 0;
+  int longest = 0;
+  if (tid == 0) s_area = 0, s_longest = 0;
   for (int i = tid; i < batch; i += kPlanThreads) {
     const int a = cu[i], b = cu[i + 1];
-    bad |= a < 0 || b < a || b > total || (i == 0 && a != 0);
+    const bool wrong = a < 0 || b < a || b > total || (i == 0 && a != 0);
+    bad |= wrong;
+    if (!wrong) {
+      area += static_cast<unsigned long long>(b - a) * (b - a + kTile);
+      longest = max(longest, b - a);
+    }
   }
   bad = __syncthreads_or(bad);
-  if (bad && tid == 0 && status != nullptr) atomicOr(status, BT_STATUS_BAD_SEQUENCES);
-  if (tid == 0) s_area = 0, s_longest = 0;
-  __syncthreads();
-  if (!bad)
-    for (int i = tid; i < batch; i += kPlanThreads) {
-      const int l = cu[i + 1] - cu[i];
-      atomicAdd(&s_area, static_cast<unsigned long long>(l) * (l + kTile));
-      atomicMax(&s_longest, l);
+  if (!bad && (tid & ~31) < batch) {  // warps that have seen a sequence
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) area += __shfl_xor_sync(0xffffffffu, area, o);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if ((tid & 31) == 0) {
+      atomicAdd(&s_area, area);
+      atomicMax(&s_longest, longest);
     }
+  }
+  if (bad && tid == 0 && status != nullptr) atomicOr(status, BT_STATUS_BAD_SEQUENCES);
   if (batch <= kPlanSort) {
     // longest first: the tiles of a launch are started in plan order, so the last ones are small
     if (tid < batch) s_len[tid] = bad ? 0 : cu[tid + 1] - cu[tid];

@@ -385,7 +385,7 @@ __device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32
       if (lo_tile != 0) tma_store_3d(lo_tm, lo_tile + j * kBoxBytes, j * 64, head, token);
     }
     ptx::bulk_commit_group();
-    ptx::bulk_wait_group<0>();
+    ptx::bulk_wait_group_read<0>();
   }
 }
 
