@@ -21,23 +21,30 @@ __device__ __forceinline__ bool counted(int64_t label, int64_t ignore_index, int
   return label != ignore_index && label >= 0 && label < vocab;
 }
 
-// (max, sum exp) of a row from its half tiles; all lanes of the warp get the result.
+// (max, sum exp) of a row from its half tiles; all lanes of the warp get the result.  Two passes, eight
+// loads of a lane in flight: a running (max, sum) waits for each load and exponential in turn (1187 half
+// tiles: 8.0 -> 5.0 us for 61 rows).
 __device__ __forceinline__ float2 merge_stats(const float2* __restrict__ ts, int n_vt, int lane) {
+  constexpr int kAhead = 8;
   float mx = -1e30f, sum = 0.f;
-  for (int i = lane; i < n_vt; i += 32) {
-    const float2 t = ts[i];
-    const float nm = fmaxf(mx, t.x);
-    sum = sum * __expf(mx - nm) + t.y * __expf(t.x - nm);
-    mx = nm;
+  for (int i0 = lane; i0 < n_vt; i0 += 32 * kAhead) {
+    float x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = i0 + u * 32 < n_vt ? ts[i0 + u * 32].x : -1e30f;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) mx = fmaxf(mx, x[u]);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float omx = __shfl_xor_sync(0xffffffffu, mx, o);
-    const float osum = __shfl_xor_sync(0xffffffffu, sum, o);
-    const float nm = fmaxf(mx, omx);
-    sum = sum * __expf(mx - nm) + osum * __expf(omx - nm);
-    mx = nm;
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  for (int i0 = lane; i0 < n_vt; i0 += 32 * kAhead) {
+    float2 t[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) t[u] = i0 + u * 32 < n_vt ? ts[i0 + u * 32] : make_float2(-1e30f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) sum += t[u].y * __expf(t[u].x - mx);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return make_float2(mx, sum);
 }
 
