@@ -546,6 +546,9 @@ __device__ __forceinline__ void epi_lce(const Params& p, uint32_t taddr, int64_t
 // model's own lm_head would; a log-probability that is compared with another one to a percent cannot
 // afford the 2^-9 |logit| of that.)  Two passes over the accumulator - maximum, then exponentials -
 // because tensor memory is cheap to read twice while the next tile's 32k-cycle main loop runs.
+// (512 rows x 1024 against 32000: 34.9 us, a plain 16-bit result 32.6; with H = 4096 104.8 and 102.7.)
+// What remains is what the tensor cores cut off their partial sums, 1.1e-6 of the log-probabilities' 2-norm
+// (fp32 arithmetic: 5e-7).
 // SHIFT: also stores logit - half-tile maximum in T.  Near the maximum, where the softmax has its
 // mass, that difference is small and its rounding harmless.
 template <typename T, bool SHIFT>

