@@ -757,9 +757,10 @@ int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns) {
 extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
                            const void* out_lo, const float* lse2, float* delta, void* dq, void* dk, void* dv,
                            const int32_t* plan, int64_t batch, int64_t total, int64_t hq, int64_t hk, int64_t d,
-                           const int64_t* g_strides, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                           const int64_t* o_strides, const int64_t* dq_strides, const int64_t* dk_strides,
-                           const int64_t* dv_strides, float scale, int dtype, int32_t* status, void* stream) {
+                           const int64_t* g_strides, const int64_t* q_strides, const int64_t* k_strides,
+                           const int64_t* v_strides, const int64_t* o_strides, const int64_t* dq_strides,
+                           const int64_t* dk_strides, const int64_t* dv_strides, float scale, int dtype,
+                           int32_t* status, void* stream) {
   using namespace bt;
   using namespace bt::attn;
   Params p{};

@@ -13,10 +13,10 @@
 // and exponentials run meanwhile, and under its start and its end as well, which no second tile inside
 // one CTA can do.  Against two tiles per CTA and one CTA per SM (bf16, 32 / 8 heads of 128): 861 -> 830
 // thousand cycles on one sequence of 8192 tokens, 69 -> 60 us on a ragged batch of 4096.
-// Measured: 8192 tokens 457 us (468 with the residual stored), 1.20 PFLOP/s of the products executed (masked halves of the diagonal tiles
-// included); at 4096 the matrix pipe is busy in 48% of the cycles and the exponentials' in 50%, the rest is
-// the hand-over between them.  Exponentials on the FMA pipes instead took fewer cycles and the same time:
-// what is left is the chip's power limit.
+// Measured: 8192 tokens 457 us (468 with the residual stored), 1.20 PFLOP/s of the products executed (masked
+// halves of the diagonal tiles included); at 4096 the matrix pipe is busy in 48% of the cycles and the
+// exponentials' in 50%, the rest is the hand-over between them.  Exponentials on the FMA pipes instead took
+// fewer cycles and the same time: what is left is the chip's power limit.
 #include <mutex>
 
 #include "attn_sm100.cuh"

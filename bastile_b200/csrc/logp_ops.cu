@@ -321,9 +321,10 @@ struct Head {
 // pairs' advantage (their tiles read half as much of W each), 7 - 13% at whole numbers of pair tiles.
 // Log-probabilities, forward, pairs / single CTAs, us: vocabulary 151936 x 4096, 61 rows 254 / 235, 128 rows
 // 276 / 240, 129 rows 285 / 341, 384 rows 543 / 473, 512 rows 532 / 611, 640 rows 766 / 724, 1024 rows
-// 1020 / 1093; 32000 x 1024, 640 rows 51 / 42.
+// 1020 / 1093; 32000 x 1024, 640 rows 51 / 42.  (Tiles drawn at run time are the pairs' alone.)
 bool narrow_tiles(int64_t rows) {
-  return ceil_div(rows, 128) * 128 * 1.1 < static_cast<double>(ceil_div(rows, 256) * 256);
+  return gemm::dynamic_tiles() == 0 &&
+         ceil_div(rows, 128) * 128 * 1.1 < static_cast<double>(ceil_div(rows, 256) * 256);
 }
 
 gemm::Launch head_product(const Head& h, const void* hidden, const int64_t* labels, int64_t rows, int64_t ld_hidden) {
