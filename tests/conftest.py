@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import sys
+from multiprocessing.context import SpawnContext
 from pathlib import Path
 
 import numpy as np
@@ -32,6 +33,24 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+def _share_by_name(target, *args, **kwargs):
+    torch.multiprocessing.set_sharing_strategy("file_system")
+    target(*args, **kwargs)
+
+
+class _Rank(SpawnContext.Process):
+    def __init__(self, group=None, target=None, name=None, args=(), **more):
+        super().__init__(group, _share_by_name, name, (target, *args), **more)
+
+
+@pytest.fixture(autouse=True)
+def _tensors_outlive_their_process(monkeypatch):
+    """Spawned ranks hand tensors to the test through a queue and exit.  By default the receiver fetches a
+    tensor's file descriptor from its sender, which fails if that is gone by then (a rank ends a few
+    milliseconds after its ``put``); shared by name they stay until they have been received."""
+    monkeypatch.setattr(SpawnContext, "Process", _Rank)
 
 
 def load_golden(name: str):
