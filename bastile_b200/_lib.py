@@ -13,6 +13,8 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
 
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
+from torch.utils.dlpack import from_dlpack, to_dlpack
 
 BT_BF16, BT_FP16, BT_FP32 = 0, 1, 2
 
@@ -209,26 +211,54 @@ class device_of:
 # here; the ops that allocate weight gradients themselves (MLP block, fused loss) then write
 # straight into the bucket instead of into a fresh tensor that would be copied there afterwards.
 _grad_sinks: dict[int, torch.Tensor] = {}
+# A destination is lent as a tensor with a storage of its own over the same memory, so that a weak
+# reference to that storage tells when the last tensor on it (the weight's ``.grad``, a slice of it in a
+# user's hands) is gone; and the destinations whose gradient the optimizer has not used yet.
+_grad_lent: dict[int, StorageWeakRef] = {}
+_grad_held: set[int] = set()
 
 
 def register_grad_sink(weight: torch.Tensor, destination: torch.Tensor) -> None:
-    _grad_sinks[weight.data_ptr()] = destination
+    key = weight.data_ptr()
+    _grad_sinks[key] = destination
+    _grad_lent.pop(key, None)
+    _grad_held.discard(key)
 
 
 def unregister_grad_sinks(destinations) -> None:
     ids = {id(d) for d in destinations}
     for key in [k for k, v in _grad_sinks.items() if id(v) in ids]:
         del _grad_sinks[key]
+        _grad_lent.pop(key, None)
+        _grad_held.discard(key)
+
+
+def hold_grad_sink(weight: torch.Tensor) -> None:
+    """``weight``'s destination holds its gradient: not lent again before ``release_grad_sinks``."""
+    if weight.data_ptr() in _grad_sinks:
+        _grad_held.add(weight.data_ptr())
+
+
+def release_grad_sinks(weights) -> None:
+    _grad_held.difference_update(w.data_ptr() for w in weights)
 
 
 def grad_sink(weight: torch.Tensor, dtype: torch.dtype):
-    """The registered destination for ``weight``'s gradient if it fits (shape, dtype, device)."""
-    dest = _grad_sinks.get(weight.data_ptr())
+    """The registered destination for ``weight``'s gradient if it fits (shape, dtype, device) and nothing
+    that is still needed lies there: a weight that is used several times gets one contribution in place,
+    the others in tensors of their own, which autograd adds."""
+    key = weight.data_ptr()
+    dest = _grad_sinks.get(key)
     if dest is None or dest.shape != weight.shape or dest.dtype != dtype or dest.device != weight.device:
         return None
-    # a FRESH view object: autograd only adopts an incoming gradient without cloning it when nothing
-    # else holds a reference to that tensor object (the registry keeps the original)
-    return dest.view(dest.shape)
+    lent = _grad_lent.get(key)
+    if key in _grad_held or (lent is not None and not lent.expired()):
+        return None
+    # a FRESH tensor object: autograd only adopts an incoming gradient without cloning it when nothing
+    # else holds a reference to that object (the registry keeps the original)
+    out = from_dlpack(to_dlpack(dest))
+    _grad_lent[key] = StorageWeakRef(out.untyped_storage())
+    return out
 
 
 # Per (device, stream) scratch that must start zeroed and that kernels leave zeroed.

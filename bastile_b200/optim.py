@@ -397,6 +397,7 @@ class ShardedAdamW:
             if side is not None:
                 g.record_stream(side)
         p.grad = None
+        _lib.hold_grad_sink(p)  # until step(): what else the weight is differentiated for goes elsewhere
         b.arrived.add(i)
         b.pending -= 1
         if b.pending == 0:
@@ -441,6 +442,8 @@ class ShardedAdamW:
             b.arrived = set()
         for dev, side in self._streams.items():
             torch.cuda.current_stream(dev).wait_stream(side)
+        for b in self.buckets:
+            _lib.release_grad_sinks(b.params)
         self.step_count += 1
 
     def close(self):
