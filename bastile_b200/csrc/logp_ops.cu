@@ -106,16 +106,20 @@ logp_coef_kernel(const float* __restrict__ dlogp, const int64_t* __restrict__ la
 }
 
 // Rows of `x` that count, copied; zeros in the place of the others, which meet zero coefficients in
-// the weight gradient's product and must be finite there.
+// the weight gradient's product and must be finite there.  For the policy loss (`scal` of
+// policy_weights_kernel) rows behind the last sequence do not count, and with bad offsets none does.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 logp_mask_rows_kernel(const T* __restrict__ x, T* __restrict__ y, const int64_t* __restrict__ labels, int64_t rows,
-                      int64_t h, int64_t ld, int64_t ignore_index, int64_t vocab) {
+                      int64_t h, int64_t ld, int64_t ignore_index, int64_t vocab, const float* __restrict__ scal,
+                      const int32_t* __restrict__ cu, int n_seq) {
   grid_dependency_wait();
   constexpr int E = Cvt<T>::N;
   const int64_t nvec = h / E;
+  int64_t covered = rows;
+  if (scal != nullptr) covered = scal[1] == 0.f ? 0 : (cu != nullptr ? cu[n_seq] : rows);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const bool in = counted(labels[row], ignore_index, vocab);
+    const bool in = row < covered && counted(labels[row], ignore_index, vocab);
     for (int64_t i = threadIdx.x; i < nvec; i += kThreads)
       st_global_v4(y + row * h + i * E, in ? ld_stream_v4(x + row * ld + i * E) : make_uint4(0, 0, 0, 0));
   }
@@ -123,7 +127,8 @@ logp_mask_rows_kernel(const T* __restrict__ x, T* __restrict__ y, const int64_t*
 
 // ------------------------------------------------------------------ the policy loss
 // Weight of a counted token of each sequence (one entry for all tokens without offsets), and
-// scal[0] = largest weight, scal[1] = 1 / that: coefficients are stored relative to it.
+// scal[0] = largest weight, scal[1] = 1 / that: coefficients are stored relative to it.  Where nothing
+// counts (bad offsets among the reasons) scal[1] is 0.
 __global__ void __launch_bounds__(1024)
 policy_weights_kernel(const int64_t* __restrict__ labels, int64_t n, const int32_t* __restrict__ cu, int n_seq,
                       int64_t ignore_index, int64_t vocab, float* __restrict__ weights, float* __restrict__ scal,
@@ -165,7 +170,7 @@ policy_weights_kernel(const int64_t* __restrict__ labels, int64_t n, const int32
   if (tid == 0) {
     const double top = s_filled > 0 ? 1.0 / (static_cast<double>(s_least) * s_filled) : 1.0;
     scal[0] = static_cast<float>(top);
-    scal[1] = static_cast<float>(1.0 / top);
+    scal[1] = s_filled > 0 ? static_cast<float>(1.0 / top) : 0.f;
   }
 }
 
@@ -355,15 +360,16 @@ int stats(const Head& h, const void* hidden, const int64_t* labels, void* logits
   return gemm::launch<gemm::EPI_LOGP_SHIFT>(L, h.s);
 }
 
-int mask_rows(const Head& h, const void* x, void* y, const int64_t* labels, int64_t rows, int64_t ld) {
+int mask_rows(const Head& h, const void* x, void* y, const int64_t* labels, int64_t rows, int64_t ld,
+              const float* scal = nullptr, const int32_t* cu = nullptr, int n_seq = 0) {
   const dim3 grid(grid_for(rows, 8)), block(kThreads);
   const cudaError_t e =
       h.dtype == BT_FP32
           ? launch_dependent(logp_mask_rows_kernel<float>, grid, block, 0, h.s, static_cast<const float*>(x),
-                             static_cast<float*>(y), labels, rows, h.H, ld, h.ignore_index, h.V)
+                             static_cast<float*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq)
           // a copy: the two 16-bit types are the same
           : launch_dependent(logp_mask_rows_kernel<__half>, grid, block, 0, h.s, static_cast<const __half*>(x),
-                             static_cast<__half*>(y), labels, rows, h.H, ld, h.ignore_index, h.V);
+                             static_cast<__half*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq);
   BT_CHECK_LAUNCHED(e, "logp: copy of the counted rows");
   return BT_OK;
 }
@@ -648,7 +654,9 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
   const void* x = d->hidden;
   int64_t ld_x = d->ld_hidden;
   if (grad && d->rows > 0) {
-    if (int rc = mask_rows(h, d->hidden, d->masked, d->labels, d->rows, d->rows > 1 ? d->ld_hidden : d->H)) return rc;
+    if (int rc = mask_rows(h, d->hidden, d->masked, d->labels, d->rows, d->rows > 1 ? d->ld_hidden : d->H, scal,
+                           d->cu_seqlens, static_cast<int>(d->n_seq)))
+      return rc;
     x = d->masked;
     ld_x = d->H;
   }

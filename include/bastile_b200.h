@@ -510,7 +510,8 @@ int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int
 
 /* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
  * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
- * counts).  loss [1], averages [4] = (kl, clipped fraction, largest weight of a token, 1 / it),
+ * counts).  loss [1], averages [4] = (kl, clipped fraction, largest weight of a token, 1 / it or 0
+ * when nothing counts),
  * logp [rows].  dhidden (fp32 [runs, rows, H] with runs as from bt_dhidden_runs, may be NULL) and the weight
  * gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in
  * `logits`) are relative to averages[2]: the caller multiplies by it and the upstream gradient.
