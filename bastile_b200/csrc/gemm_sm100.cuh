@@ -106,7 +106,7 @@ struct Params {
   // Dynamic tile hand-out (pair kernel, optional): word 0 is the next-tile counter, then
   // kSchedRing published tile ids per CTA pair.  nullptr: tiles are dealt round-robin.
   unsigned long long* sched;
-  // --- plain epilogue: out = T(alpha * (acc + addend))
+  // --- plain epilogue: out = T(alpha * row_alpha[row] * (acc + addend))
   void* out;
   int64_t ldo;
   // plain epilogue, result split along N over three tensors (n_seg0 > 0): columns [0, n_seg0) go
@@ -123,6 +123,7 @@ struct Params {
   const void* addend_t;  // second addend, stored in the operand type (a residual stream)
   int64_t ld_add_t;
   const float* alpha;
+  const float* row_alpha;  // may be null
   // --- SwiGLU epilogues (row stride ld_act)
   void* gate;  // fwd: out, bwd: in
   void* up;    // fwd: out, bwd: in
@@ -277,8 +278,9 @@ template <typename T>
 __device__ __forceinline__ void epi_plain(const Params& p, uint32_t taddr, int64_t row, int n0, int run,
                                           int half, OutStage& stg, const CUtensorMap* tmO0,
                                           const CUtensorMap* tmO1, const CUtensorMap* tmO2, int lane) {
-  const float alpha = p.alpha != nullptr ? __ldg(p.alpha) : 1.0f;
   const bool row_ok = row < p.M;
+  float alpha = p.alpha != nullptr ? __ldg(p.alpha) : 1.0f;
+  if (p.row_alpha != nullptr && row_ok) alpha *= p.row_alpha[row];
   const int row0 = static_cast<int>(row) - lane;  // first row of this warp's 32
   // where this tile's columns live: one result tensor, or one of three side by side
   void* out = run == 0 ? p.out : static_cast<float*>(p.out) + run * p.split_stride;

@@ -5,6 +5,8 @@
 //   r_t = exp(logp_t - old_t)
 //   loss = sum_t w_t ( -min(r_t A_t, clip(r_t, 1 - lo, 1 + hi) A_t) + kl_coef (e^d - d - 1) ),  d = ref_t - logp_t
 //   w_t = 1 / tokens, or 1 / (sequences * tokens of t's sequence)
+#include <type_traits>
+
 #include "gemm_sm100.cuh"
 
 namespace bt {
@@ -105,6 +107,20 @@ logp_coef_kernel(const float* __restrict__ dlogp, const int64_t* __restrict__ la
     coef[i] = counted(labels[i], ignore_index, vocab) ? dlogp[i] * up : 0.f;
 }
 
+// fp16 holds dlogits = coef (onehot - softmax) between 2^-24 and 65504 only, while a coefficient may be
+// anything: ratios and KL gaps are exponentials.  A row whose coefficient lies outside [2^-8, 2^15) is
+// therefore formed from coef 2^-e, which does not; the product with W gives that row's d hidden 2^e times
+// in its fp32 epilogue, and the one with x takes the row of x times 2^(e - E), E the greatest e so far,
+// so that d weight comes out in units of 2^E.  Powers of two: rows inside the interval keep their bits.
+__device__ __forceinline__ int row_exponent(double coef) {
+  if (coef == 0.0 || !isfinite(coef)) return 0;
+  int e;
+  frexp(coef, &e);
+  e = e > 15 ? e - 15 : (e < -7 ? e + 7 : 0);
+  return max(-60, min(100, e));
+}
+constexpr int kNoExponent = -1000;  // E before the first coefficient
+
 // Rows of `x` that count, copied; zeros in the place of the others, which meet zero coefficients in
 // the weight gradient's product and must be finite there.  For the policy loss (`scal` of
 // policy_weights_kernel) rows behind the last sequence do not count, and with bad offsets none does.
@@ -132,7 +148,7 @@ logp_mask_rows_kernel(const T* __restrict__ x, T* __restrict__ y, const int64_t*
 __global__ void __launch_bounds__(1024)
 policy_weights_kernel(const int64_t* __restrict__ labels, int64_t n, const int32_t* __restrict__ cu, int n_seq,
                       int64_t ignore_index, int64_t vocab, float* __restrict__ weights, float* __restrict__ scal,
-                      int32_t* __restrict__ status) {
+                      int32_t* __restrict__ top_exp, int32_t* __restrict__ status) {
   grid_dependency_wait();
   __shared__ int s_filled, s_least;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -171,6 +187,7 @@ policy_weights_kernel(const int64_t* __restrict__ labels, int64_t n, const int32
     const double top = s_filled > 0 ? 1.0 / (static_cast<double>(s_least) * s_filled) : 1.0;
     scal[0] = static_cast<float>(top);
     scal[1] = s_filled > 0 ? static_cast<float>(1.0 / top) : 0.f;
+    top_exp[0] = kNoExponent;
   }
 }
 
@@ -187,7 +204,9 @@ struct PolicyArgs {
   float* logp;
   float* lse;
   float* coef;
-  float* terms;  // [3][total]: weighted loss, kl, clipped
+  float* row_scale;  // fp16 gradients, else null: 2^e of each row (the memory of tgt_logit)
+  int32_t* top_exp;  // E of this chunk, which starts as the one before
+  float* terms;      // [3][total]: weighted loss, kl, clipped
   int64_t rows, row0, total, ignore_index, vocab;
   int n_vt, n_seq;
   float clip_low, clip_high, kl_coef;
@@ -238,17 +257,25 @@ policy_rows_kernel(const PolicyArgs a) {
     }
     a.logp[row] = static_cast<float>(logp);
     a.lse[row] = st.x + logf(st.y);
-    a.coef[row] = static_cast<float>(coef * w * static_cast<double>(a.scal[1]));
+    coef = coef * w * static_cast<double>(a.scal[1]);
+    if (a.row_scale != nullptr) {
+      const int e = row_exponent(coef);
+      if (coef != 0.0) atomicMax(a.top_exp, e);
+      coef = ldexp(coef, -e);
+      a.row_scale[row] = ldexpf(1.f, e);
+    }
+    a.coef[row] = static_cast<float>(coef);
     a.terms[g] = static_cast<float>(term * w);
     a.terms[a.total + g] = static_cast<float>(kl * w);
     a.terms[2 * a.total + g] = held ? w : 0.f;
   }
 }
 
-// loss, averages[0..1] = sums of the three rows of terms (fp64, fixed order).
+// loss, averages[0..1] = sums of the three rows of terms (fp64, fixed order); averages[4] = the scale of
+// d weight, the largest token weight times 2^E.
 __global__ void __launch_bounds__(1024)
-policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restrict__ loss,
-                     float* __restrict__ averages) {
+policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restrict__ loss, float* __restrict__ averages,
+                     const int32_t* __restrict__ top_exp) {
   grid_dependency_wait();
   __shared__ double s_sum[32];
   const float* t = terms + blockIdx.x * n;
@@ -262,18 +289,28 @@ policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restri
     double s = 0.0;
     for (int i = 0; i < 32; ++i) s += s_sum[i];
     (blockIdx.x == 0 ? loss : averages + (blockIdx.x - 1))[0] = static_cast<float>(s);
+    if (blockIdx.x == 0)
+      averages[4] = top_exp != nullptr && *top_exp != kNoExponent ? ldexpf(averages[2], *top_exp) : averages[2];
   }
 }
 
 // Shifted logits -> coef (onehot - softmax), in place: one read and one write of the chunk, 16 bytes
 // per thread and step.  exp(logit - lse) = exp(stored) exp(half-tile max - lse), the second factor
 // once per vector.  Bound by memory: 1024 rows x 151936, 622 MB in 106 us, 5.9 TB/s; kept out of the products'
-// epilogues because a row's lse needs all of its tiles.
+// epilogues because a row's lse needs all of its tiles.  fp16: also brings the rows of x to the common
+// 2^E (rows inside the interval of row_exponent are left alone while E is 0), and hands E to the next chunk.
+struct Exponents {
+  const float* row_scale;  // null: no fp16 gradients
+  const int32_t* top;
+  int32_t* next;
+  void* x;
+  int64_t h;
+};
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 policy_dlogits_kernel(T* __restrict__ logits, const float2* __restrict__ tile_stats, const float* __restrict__ lse,
                       const int64_t* __restrict__ labels, const float* __restrict__ coef, int64_t rows, int64_t V,
-                      int64_t ld, int n_vt) {
+                      int64_t ld, int n_vt, const Exponents ex) {
   grid_dependency_wait();
   constexpr int E = Cvt<T>::N;
   const int64_t nvec = (V + E - 1) / E;
@@ -304,6 +341,41 @@ policy_dlogits_kernel(T* __restrict__ logits, const float2* __restrict__ tile_st
       }
       st_global_v4(lr + c0, Cvt<T>::pack(f));
     }
+  }
+  if constexpr (std::is_same<T, __half>::value) {
+    if (ex.row_scale == nullptr || blockIdx.y != 0) return;
+    const int top = *ex.top;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ex.next = top;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+      const float f = coef[row] != 0.f ? ldexpf(ex.row_scale[row], -top) : 1.f;
+      if (f == 1.f) continue;
+      T* xr = static_cast<T*>(ex.x) + row * ex.h;
+      for (int64_t i = threadIdx.x; i < ex.h / E; i += kThreads) {
+        float v[E];
+        Cvt<T>::unpack(ld_global_v4(xr + i * E), v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= f;
+        st_global_v4(xr + i * E, Cvt<T>::pack(v));
+      }
+    }
+  }
+}
+
+// The sum of d weight over the chunks so far, brought to the units of the newest one; nothing to do while
+// E has not grown.
+__global__ void __launch_bounds__(kThreads)
+policy_rescale_kernel(float* __restrict__ acc, int64_t n4, const int32_t* __restrict__ before,
+                      const int32_t* __restrict__ now) {
+  grid_dependency_wait();
+  const int e0 = *before, e1 = *now;
+  if (e0 == e1 || e0 == kNoExponent) return;  // (no coefficient so far: zeros)
+  const float f = ldexpf(1.f, e0 - e1);
+  float4* a = reinterpret_cast<float4*>(acc);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n4; i += step) {
+    float4 v = a[i];
+    v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+    a[i] = v;
   }
 }
 
@@ -398,7 +470,8 @@ int dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype) {
 }
 
 // parts[run][rows, H] (fp32, runs `stride` elements apart) of dlogits[rows, V] W[V, H]
-int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows, int64_t stride, int runs) {
+int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows, int64_t stride, int runs,
+                  const float* row_scale = nullptr) {
   gemm::Launch L;
   L.dtype = h.dtype;
   L.a0.ptr = dlogits, L.a0.kmajor = 1, L.a0.mn = rows, L.a0.k = h.V, L.a0.ld = h.ld_logits;
@@ -412,6 +485,7 @@ int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows
   L.p.vec_ok = rows_aligned(parts, h.H, 4) && stride % 4 == 0;
   L.p.splits = runs;
   L.p.split_stride = stride;
+  L.p.row_alpha = row_scale;
   return gemm::launch<gemm::EPI_PLAIN>(L, h.s);
 }
 
@@ -466,7 +540,7 @@ int dweight(const Head& h, const void* dlogits, const void* x, void* out, int64_
 }
 
 int policy_dlogits(const Head& h, void* logits, const float* tile_stats, const float* lse, const int64_t* labels,
-                   const float* coef, int64_t rows) {
+                   const float* coef, int64_t rows, const Exponents& ex) {
   const int64_t vec = 16 / esize(h.dtype);
   // enough CTAs for ~8 per SM: rows are split into column segments when there are few
   const int sms = sm_count();
@@ -479,13 +553,13 @@ int policy_dlogits(const Head& h, void* logits, const float* tile_stats, const f
   cudaError_t e;
   if (h.dtype == BT_BF16)
     e = launch_dependent(policy_dlogits_kernel<__nv_bfloat16>, grid, block, 0, h.s, static_cast<__nv_bfloat16*>(logits),
-                         ts, lse, labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+                         ts, lse, labels, coef, rows, h.V, h.ld_logits, h.n_vt, ex);
   else if (h.dtype == BT_FP16)
     e = launch_dependent(policy_dlogits_kernel<__half>, grid, block, 0, h.s, static_cast<__half*>(logits), ts, lse,
-                         labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+                         labels, coef, rows, h.V, h.ld_logits, h.n_vt, ex);
   else
     e = launch_dependent(policy_dlogits_kernel<float>, grid, block, 0, h.s, static_cast<float*>(logits), ts, lse,
-                         labels, coef, rows, h.V, h.ld_logits, h.n_vt);
+                         labels, coef, rows, h.V, h.ld_logits, h.n_vt, ex);
   BT_CHECK_LAUNCHED(e, "policy: dlogits");
   return BT_OK;
 }
@@ -641,6 +715,9 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
   }
   const int runs = d->rows > 0 ? dhidden_runs(d->chunk < d->rows ? d->chunk : d->rows, d->H, d->V, d->dtype) : 1;
   float* scal = d->averages + 2;
+  // E after chunk k is word k % 3: the one before it is still needed beside it, and the next is prepared
+  int32_t* top_exp = reinterpret_cast<int32_t*>(d->averages + 5);
+  const bool scaled = grad && d->dtype == BT_FP16;
   float* weights = d->ws;
   float* terms = weights + d->n_seq;
   float* lse = terms + 3 * d->rows;
@@ -649,7 +726,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
   float* tile_stats = d->ws + even(d->n_seq + 3 * d->rows + 3 * d->chunk);
   BT_CHECK_LAUNCHED(launch_dependent(policy_weights_kernel, dim3(1), dim3(1024), 0, h.s, d->labels, d->rows,
                                      d->cu_seqlens, static_cast<int>(d->n_seq), d->ignore_index, d->V, weights, scal,
-                                     status),
+                                     top_exp, status),
                     "policy_fwd: weights");
   const void* x = d->hidden;
   int64_t ld_x = d->ld_hidden;
@@ -660,7 +737,8 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     x = d->masked;
     ld_x = d->H;
   }
-  for (int64_t r = 0; r < d->rows; r += d->chunk) {
+  int k = 0;  // chunk
+  for (int64_t r = 0; r < d->rows; r += d->chunk, ++k) {
     const int64_t n = d->rows - r < d->chunk ? d->rows - r : d->chunk;
     const char* xc = row_ptr(x, r, ld_x, d->dtype);
     if (int rc = stats(h, xc, d->labels + r, grad ? d->logits : nullptr, tile_stats, tgt, n, ld_x)) return rc;
@@ -670,14 +748,22 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     a.cu = d->cu_seqlens, a.weights = weights, a.scal = scal, a.logp = d->logp + r, a.lse = lse, a.coef = coef;
     a.terms = terms, a.rows = n, a.row0 = r, a.total = d->rows, a.ignore_index = d->ignore_index, a.vocab = d->V;
     a.n_vt = h.n_vt, a.n_seq = static_cast<int>(d->n_seq);
+    a.row_scale = scaled ? tgt : nullptr, a.top_exp = top_exp + k % 3;
     a.clip_low = d->clip_low, a.clip_high = d->clip_high, a.kl_coef = d->kl_coef;
     BT_CHECK_LAUNCHED(launch_dependent(policy_rows_kernel, dim3(grid_for(ceil_div(n, kThreads / 32), 8)),
                                        dim3(kThreads), 0, h.s, a),
                       "policy_fwd: rows");
     if (!grad) continue;
-    if (int rc = policy_dlogits(h, d->logits, tile_stats, lse, d->labels + r, coef, n)) return rc;
+    const Exponents ex{a.row_scale, a.top_exp, top_exp + (k + 1) % 3, const_cast<char*>(xc), d->H};
+    if (int rc = policy_dlogits(h, d->logits, tile_stats, lse, d->labels + r, coef, n, ex)) return rc;
     if (d->dhidden != nullptr) {
-      if (int rc = dhidden_parts(h, d->logits, d->dhidden + r * d->H, n, d->rows * d->H, runs)) return rc;
+      if (int rc = dhidden_parts(h, d->logits, d->dhidden + r * d->H, n, d->rows * d->H, runs, a.row_scale)) return rc;
+    }
+    if (scaled && d->want_dweight && r > 0) {
+      const int64_t n4 = d->V * d->H / 4;
+      BT_CHECK_LAUNCHED(launch_dependent(policy_rescale_kernel, dim3(grid_for(ceil_div(n4, kThreads), 16)),
+                                         dim3(kThreads), 0, h.s, d->dweight_acc, n4, top_exp + (k + 2) % 3, a.top_exp),
+                        "policy_fwd: sum of d weight");
     }
     if (d->want_dweight && r + n < d->rows) {  // the last chunk's product waits for the upstream gradient
       if (int rc = dweight(h, d->logits, xc, d->dweight_acc, n, BT_FP32, r > 0 ? d->dweight_acc : nullptr, nullptr))
@@ -685,7 +771,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     }
   }
   BT_CHECK_LAUNCHED(launch_dependent(policy_reduce_kernel, dim3(3), dim3(1024), 0, h.s, terms, d->rows, d->loss,
-                                     d->averages),
+                                     d->averages, scaled && k > 0 ? top_exp + (k - 1) % 3 : nullptr),
                     "policy_fwd: sums");
   return BT_OK;
 }

@@ -191,7 +191,7 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
     ld = _ld_logits(vocab)
     step = _chunk_rows(chunk_size, rows, ld)
     n_chunks = -(-rows // step)
-    loss, averages, logp = _f32(dev), _f32(dev, 4), _f32(dev, rows)
+    loss, averages, logp = _f32(dev), _f32(dev, 8), _f32(dev, rows)
     ws = _f32(dev, int(lib.bt_policy_fwd_ws_floats(rows, step, n_seq, vocab)))
     logits = torch.empty((step, ld), dtype=x.dtype, device=dev) if grad else None
     masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
@@ -249,7 +249,9 @@ class LinearPolicyLossFunction(torch.autograd.Function):
                 if x_last is None:
                     dw.zero_()
                 else:
-                    # dW = alpha (dlogits^T x + the other chunks)
+                    # dW = alpha (dlogits^T x + the other chunks); fp16 has a scale of its own for it
+                    if x_dtype == torch.float16:
+                        alpha = dloss.detach().to(torch.float32) * averages[4]
                     st = _lib.status_word(dev)
                     _lib.check(lib.bt_gemm(dlogits.data_ptr(), x_last.data_ptr(), dw.data_ptr(), vocab, hdim,
                                            x_last.shape[0], dlogits.shape[1], hdim, hdim, 0, 0, code,
@@ -284,8 +286,8 @@ def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tens
     offsets as for ``pack_sequences``) the mean over sequences of their tokens' means - sequences
     without a counted token are left out, tokens behind the last sequence count as ignored.
     ``old_log_probs``, ``advantages`` and ``ref_log_probs`` have the target's shape and get no gradients.
-    Gradients of logits are formed in the hidden states' type relative to the largest token weight: with
-    fp16 those below 6e-8 of it vanish, so scale tiny advantages up (and ``loss`` down) there."""
+    Gradients of logits are formed in the hidden states' type relative to the largest token weight (with
+    fp16, rows of very large or small coefficients are formed scaled by a power of two)."""
     what = "fused_linear_policy_loss"
     for name, t in (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs)):
         if t is None and name == "ref_log_probs":

@@ -510,11 +510,12 @@ int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int
 
 /* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
  * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
- * counts).  loss [1], averages [4] = (kl, clipped fraction, largest weight of a token, 1 / it or 0
- * when nothing counts),
- * logp [rows].  dhidden (fp32 [runs, rows, H] with runs as from bt_dhidden_runs, may be NULL) and the weight
- * gradient (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in
- * `logits`) are relative to averages[2]: the caller multiplies by it and the upstream gradient.
+ * counts).  loss [1], logp [rows], averages [8] = (kl, clipped fraction, largest weight of a token, 1 / it
+ * or 0 when nothing counts, scale of the weight gradient, 3 words of scratch).  dhidden (fp32 [runs, rows, H]
+ * with runs as from bt_dhidden_runs, may be NULL) is relative to averages[2], the weight gradient
+ * (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in `logits` and whose
+ * rows of hidden in `masked`) to averages[4]: the caller multiplies by it and the upstream gradient.  The two
+ * differ with fp16 alone, where dlogits of coefficients outside [2^-8, 2^15) are stored scaled.
  * masked, logits: needed with either gradient.
  * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats. */
 typedef struct {

@@ -48,3 +48,84 @@ def test_bad_offsets_give_no_gradient_whatever_the_rows_hold():
         assert (grad == 0).all()
     with pytest.raises(_lib.BastileB200Error, match="offsets"):
         _lib.check_all_status()
+
+
+def scaled_bounds(o, coef, e_coef, top_weight, shifted):
+    """Gradients and bounds where fp16 rows are formed scaled.  A row's coefficient, relative to the largest token
+    weight, is brought into [2^-8, 2^15) by a power of two 2^-e: a step of 2^-25 below the normal range is then at
+    most 2^-17 of the coefficient.  Its row of x is multiplied by 2^(e - E): off by 2^-25 in those units."""
+    u = 2.0 ** -11
+    coef, e_coef = (torch.where(o.live, c, 0.0)[:, None] for c in (coef, e_coef))
+    rel = coef[:, 0].abs() / top_weight
+    ex = torch.frexp(rel)[1].double()
+    e = torch.where(ex > 15, ex - 15, torch.where(ex < -7, ex + 7, 0.0))
+    e = torch.where(rel > 0, e, -1000.0)
+    top = e.max()
+    p = (o.z - o.lse[:, None]).exp()
+    dl = -coef * p
+    dl.scatter_add_(1, o.col, coef)
+    e_p = p * (2 * o.e[:, None] + 2.0 ** -19)
+    if shifted:
+        n, v = o.z.shape
+        zz = torch.nn.functional.pad(o.z, (0, -v % 128), value=-torch.inf).view(n, -1, 128)
+        e_p = e_p + p * u * (zz - zz.amax(-1, keepdim=True)).view(n, -1)[:, :v].abs()
+    e_dl = coef.abs() * (e_p + 2.0 ** -17) + e_coef * (dl.abs() / coef.abs().clamp(min=1e-300)) + u * dl.abs()
+    sums = 2.0 ** -19  # fp32 sums
+    dx = (dl @ o.w, 1.01 * (e_dl @ o.w.abs() + sums * (dl.abs() @ o.w.abs()) + u * (dl @ o.w).abs()) + 2.0 ** -24)
+    e_x = torch.where(rel > 0, 2.0 ** -25 * 2.0 ** (top - e).clamp(max=200), 0.0)[:, None].expand_as(o.x)
+    dw = (dl.t() @ o.x, 1.01 * (e_dl.t() @ (o.x.abs() + e_x) + dl.abs().t() @ e_x + sums * (dl.abs().t() @ o.x.abs())))
+    return dx, dw
+
+
+@pytest.mark.parametrize("chunk", [4096, 40])
+@pytest.mark.parametrize("what", ["ratios", "kl", "tiny", "mixed"])
+def test_fp16_coefficients_of_any_size(what, chunk):
+    """Ratios and KL gaps are exponentials: coefficients beyond 65504 (and far below 2^-24) with gradients that are
+    ordinary numbers once they are multiplied with a token's weight."""
+    from bastile_b200 import _lib
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    x, w, t, _, g = make(90, 64, 700, torch.float16, seed=23)
+    w32 = w.float()
+    o = Oracle(x, w, t)
+    old, adv, ref = policy_inputs(o, g)
+    kl = 0.0
+    if what == "ratios":
+        adv[71], adv[3], old[71], old[3] = -1.0, -0.5, o.logp[71] - 13.0, o.logp[3] - 12.0
+    elif what == "kl":
+        kl, ref[75], ref[2] = 0.05, o.logp[75] + 15.0, o.logp[2] + 14.0
+    elif what == "tiny":
+        adv *= 1e-7
+    else:
+        adv[::2] *= 1e-6
+        adv[79], old[79] = -1.0, o.logp[79] - 13.0
+    up = 1.0 if what != "tiny" else 1e7
+    want, *_ = policy_oracle(o, old, adv, ref if kl else None, 0.2, 0.28, kl, None)
+    assert (want["coef"].abs().max() * o.live.sum() > 65504) == (what != "tiny")
+    dx, dw = scaled_bounds(o, up * want["coef"], up * want["e_coef"], float(up / o.live.sum()), shifted=True)
+    x.requires_grad_(True), w32.requires_grad_(True)
+    got = fused_linear_policy_loss(x, w32, t, old, adv, ref if kl else None, 0.2, 0.28, kl, chunk_size=chunk)
+    for _ in range(2):
+        a, b = torch.autograd.grad(got.loss * up, (x, w32), retain_graph=True)
+        close(a, *dx, "dhidden")
+        close(b, *dw, "dweight")
+    _lib.check_all_status()
+
+
+def test_fp16_ordinary_coefficients_are_left_alone():
+    """The same tokens beside one with a huge coefficient and without it: their rows have the same bits."""
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    x, w, t, _, g = make(60, 64, 700, torch.float16, seed=24)
+    o = Oracle(x, w, t)
+    old, adv, _ = policy_inputs(o, g)
+    x.requires_grad_(True)
+
+    def rows():
+        return torch.autograd.grad(fused_linear_policy_loss(x, w, t, old, adv).loss, x)[0]
+
+    want = rows()
+    adv[8], old[8] = -1.0, o.logp[8] - 14.0
+    got = rows()
+    keep = torch.arange(60, device=DEV) != 8
+    assert torch.equal(got[keep], want[keep]) and torch.isfinite(got[8]).all() and (got[8] != 0).any()
