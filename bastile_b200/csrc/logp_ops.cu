@@ -77,36 +77,6 @@ logp_rows_kernel(const float2* __restrict__ tile_stats, const float* __restrict_
   }
 }
 
-// Upstream gradient of the log-probabilities as the coefficients of the dlogits product, scaled by a
-// power of two so that the largest is in [1/2, 1): with fp16 operands a mean over many tokens would
-// otherwise push them, times the softmax, below the type's range.  scal[0] = scale back.
-__global__ void __launch_bounds__(1024)
-logp_coef_kernel(const float* __restrict__ dlogp, const int64_t* __restrict__ labels, int64_t n, int64_t ignore_index,
-                 int64_t vocab, float* __restrict__ coef, float* __restrict__ scal) {
-  grid_dependency_wait();
-  __shared__ float s_max[32];
-  float mx = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (counted(labels[i], ignore_index, vocab)) {
-      const float a = fabsf(dlogp[i]);
-      if (a <= 3.0e38f) mx = fmaxf(mx, a);  // infinities and NaN keep their place, but set no scale
-    }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
-  __syncthreads();
-  mx = s_max[threadIdx.x & 31];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  int e = 0;
-  if (mx > 0.f) frexpf(mx, &e);
-  e = max(-125, min(125, e));
-  const float up = ldexpf(1.f, -e);
-  if (threadIdx.x == 0) scal[0] = ldexpf(1.f, e);
-  for (int64_t i = threadIdx.x; i < n; i += 1024)
-    coef[i] = counted(labels[i], ignore_index, vocab) ? dlogp[i] * up : 0.f;
-}
-
 // fp16 holds dlogits = coef (onehot - softmax) between 2^-24 and 65504 only, while a coefficient may be
 // anything: ratios and KL gaps are exponentials.  A row whose coefficient lies outside [2^-8, 2^15) is
 // therefore formed from coef 2^-e, which does not; the product with W gives that row's d hidden 2^e times
@@ -121,14 +91,53 @@ __device__ __forceinline__ int row_exponent(double coef) {
 }
 constexpr int kNoExponent = -1000;  // E before the first coefficient
 
+// Upstream gradient of the log-probabilities as the coefficients of the dlogits product, scaled by a
+// power of two so that the largest is in [1/2, 1): with fp16 operands a mean over many tokens would
+// otherwise push them, times the softmax, below the type's range.  scal[0] = scale back.  row_scale (fp16,
+// else null): 2^e of each row, at most 1 here.
+__global__ void __launch_bounds__(1024)
+logp_coef_kernel(const float* __restrict__ dlogp, const int64_t* __restrict__ labels, int64_t n, int64_t ignore_index,
+                 int64_t vocab, float* __restrict__ coef, float* __restrict__ row_scale, float* __restrict__ scal) {
+  grid_dependency_wait();
+  __shared__ float s_max[32];
+  float mx = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+    if (counted(labels[i], ignore_index, vocab)) {
+      const float a = fabsf(dlogp[i]);
+      if (isfinite(a)) mx = fmaxf(mx, a);  // infinities and NaN keep their place, but set no scale
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  mx = s_max[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  int e = 0;
+  if (mx > 0.f) frexpf(mx, &e);
+  e = max(-125, min(125, e));
+  const float up = ldexpf(1.f, -e);
+  if (threadIdx.x == 0) scal[0] = ldexpf(1.f, e);
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    float c = counted(labels[i], ignore_index, vocab) ? dlogp[i] * up : 0.f;
+    if (row_scale != nullptr) {
+      const int e = row_exponent(c);
+      c = ldexpf(c, -e);
+      row_scale[i] = ldexpf(1.f, e);
+    }
+    coef[i] = c;
+  }
+}
+
 // Rows of `x` that count, copied; zeros in the place of the others, which meet zero coefficients in
 // the weight gradient's product and must be finite there.  For the policy loss (`scal` of
-// policy_weights_kernel) rows behind the last sequence do not count, and with bad offsets none does.
+// policy_weights_kernel) rows behind the last sequence do not count, and with bad offsets none does.  For the
+// log-probabilities (`row_scale`, or null) rows are multiplied by 2^e: E is 0, all coefficients being known.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 logp_mask_rows_kernel(const T* __restrict__ x, T* __restrict__ y, const int64_t* __restrict__ labels, int64_t rows,
                       int64_t h, int64_t ld, int64_t ignore_index, int64_t vocab, const float* __restrict__ scal,
-                      const int32_t* __restrict__ cu, int n_seq) {
+                      const int32_t* __restrict__ cu, int n_seq, const float* __restrict__ row_scale) {
   grid_dependency_wait();
   constexpr int E = Cvt<T>::N;
   const int64_t nvec = h / E;
@@ -136,8 +145,18 @@ logp_mask_rows_kernel(const T* __restrict__ x, T* __restrict__ y, const int64_t*
   if (scal != nullptr) covered = scal[1] == 0.f ? 0 : (cu != nullptr ? cu[n_seq] : rows);
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const bool in = row < covered && counted(labels[row], ignore_index, vocab);
-    for (int64_t i = threadIdx.x; i < nvec; i += kThreads)
-      st_global_v4(y + row * h + i * E, in ? ld_stream_v4(x + row * ld + i * E) : make_uint4(0, 0, 0, 0));
+    const float f = in && row_scale != nullptr ? row_scale[row] : 1.f;
+    for (int64_t i = threadIdx.x; i < nvec; i += kThreads) {
+      uint4 u = in ? ld_stream_v4(x + row * ld + i * E) : make_uint4(0, 0, 0, 0);
+      if (f != 1.f) {
+        float v[E];
+        Cvt<T>::unpack(u, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= f;
+        u = Cvt<T>::pack(v);
+      }
+      st_global_v4(y + row * h + i * E, u);
+    }
   }
 }
 
@@ -433,15 +452,17 @@ int stats(const Head& h, const void* hidden, const int64_t* labels, void* logits
 }
 
 int mask_rows(const Head& h, const void* x, void* y, const int64_t* labels, int64_t rows, int64_t ld,
-              const float* scal = nullptr, const int32_t* cu = nullptr, int n_seq = 0) {
+              const float* scal, const int32_t* cu, int n_seq, const float* row_scale) {
   const dim3 grid(grid_for(rows, 8)), block(kThreads);
   const cudaError_t e =
       h.dtype == BT_FP32
           ? launch_dependent(logp_mask_rows_kernel<float>, grid, block, 0, h.s, static_cast<const float*>(x),
-                             static_cast<float*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq)
-          // a copy: the two 16-bit types are the same
+                             static_cast<float*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq,
+                             row_scale)
+          // a copy, but for fp16's scales: the two 16-bit types are the same
           : launch_dependent(logp_mask_rows_kernel<__half>, grid, block, 0, h.s, static_cast<const __half*>(x),
-                             static_cast<__half*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq);
+                             static_cast<__half*>(y), labels, rows, h.H, ld, h.ignore_index, h.V, scal, cu, n_seq,
+                             row_scale);
   BT_CHECK_LAUNCHED(e, "logp: copy of the counted rows");
   return BT_OK;
 }
@@ -471,7 +492,7 @@ int dhidden_runs(int64_t rows, int64_t H, int64_t V, int dtype) {
 
 // parts[run][rows, H] (fp32, runs `stride` elements apart) of dlogits[rows, V] W[V, H]
 int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows, int64_t stride, int runs,
-                  const float* row_scale = nullptr) {
+                  const float* row_scale) {
   gemm::Launch L;
   L.dtype = h.dtype;
   L.a0.ptr = dlogits, L.a0.kmajor = 1, L.a0.mn = rows, L.a0.k = h.V, L.a0.ld = h.ld_logits;
@@ -641,16 +662,19 @@ extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W
                "logp_bwd: more than one chunk needs an accumulator for the weight gradient");
   if (chunk > rows) chunk = rows;
   const int runs = dhidden_runs(chunk, H, V, dtype);
-  float* scal = ws;  // [1 + rows]: scale back, coefficients
+  float* scal = ws;  // [1 + 2 rows]: scale back, coefficients, fp16's scales of the rows
   float* coef = ws + 1;
+  float* row_scale = dtype == BT_FP16 ? coef + rows : nullptr;
   BT_CHECK_LAUNCHED(launch_dependent(logp_coef_kernel, dim3(1), dim3(1024), 0, h.s, dlogp, labels, rows, ignore_index,
-                                     V, coef, scal),
+                                     V, coef, row_scale, scal),
                     "logp_bwd: coefficients");
-  if (int rc = mask_rows(h, hidden, masked, labels, rows, rows > 1 ? ld_hidden : H)) return rc;
+  const int64_t ld = rows > 1 ? ld_hidden : H;
+  if (int rc = mask_rows(h, hidden, masked, labels, rows, ld, nullptr, nullptr, 0, row_scale)) return rc;
   for (int64_t r = 0; r < rows; r += chunk) {
     const int64_t n = rows - r < chunk ? rows - r : chunk;
     const char* x = row_ptr(masked, r, H, dtype);
-    gemm::Launch L = head_product(h, x, labels + r, n, H);
+    // (logits of ignored rows, which may be anything, are never used; `masked` is for the weight's product)
+    gemm::Launch L = head_product(h, row_ptr(hidden, r, ld, dtype), labels + r, n, ld);
     L.p.row_lse = lse + r;
     L.p.row_coef = coef + r;
     L.p.out = dlogits;
@@ -658,7 +682,9 @@ extern "C" int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W
     L.p.vec_ok = rows_aligned(dlogits, h.ld_logits, esize(dtype));
     if (int rc = gemm::launch<gemm::EPI_DLOGITS>(L, h.s)) return rc;
     if (dhidden != nullptr) {
-      if (int rc = dhidden_parts(h, dlogits, dhidden_parts_, n, chunk * H, runs)) return rc;
+      if (int rc = dhidden_parts(h, dlogits, dhidden_parts_, n, chunk * H, runs,
+                                 row_scale != nullptr ? row_scale + r : nullptr))
+        return rc;
       if (int rc = sum_runs(dhidden_parts_, const_cast<char*>(row_ptr(dhidden, r, H, dtype)), n * H, runs, chunk * H,
                             scal, dtype, h.s))
         return rc;
@@ -732,7 +758,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
   int64_t ld_x = d->ld_hidden;
   if (grad && d->rows > 0) {
     if (int rc = mask_rows(h, d->hidden, d->masked, d->labels, d->rows, d->rows > 1 ? d->ld_hidden : d->H, scal,
-                           d->cu_seqlens, static_cast<int>(d->n_seq)))
+                           d->cu_seqlens, static_cast<int>(d->n_seq), nullptr))
       return rc;
     x = d->masked;
     ld_x = d->H;

@@ -165,7 +165,7 @@ class LinearLogProbsFunction(torch.autograd.Function):
         code = _lib.dtype_code(x.dtype)
         parts = _f32(dev, _runs(dev, step, hdim, vocab, code), step, hdim) if need_x else None
         acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
-        ws = _f32(dev, rows + 1)
+        ws = _f32(dev, 2 * rows + 1)
         st = _lib.status_word(dev)
         with _lib.device_of(dev), _lib.timed("logp_bwd", 2 + n_chunks * (1 + 2 * int(need_x) + int(need_w)), dev):
             rc = lib.bt_logp_bwd(g.data_ptr(), x.data_ptr(), w.data_ptr(), labels.data_ptr(), lse.data_ptr(),

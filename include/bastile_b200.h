@@ -502,7 +502,7 @@ int bt_sum_runs(const float* parts, void* out, int64_t n, int64_t runs, int64_t 
                 void* stream);
 /* Gradients for the upstream gradient dlogp[rows]; logits are recomputed.  dhidden [rows, H] in `dtype`
  * (with dhidden_parts [runs, min(chunk, rows), H] fp32) and dweight [V, H] in dweight_dtype may each be
- * NULL; dweight_acc [V, H] fp32 is needed for dweight when rows > chunk; ws: rows + 1 floats. */
+ * NULL; dweight_acc [V, H] fp32 is needed for dweight when rows > chunk; ws: 2 rows + 1 floats. */
 int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int64_t* labels, const float* lse,
                 void* masked, void* dlogits, void* dhidden, float* dhidden_parts, void* dweight, float* dweight_acc,
                 float* ws, int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk,

@@ -129,3 +129,23 @@ def test_fp16_ordinary_coefficients_are_left_alone():
     got = rows()
     keep = torch.arange(60, device=DEV) != 8
     assert torch.equal(got[keep], want[keep]) and torch.isfinite(got[8]).all() and (got[8] != 0).any()
+
+
+@pytest.mark.parametrize("chunk", [4096, 40])
+def test_fp16_upstream_gradients_of_different_sizes(chunk):
+    """Token weights six orders of magnitude apart: a small one's row of d hidden has its own digits."""
+    from bastile_b200 import _lib
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_log_probs
+
+    x, w, t, up, _ = make(90, 64, 700, torch.float16, seed=25)
+    w32 = w.float().requires_grad_(True)
+    o = Oracle(x, w, t)
+    size = 10.0 ** -(torch.arange(90, device=DEV) % 7)
+    up = up * size * 64.0
+    x.requires_grad_(True)
+    top = 2.0 ** float(torch.frexp((up * o.live).abs().max())[1])  # relative to this the largest is in [1/2, 1)
+    dx, dw = scaled_bounds(o, up.double(), torch.zeros_like(o.e), top, shifted=False)
+    a, b = torch.autograd.grad(fused_linear_log_probs(x, w32, t, chunk_size=chunk), (x, w32), up)
+    close(a, *dx, "dhidden")
+    close(b, *dw, "dweight")
+    _lib.check_all_status()
