@@ -46,7 +46,7 @@ class PolicyDesc(ctypes.Structure):
                                         "loss", "averages", "dhidden", "dweight_acc", "masked", "logits", "ws")]
     _fields_ += [(n, c_int64) for n in ("rows", "H", "V", "ld_hidden", "chunk", "n_seq", "ignore_index")]
     _fields_ += [(n, c_float) for n in ("clip_low", "clip_high", "kl_coef")]
-    _fields_ += [("want_dweight", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+    _fields_ += [("want_dweight", ctypes.c_int32), ("dtype", ctypes.c_int32), ("dhidden_parts", c_void_p)]
 
 
 I64x3 = c_int64 * 3

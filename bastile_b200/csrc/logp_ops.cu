@@ -510,13 +510,13 @@ int dhidden_parts(const Head& h, const void* dlogits, float* parts, int64_t rows
   return gemm::launch<gemm::EPI_PLAIN>(L, h.s);
 }
 
-// out = T(alpha * sum over runs), in the runs' order; four elements per thread and step.
+// out = T(alpha * sum over runs), in the runs' order; four elements per thread and step.  alpha: null is 1.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 sum_runs_kernel(const float* __restrict__ parts, T* __restrict__ out, int64_t n4, int runs, int64_t stride4,
                 const float* __restrict__ alpha) {
   grid_dependency_wait();
-  const float a = __ldg(alpha);
+  const float a = alpha != nullptr ? __ldg(alpha) : 1.f;
   const float4* in = reinterpret_cast<const float4*>(parts);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n4; i += step) {
@@ -740,6 +740,10 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
                  "policy_fwd: more than one chunk needs an accumulator for the weight gradient");
   }
   const int runs = d->rows > 0 ? dhidden_runs(d->chunk < d->rows ? d->chunk : d->rows, d->H, d->V, d->dtype) : 1;
+  // one chunk: its runs are added up when the upstream gradient is known; more: each before the next
+  const bool sum_now = d->rows > d->chunk && runs > 1;
+  BT_CHECK_ARG(d->dhidden == nullptr || !sum_now || (d->dhidden_parts != nullptr && aligned16(d->dhidden_parts)),
+               "policy_fwd: more than one chunk needs a 16-byte aligned buffer for the parts of the gradient of hidden");
   float* scal = d->averages + 2;
   // E after chunk k is word k % 3: the one before it is still needed beside it, and the next is prepared
   int32_t* top_exp = reinterpret_cast<int32_t*>(d->averages + 5);
@@ -783,7 +787,13 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     const Exponents ex{a.row_scale, a.top_exp, top_exp + (k + 1) % 3, const_cast<char*>(xc), d->H};
     if (int rc = policy_dlogits(h, d->logits, tile_stats, lse, d->labels + r, coef, n, ex)) return rc;
     if (d->dhidden != nullptr) {
-      if (int rc = dhidden_parts(h, d->logits, d->dhidden + r * d->H, n, d->rows * d->H, runs, a.row_scale)) return rc;
+      float* sum = d->dhidden + r * d->H;
+      if (int rc = dhidden_parts(h, d->logits, sum_now ? d->dhidden_parts : sum, n,
+                                 (sum_now ? d->chunk : d->rows) * d->H, runs, a.row_scale))
+        return rc;
+      if (sum_now) {
+        if (int rc = sum_runs(d->dhidden_parts, sum, n * d->H, runs, d->chunk * d->H, nullptr, BT_FP32, h.s)) return rc;
+      }
     }
     if (scaled && d->want_dweight && r > 0) {
       const int64_t n4 = d->V * d->H / 4;

@@ -196,16 +196,20 @@ def _policy(hidden, weight, target, old, adv, ref, cu, clip_low, clip_high, kl_c
     logits = torch.empty((step, ld), dtype=x.dtype, device=dev) if grad else None
     masked = torch.empty((rows, hdim), dtype=x.dtype, device=dev) if grad else None
     code = _lib.dtype_code(x.dtype)
-    # fp32 until the upstream gradient is known: one rounding to the hidden states' type
-    dx = _f32(dev, _runs(dev, step, hdim, vocab, code), rows, hdim) if need_x else None
+    # fp32 until the upstream gradient is known: one rounding to the hidden states' type.  The runs of a single
+    # chunk are added up then; those of several at once, so that only the sums are kept.
+    runs = _runs(dev, step, hdim, vocab, code) if need_x else 1
+    dx = _f32(dev, runs if n_chunks <= 1 else 1, rows, hdim) if need_x else None
+    parts = _f32(dev, runs, step, hdim) if n_chunks > 1 and runs > 1 else None
     acc = _f32(dev, vocab, hdim) if need_w and n_chunks > 1 else None
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     d = _lib.PolicyDesc(ptr(x), ptr(w), ptr(labels), ptr(old), ptr(adv), ptr(ref), ptr(cu), ptr(logp), ptr(loss),
                         ptr(averages), ptr(dx), ptr(acc), ptr(masked), ptr(logits), ptr(ws), rows, hdim, vocab, _ld(x),
-                        step, n_seq, ignore_index, clip_low, clip_high, kl_coef, int(need_w), code)
+                        step, n_seq, ignore_index, clip_low, clip_high, kl_coef, int(need_w), code, ptr(parts))
     st = _lib.status_word(dev)
     with _lib.device_of(dev), _lib.timed("policy_fwd", 2 + int(grad) + n_chunks *
-                                         (2 + int(grad) + int(need_x) + int(need_w)) - int(need_w), dev):
+                                         (2 + int(grad) + int(need_x) + int(need_w) + int(parts is not None)) -
+                                         int(need_w), dev):
         rc = lib.bt_policy_fwd(ctypes.byref(d), st.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "bt_policy_fwd")
     last = masked[(n_chunks - 1) * step:] if need_w and n_chunks else None

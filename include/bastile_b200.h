@@ -511,8 +511,9 @@ int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int
 /* One policy-loss call.  cu_seqlens NULL and n_seq 1: the mean over counted tokens; else the mean over the
  * n_seq sequences of their tokens' means (offsets are checked as in bt_attn_plan; with bad ones nothing
  * counts).  loss [1], logp [rows], averages [8] = (kl, clipped fraction, largest weight of a token, 1 / it
- * or 0 when nothing counts, scale of the weight gradient, 3 words of scratch).  dhidden (fp32 [runs, rows, H]
- * with runs as from bt_dhidden_runs, may be NULL) is relative to averages[2], the weight gradient
+ * or 0 when nothing counts, scale of the weight gradient, 3 words of scratch).  dhidden (fp32, may
+ * be NULL) is [runs, rows, H] with runs as from bt_dhidden_runs when rows <= chunk; otherwise [rows, H], the sums,
+ * with dhidden_parts [runs, chunk, H] as scratch unless runs is 1.  It is relative to averages[2], the weight gradient
  * (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in `logits` and whose
  * rows of hidden in `masked`) to averages[4]: the caller multiplies by it and the upstream gradient.  The two
  * differ with fp16 alone, where dlogits of coefficients outside [2^-8, 2^15) are stored scaled.
@@ -538,6 +539,7 @@ typedef struct {
   float clip_low, clip_high, kl_coef;
   int32_t want_dweight;
   int32_t dtype;
+  float* dhidden_parts;
 } bt_policy_desc;
 int64_t bt_policy_fwd_ws_floats(int64_t rows, int64_t chunk, int64_t n_seq, int64_t V);
 int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* stream);

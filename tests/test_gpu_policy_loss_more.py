@@ -149,3 +149,24 @@ def test_fp16_upstream_gradients_of_different_sizes(chunk):
     close(a, *dx, "dhidden")
     close(b, *dw, "dweight")
     _lib.check_all_status()
+
+
+@pytest.mark.parametrize("need_w", [False, True])
+def test_a_smaller_chunk_keeps_no_more_memory(need_w):
+    """What a loss keeps until its backward: fp32 d hidden once, whatever its product is cut into."""
+    from bastile_b200 import _lib
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    rows, h, v, chunk = 2000, 256, 9001, 64
+    assert _lib.get_lib().bt_dhidden_runs(chunk, h, v, _lib.BT_BF16) > 4
+    x, w, t, _, g = make(rows, h, v, torch.bfloat16, seed=26)
+    zero, one = torch.zeros(rows, device=DEV), torch.ones(rows, device=DEV)
+    x.requires_grad_(True), w.requires_grad_(need_w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    got = fused_linear_policy_loss(x, w, t, zero, one, chunk_size=chunk)
+    kept = torch.cuda.memory_allocated() - before
+    ld = (v + 7) // 8 * 8
+    most = 4 * rows * h + (4 * v * h + 2 * rows * h + 2 * chunk * ld if need_w else 0) + 4 * rows
+    assert kept <= most + (1 << 20), (kept, most)
+    del got
