@@ -20,12 +20,20 @@ MAX_HEAD_DIM = 128
 
 class PackedSequences:
     """The layout of one packed batch (made by ``pack_sequences``): usable by any number of
-    attention calls, forward and backward, on work ordered behind its creation."""
+    attention calls, forward and backward, on any stream on work ordered behind its creation; it may be
+    dropped as soon as the calls have been made."""
 
-    __slots__ = ("plan", "batch", "total_tokens", "device")
+    __slots__ = ("plan", "batch", "total_tokens", "device", "stream")
 
     def __init__(self, plan: Tensor, batch: int, total_tokens: int):
         self.plan, self.batch, self.total_tokens, self.device = plan, batch, total_tokens, plan.device
+        self.stream = _lib.stream_ptr(plan.device) if plan.is_cuda else None
+
+    def keep_for(self, dev: torch.device) -> None:
+        """The plan's memory belongs to the stream that made it: not given to its next user before the work
+        that other streams have queued is done (kernels take addresses from it)."""
+        if _lib.stream_ptr(dev) != self.stream:
+            self.plan.record_stream(torch.cuda.current_stream(dev))
 
 
 def pack_sequences(cu_seqlens: Tensor, total_tokens: int) -> PackedSequences:
@@ -80,6 +88,7 @@ def _forward(q, k, v, sequences, scale, keep: bool):
     lo = torch.empty_like(out) if keep else None  # what rounding cut off: dout . out is formed from both
     if t > 0:
         st = _lib.status_word(dev)
+        sequences.keep_for(dev)  # (the backward runs on this stream too)
         with _lib.device_of(dev), _lib.timed("attn_fwd", 1, dev):
             rc = lib.bt_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                  lo.data_ptr() if keep else None, lse2.data_ptr() if keep else None,
