@@ -105,6 +105,7 @@ SIGNATURES = {
     "bt_attn_plan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "bt_attn_fwd": (c_int, [c_void_p] * 7 + [c_int64] * 5 + [POINTER(c_int64)] * 4 +
                     [c_float, c_int, c_void_p, c_void_p]),
+    "bt_attn_delta_floats": (c_int64, [c_int64, c_int64, c_int]),
     "bt_attn_bwd": (c_int, [c_void_p] * 12 + [c_int64] * 5 + [POINTER(c_int64)] * 8 +
                     [c_float, c_int, c_void_p, c_void_p]),
     "bt_logp_fwd_ws_floats": (c_int64, [c_int64] * 2),

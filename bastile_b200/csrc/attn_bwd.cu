@@ -26,28 +26,52 @@ constexpr int kBwdThreads = 384;
 // off by dO . (that), which is as much in dQ and dK as the rounding of dS (2-norm of the error of dQ at
 // bf16: 2.7e-3 instead of 2.4e-3; 1.7e-3 is the rounding of the result).
 template <typename T>
+constexpr bool kScaled = std::is_same<T, __half>::value;
+
+// What fp16 wants to know of V and the sequences besides.
+template <typename T>
+struct BoundArgs {
+  const T* v;
+  int64_t v_st, v_sh;
+  int hk;
+  const int32_t* covered;  // tokens of sequences
+  float2* out;             // one per block
+};
+
+template <typename T>
+__device__ __forceinline__ float greatest(const float (&x)[8], float m) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fabsf(x[e]) <= 65504.f ? fmaxf(m, fabsf(x[e])) : m;
+  return m;
+}
+
+template <typename T>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ out_lo, const T* __restrict__ dout,
                   float* __restrict__ delta, int64_t rows, int heads, int64_t total, int d, int64_t o_st, int64_t o_sh,
-                  int64_t g_st, int64_t g_sh) {
+                  int64_t g_st, int64_t g_sh, const BoundArgs<T> bound) {
   grid_dependency_wait();
   constexpr int kRows = 4;
+  const int covered = kScaled<T> ? __ldg(bound.covered) : 0;
+  float max_g = 0.f, max_v = 0.f;
   const int sub = threadIdx.x & 15;
   const bool live = sub * 8 < d;
   const bool small = rows <= 0xffffffffll;  // a 64-bit division costs more than the row's arithmetic
   const int64_t step = static_cast<int64_t>(gridDim.x) * 16 * kRows;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16 * kRows; r0 < rows; r0 += step) {
     uint4 a[kRows], b[kRows], c[kRows];
-    int64_t at[kRows];
+    int64_t at[kRows], tok_of[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
       a[i] = b[i] = c[i] = make_uint4(0, 0, 0, 0);
       at[i] = -1;
+      tok_of[i] = 0;
       if (r < rows) {
         const int64_t tok = small ? static_cast<uint32_t>(r) / static_cast<uint32_t>(heads) : r / heads;
         const int64_t head = r - tok * heads;
         at[i] = head * total + tok;
+        tok_of[i] = tok;
         if (live) {
           a[i] = ld_stream_v4(out + tok * o_st + head * o_sh + sub * 8);
           if (out_lo != nullptr) c[i] = ld_stream_v4(out_lo + tok * o_st + head * o_sh + sub * 8);
@@ -63,11 +87,72 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ out_lo, const
       Cvt<T>::unpack(c[i], z);
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc = fmaf(x[e] + z[e], y[e], acc);
+      if (kScaled<T> && tok_of[i] < covered) max_g = greatest<T>(y, max_g);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
       if (at[i] >= 0 && sub == 0) delta[at[i]] = acc;
     }
   }
+  if constexpr (kScaled<T>) {
+    const int64_t v_rows = static_cast<int64_t>(covered) * bound.hk;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 16 * kRows; r0 < v_rows; r0 += step) {
+      uint4 a[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
+        a[i] = make_uint4(0, 0, 0, 0);
+        if (r < v_rows && live) {
+          const int64_t tok = small ? static_cast<uint32_t>(r) / static_cast<uint32_t>(bound.hk) : r / bound.hk;
+          a[i] = ld_global_v4(bound.v + tok * bound.v_st + (r - tok * bound.hk) * bound.v_sh + sub * 8);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        float x[8];
+        Cvt<T>::unpack(a[i], x);
+        max_v = greatest<T>(x, max_v);
+      }
+    }
+    __shared__ float2 s_max[8];
+    // (bits of non-negative floats are ordered as integers)
+    const float g = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(max_g)));
+    const float v = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(max_v)));
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = make_float2(g, v);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float2 m = s_max[0];
+      for (int i = 1; i < 8; ++i) m.x = fmaxf(m.x, s_max[i].x), m.y = fmaxf(m.y, s_max[i].y);
+      bound.out[blockIdx.x] = m;
+    }
+  }
+}
+
+// 2^k of dS, the same in every CTA; `place` has room for a float2 per warp.
+template <typename T>
+__device__ __forceinline__ float ds_scale(const Params& p, float2* place) {
+  if constexpr (!kScaled<T>) {
+    return 1.f;
+  } else {
+    float2 m = make_float2(0.f, 0.f);
+    for (int i = threadIdx.x; i < p.n_bounds; i += kBwdThreads) {
+      const float2 b = __ldg(p.bounds + i);
+      m.x = fmaxf(m.x, b.x), m.y = fmaxf(m.y, b.y);
+    }
+    m.x = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(m.x)));
+    m.y = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(m.y)));
+    if ((threadIdx.x & 31) == 0) place[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int i = 0; i < kBwdThreads / 32; ++i) m.x = fmaxf(m.x, place[i].x), m.y = fmaxf(m.y, place[i].y);
+    const float most = 2.f * p.d * m.x * m.y;
+    int e;
+    frexpf(most, &e);
+    return most > 0.f ? ldexpf(1.f, min(15 - e, 60)) : 1.f;
+  }
+}
+// 2^k (dP - D), D scaled before
+template <typename T>
+__device__ __forceinline__ f32x2 minus_d(f32x2 dp, f32x2 scale, f32x2 minus_scaled_d) {
+  return kScaled<T> ? fma2(dp, scale, minus_scaled_d) : add2(dp, minus_scaled_d);
 }
 
 template <int DT>
@@ -162,6 +247,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
+  const float up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
+  const float dk_scale = p.scale / up;
+
   const bool shared_tiles = PAIR && p.plan.area() < p.share * static_cast<float>(p.plan.longest());
   const int unit = static_cast<int>(shared_tiles ? blockIdx.x / 2 : blockIdx.x);
   const int hk = unit % p.hk;
@@ -212,7 +300,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + token;
           const bool in = r < valid;
           vec[st * 256 + r] = in ? -__ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
-          vec[st * 256 + 128 + r] = in ? -__ldg(p.delta + at) : 0.f;
+          vec[st * 256 + 128 + r] = in ? -__ldg(p.delta + at) * up : 0.f;
         }
         ptx::mbar_arrive(&vec_full[st]);
         ok = ring_load<DT>(sG + st * TB, &tmG, head, it.start + tok0, valid, &g_full[st], &g_empty[st], par, fix,
@@ -312,7 +400,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     if (n > 0) {
       const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t ts = tmem + lane_base + half * 64, tp = ts + 128;
-      const f32x2 c2 = pair(p.scale_log2, p.scale_log2);
+      const f32x2 c2 = pair(p.scale_log2, p.scale_log2), up2 = pair(up, up);
       bool ok = true;
       int i = i0 + x0 % per;
       for (int x = 0; x < n; ++x) {
@@ -366,8 +454,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           for (int e = 0; e < 8; ++e) {
             const float4 d4 = dl[g * 8 + e];
             const int b = g * 32 + 4 * e;
-            const f32x2 u = mul2(pair(s[b], s[b + 1]), add2(pair(dp[b], dp[b + 1]), pair(d4.x, d4.y)));
-            const f32x2 v = mul2(pair(s[b + 2], s[b + 3]), add2(pair(dp[b + 2], dp[b + 3]), pair(d4.z, d4.w)));
+            const f32x2 u = mul2(pair(s[b], s[b + 1]), minus_d<T>(pair(dp[b], dp[b + 1]), up2, pair(d4.x, d4.y)));
+            const f32x2 v =
+                mul2(pair(s[b + 2], s[b + 3]), minus_d<T>(pair(dp[b + 2], dp[b + 3]), up2, pair(d4.z, d4.w)));
             pk[2 * e] = pack2<T>(lo_of(u), hi_of(u));
             pk[2 * e + 1] = pack2<T>(lo_of(v), hi_of(v));
           }
@@ -404,7 +493,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (ok)
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
-            store_sum_cols<T>(mine + c, sQ + (c / 4 * 128 + row) * 16, dst, c, p.d, rank != 0 ? p.scale : 1.0f,
+            store_sum_cols<T>(mine + c, sQ + (c / 4 * 128 + row) * 16, dst, c, p.d, rank != 0 ? dk_scale : 1.0f,
                               row_ok);
       } else if (ok) {
         T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
@@ -413,7 +502,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll 1
         for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
           store_cols<T>(tmem + lane_base + 256 + c, dv, nullptr, c, p.d, 1.0f, row_ok);
-          store_cols<T>(tmem + lane_base + 256 + DT + c, dk, nullptr, c, p.d, p.scale, row_ok);
+          store_cols<T>(tmem + lane_base + 256 + DT + c, dk, nullptr, c, p.d, dk_scale, row_ok);
         }
       }
     }
@@ -493,6 +582,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   ptx::tcgen05_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
+
+  const float up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
+  const float dq_scale = p.scale / up;
 
   const int groups = p.hk * p.nsub;
   const int hs = static_cast<int>(blockIdx.x) % groups;
@@ -611,8 +703,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const uint32_t ts0 = tmem + lane_base + half * 64, tp = ts0 + 256;
       const int64_t at = static_cast<int64_t>(head) * p.total + token;
       const float nl = row_ok ? -p.lse2[at] : -INFINITY;
-      const float dl = row_ok ? -p.delta[at] : 0.f;
-      const f32x2 c2 = pair(p.scale_log2, p.scale_log2), nl2 = pair(nl, nl), dl2 = pair(dl, dl);
+      const float dl = row_ok ? -p.delta[at] * up : 0.f;
+      const f32x2 c2 = pair(p.scale_log2, p.scale_log2), nl2 = pair(nl, nl), dl2 = pair(dl, dl),
+                  up2 = pair(up, up);
       const int lim = min(tok, it.len - 1);
       const int safe = min(first, it.len - 1);
       bool ok = true;
@@ -643,7 +736,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (lane == 0) ptx::mbar_arrive(dp_free);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const f32x2 u = mul2(pair(s[2 * e], s[2 * e + 1]), add2(pair(dp[2 * e], dp[2 * e + 1]), dl2));
+          const f32x2 u = mul2(pair(s[2 * e], s[2 * e + 1]), minus_d<T>(pair(dp[2 * e], dp[2 * e + 1]), up2, dl2));
           s[2 * e] = lo_of(u);
           s[2 * e + 1] = hi_of(u);
         }
@@ -671,13 +764,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (first + p.tq <= it.len) {  // into Q's place
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
-            stage_cols<T>(ta + c, sQ, 0, row, c, p.scale);
+            stage_cols<T>(ta + c, sQ, 0, row, c, dq_scale);
           store_tile<DT>(warp == 0 && lane == 0, staged, sQ, &tmD, 0, &tmD, hs * p.gp, it.start + first, lane,
                          cta_abort, p.status);
         } else {
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
-            store_cols<T>(ta + c, dq, nullptr, c, p.d, p.scale, row_ok);
+            store_cols<T>(ta + c, dq, nullptr, c, p.d, dq_scale, row_ok);
         }
       }
     }
@@ -734,14 +827,23 @@ int run_bwd(const Maps& m, Params p, int64_t batch, cudaStream_t s) {
 }
 
 template <typename T>
-int run_delta(const void* out, const void* out_lo, const void* dout, float* delta, int64_t total, int64_t hq, int64_t d,
-              const int64_t* os, const int64_t* gs, cudaStream_t s) {
+int run_delta(const void* out, const void* out_lo, const void* dout, const void* v, Params* p, int64_t total, int64_t hq,
+              int64_t d, const int64_t* os, const int64_t* gs, const int64_t* vs, cudaStream_t s) {
   const int64_t rows = total * hq;
-  const int64_t want = ceil_div(rows, 64), cap = static_cast<int64_t>(sm_count()) * 8;
-  BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(static_cast<unsigned>(want < cap ? want : cap)),
+  const int64_t want = ceil_div(rows, 64), sms = static_cast<int64_t>(sm_count()) * 8;
+  const int64_t cap = sms < kMaxBounds ? sms : kMaxBounds;
+  const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
+  float* delta = p->delta;
+  BoundArgs<T> bound{static_cast<const T*>(v), vs[0], vs[1], p->hk, p->plan.words + p->plan.n - 1, nullptr};
+  if (kScaled<T>) {  // behind D
+    bound.out = reinterpret_cast<float2*>(delta + (rows + 1) / 2 * 2);
+    p->bounds = bound.out;
+    p->n_bounds = static_cast<int>(grid);
+  }
+  BT_CHECK_LAUNCHED(launch_dependent(attn_delta_kernel<T>, dim3(grid),
                                      dim3(256), 0, s, static_cast<const T*>(out), static_cast<const T*>(out_lo),
                                      static_cast<const T*>(dout), delta, rows, static_cast<int>(hq), total,
-                                     static_cast<int>(d), os[0], os[1], gs[0], gs[1]),
+                                     static_cast<int>(d), os[0], os[1], gs[0], gs[1], bound),
                     "attn_bwd delta");
   return BT_OK;
 }
@@ -752,6 +854,11 @@ int run_delta(const void* out, const void* out_lo, const void* dout, float* delt
 
 int bt_internal_set_wait_limit_attn_bwd(unsigned long long ns) {
   return bt::ptx::set_wait_limit_ns(ns) == cudaSuccess ? 0 : -1;
+}
+
+extern "C" int64_t bt_attn_delta_floats(int64_t total, int64_t hq, int dtype) {
+  if (total < 0 || hq < 0) return 0;
+  return dtype == BT_FP16 ? (total * hq + 1) / 2 * 2 + 2 * bt::attn::kMaxBounds : total * hq;
 }
 
 extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -768,6 +875,7 @@ extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const
   const int nq = static_cast<int>(hq), nk = static_cast<int>(hk), nd = static_cast<int>(d);
   BT_CHECK_ARG(lse2 != nullptr && delta != nullptr, "attn_bwd: null pointer");
   BT_CHECK_ARG(aligned16(out_lo), "attn_bwd out_lo: must be 16-byte aligned");
+  BT_CHECK_ARG(reinterpret_cast<uintptr_t>(delta) % 8 == 0, "attn_bwd delta: must be 8-byte aligned");
   BT_CHECK_ARG((dk == nullptr) == (dv == nullptr), "attn_bwd: dk and dv are computed together");
   if (int rc = check_view("attn_bwd dout", dout, g_strides[0], g_strides[1], nq, total)) return rc;
   if (int rc = check_view("attn_bwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
@@ -801,9 +909,10 @@ extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const
   if (int rc = rows(&m.dq, dq, dq_strides, true, "attn_bwd dq")) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BT_BF16) {
-    if (int rc = run_delta<__nv_bfloat16>(out, out_lo, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+    if (int rc = run_delta<__nv_bfloat16>(out, out_lo, dout, v, &p, total, hq, d, o_strides, g_strides, v_strides, s))
+      return rc;
     return d <= 64 ? run_bwd<__nv_bfloat16, 64>(m, p, batch, s) : run_bwd<__nv_bfloat16, 128>(m, p, batch, s);
   }
-  if (int rc = run_delta<__half>(out, out_lo, dout, delta, total, hq, d, o_strides, g_strides, s)) return rc;
+  if (int rc = run_delta<__half>(out, out_lo, dout, v, &p, total, hq, d, o_strides, g_strides, v_strides, s)) return rc;
   return d <= 64 ? run_bwd<__half, 64>(m, p, batch, s) : run_bwd<__half, 128>(m, p, batch, s);
 }

@@ -395,6 +395,13 @@ struct View {
   int64_t st, sh;  // element strides of a token and of a head
 };
 
+// fp16 has 40 powers of two for dS = P (dP - D): upstream gradients of 1e-4 and probabilities of a long row
+// leave few of them above its last step.  dS is formed times 2^k such that the greatest value that it can
+// have, 2 head_dim max|dO| max|V|, stays below 2^15; dQ and dK are scaled back in fp32.  The D kernel, which
+// reads dO anyway, leaves one (max|dO|, max|V|) per block; infinities, NaN and rows behind the last sequence
+// have no say.
+constexpr int kMaxBounds = 2048;  // blocks of the D kernel
+
 struct Params {
   Plan plan;
   int hq, hk, d, total;
@@ -406,6 +413,8 @@ struct Params {
   float* delta;  // [hq][total] dot(dO, O)
   View o, dq, dk, dv;
   void* o_lo;  // laid out as o
+  const float2* bounds;  // fp16 backward: [n_bounds] (max|dO|, max|V|)
+  int n_bounds;
   int32_t* status;
 };
 

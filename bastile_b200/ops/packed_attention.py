@@ -121,7 +121,8 @@ class PackedAttentionFunction(torch.autograd.Function):
         dk = torch.empty((t, hk, d), dtype=q.dtype, device=dev) if need_kv else None
         dv = torch.empty((t, hk, d), dtype=q.dtype, device=dev) if need_kv else None
         if q.numel() > 0:
-            delta = torch.empty((hq, t), dtype=torch.float32, device=dev)
+            code = _lib.dtype_code(q.dtype)
+            delta = torch.empty(int(lib.bt_attn_delta_floats(t, hq, code)), dtype=torch.float32, device=dev)
             st = _lib.status_word(dev)
             none = _lib.I64x2(0, 0)
             with _lib.device_of(dev), _lib.timed("attn_bwd", 1 + int(need_q) + int(need_kv), dev):
@@ -131,7 +132,7 @@ class PackedAttentionFunction(torch.autograd.Function):
                                      plan.data_ptr(), batch, t, hq, hk, d, _strides(dout), _strides(q), _strides(k),
                                      _strides(v), _strides(out), _strides(dq) if need_q else none,
                                      _strides(dk) if need_kv else none, _strides(dv) if need_kv else none, scale,
-                                     _lib.dtype_code(q.dtype), st.data_ptr(), _lib.stream_ptr(dev))
+                                     code, st.data_ptr(), _lib.stream_ptr(dev))
             _lib.check(rc, "bt_attn_bwd")
         return dq, dk, dv, None, None
 

@@ -471,8 +471,9 @@ int bt_attn_fwd(const void* q, const void* k, const void* v, void* out, void* ou
 
 /* Gradients of bt_attn_fwd for the upstream gradient `dout` (bt_attn_fwd's out, out_lo - may
  * be NULL, with the gradients then a little less exact - and lse2 come back in).
- * dq may be NULL, and so may dk and dv together; `delta` is [hq, total] fp32 scratch.  Rows behind the
- * last sequence get zeros.  No atomics: the same inputs give the same bits. */
+ * dq may be NULL, and so may dk and dv together; `delta` is bt_attn_delta_floats(total, hq, dtype) fp32
+ * values of scratch.  Rows behind the last sequence get zeros.  No atomics: the same inputs give the same bits. */
+int64_t bt_attn_delta_floats(int64_t total, int64_t hq, int dtype);
 int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* out_lo,
                 const float* lse2, float* delta, void* dq, void* dk, void* dv, const int32_t* plan, int64_t batch,
                 int64_t total, int64_t hq, int64_t hk, int64_t d, const int64_t* g_strides,

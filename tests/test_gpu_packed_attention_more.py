@@ -32,3 +32,60 @@ def test_a_dropped_plan_outlives_the_calls_on_another_stream():
         for n, x in zip(("out", "dq", "dk", "dv"), got):
             assert torch.equal(x, want[n]), n
         del reuse
+
+
+def off(got, x):
+    return float((got.double() - x).norm() / x.norm())
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 2e-7])
+@pytest.mark.parametrize("big", ["q", "k"])
+def test_fp16_small_upstream_gradients_keep_their_digits(big, size):
+    """Long rows (probabilities of 1 / 4000) and small upstream gradients: dS lies below fp16's normal range.
+    dS and the result are rounded once each, by at most u / sqrt(3) in the mean square; what a result loses in
+    its own subnormal steps comes on top.  (q or k are large so that dk or dq are not themselves subnormal.)"""
+    n, d, factor = 4000, 64, 64.0
+    q, k, v, cu, dout = inputs([n], 2, 1, d, torch.float16, seed=32, tail=7)
+    q, k = (q * factor, k) if big == "q" else (q, k * factor)
+    v, dout = v * (256.0 if size < 1e-5 else 8.0), (dout * size).half()
+    dout[n:] = 3e4  # rows behind the last sequence have no say in the scale
+    v[n:] = 6e4
+    scale = d ** -0.5 / factor
+    want = oracle(q, k, v, cu, scale, dout)
+    got = attend(q, k, v, cu, dout, scale=scale)
+    name = "dk" if big == "q" else "dq"
+    x = want[name][0]
+    own = 2.0 ** -24 / 12 ** 0.5 / float(x[:n].square().mean().sqrt())
+    bar = 1.25 * (2 * (2.0 ** -11) ** 2 / 3 + own ** 2) ** 0.5
+    assert off(got[name], x) <= bar, (off(got[name], x), bar, own)
+
+
+def test_fp16_large_upstream_gradients():
+    """dP far beyond 65504 times a small probability: dS once overflowed where the probability is not small."""
+    q, k, v, cu, dout = inputs([300], 2, 1, 64, torch.float16, seed=33)
+    v, dout = v * 64.0, dout * 512.0
+    scale = 2.0 ** -12
+    want = oracle(q, k, v, cu, scale, dout)
+    got = attend(q, k, v, cu, dout, scale=scale)
+    for n in ("dq", "dk"):
+        bar = 1.25 * (2 * (2.0 ** -11) ** 2 / 3) ** 0.5
+        assert torch.isfinite(got[n]).all() and off(got[n], want[n][0]) <= bar, n
+
+
+def test_fp16_infinite_upstream_gradients_stay_where_they_are():
+    q, k, v, cu, dout = inputs([100, 90], 2, 1, 64, torch.float16, seed=34)
+    want = attend(q, k, v, cu, dout)
+    dout[120] = float("inf")
+    got = attend(q, k, v, cu, dout)
+    for n in ("dq", "dk", "dv"):
+        assert torch.equal(got[n][:100], want[n][:100]), n
+        assert not torch.isfinite(got[n][100:]).all(), n
+
+
+def test_fp16_gradients_scale_with_the_upstream_gradient():
+    """A power of two on the upstream gradient: the same bits, scaled, while the results stay normal numbers."""
+    q, k, v, cu, dout = inputs([130, 70], 4, 2, 64, torch.float16, seed=35)
+    a, b = attend(q, k, v, cu, dout * 8.0), attend(q, k, v, cu, dout)
+    for n in ("dq", "dk"):
+        big = b[n].abs() >= 2.0 ** -14
+        assert torch.equal(a[n][big], (b[n] * 8.0)[big]), n
