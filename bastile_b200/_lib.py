@@ -335,6 +335,7 @@ class timed:
 
 
 STATUS_WAIT_MASK, STATUS_BAD_LABEL, STATUS_BAD_SEQUENCES = 0x0F, 0x10, 0x20  # BT_STATUS_* of include/bastile_b200.h
+STATUS_IMPLIED_SEQUENCES = 0x40  # set by the transformers path, not by a kernel; results are valid
 
 
 def _describe_status(v: int) -> str:
@@ -347,6 +348,9 @@ def _describe_status(v: int) -> str:
     if v & STATUS_BAD_SEQUENCES:
         parts.append("sequence offsets do not start at 0, fall, or run past the packed tokens (or a padding "
                      "mask has holes, or position ids restart inside a sequence)")
+    if v & STATUS_IMPLIED_SEQUENCES:
+        parts.append("position ids alone told the sequences of a packed row: they were kept apart, but finding them "
+                     "waits for the device in every forward (pass cu_seq_lens_q)")
     return "; ".join(parts) or f"status {v:#x}"
 
 

@@ -8,6 +8,8 @@ what the kernels need, on the device and without a host synchronisation.
 
 from __future__ import annotations
 
+import inspect
+
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
@@ -189,16 +191,49 @@ def _padded_offsets(mask: Tensor) -> Tensor:
     return torch.nn.functional.pad(cu, (0, 1), value=b * t).to(torch.int32)
 
 
-def _report(bad: Tensor) -> None:
-    """Set BT_STATUS_BAD_SEQUENCES in the stream's status word where ``bad`` - without waiting for it."""
-    _lib.status_word(bad.device).bitwise_or_(bad.to(torch.int32) * _lib.STATUS_BAD_SEQUENCES)
+def _report(bad: Tensor, what: int = _lib.STATUS_BAD_SEQUENCES) -> None:
+    """Set ``what`` in the stream's status word where ``bad`` - without waiting for it."""
+    _lib.status_word(bad.device).bitwise_or_(bad.to(torch.int32) * what)
 
 
-def hf_packed_mask(batch_size, q_length, kv_length, *args, attention_mask=None, **kwargs):
-    """The mask that transformers prepares once per forward: nothing, or for a padded batch its offsets."""
+def _mask_leaves(function) -> list:
+    """The mask functions of which transformers put ``function`` together by intersection."""
+    if getattr(function, "__qualname__", "").startswith("and_masks.<locals>"):
+        parts = inspect.getclosurevars(function).nonlocals.get("mask_functions", ())
+        return [leaf for part in parts for leaf in _mask_leaves(part)]
+    return [function]
+
+
+def _packed_offsets(same_sequence, b: int, t: int, device) -> Tensor:
+    """Offsets of the sequences of a [B, T] batch: a row begins one, and so does a token that ``same_sequence``
+    keeps apart from the one before it.  Their number is read from the device, as transformers itself does to
+    find out that there are several."""
+    rows, at = torch.arange(b, device=device)[:, None], torch.arange(1, t, device=device)[None]
+    first = torch.ones(b, t, dtype=torch.bool, device=device)
+    if t > 1:
+        first[:, 1:] = ~same_sequence(rows, 0, at, at - 1)
+    cu = torch.nn.functional.pad(first.reshape(-1).nonzero()[:, 0], (0, 1), value=b * t).to(torch.int32)
+    cu.implied = True
+    return cu
+
+
+def hf_packed_mask(batch_size, q_length, kv_length, *args, attention_mask=None, mask_function=None, device=None,
+                   **kwargs):
+    """The mask that transformers prepares once per forward: nothing, or the offsets of a padded batch or of
+    rows whose position ids start several sequences (``mask_function`` then keeps these apart).  Any other
+    mask function - bidirectional, windows, chunks, overlays - is refused."""
+    from transformers import masking_utils
+
+    packed = None
+    for leaf in [] if mask_function is None else _mask_leaves(mask_function):
+        if getattr(leaf, "__qualname__", "").startswith("packed_sequence_mask_function.<locals>"):
+            packed = leaf
+        elif leaf is not masking_utils.causal_mask_function:
+            raise ValueError(f"{HF_NAME}: full causal attention only, got the mask function "
+                             f"{getattr(leaf, '__qualname__', leaf)}")
     if attention_mask is None:
-        return None
-    if attention_mask.dim() != 2 or attention_mask.shape[1] != q_length or kv_length != q_length:
+        return None if packed is None else _packed_offsets(packed, batch_size, q_length, device)
+    if packed is not None or attention_mask.dim() != 2 or attention_mask.shape[1] != q_length or kv_length != q_length:
         raise ValueError(f"{HF_NAME}: takes [batch, tokens] padding masks and no cached tokens, got a mask of "
                          f"{tuple(attention_mask.shape)} for {q_length} queries and {kv_length} keys")
     return _padded_offsets(attention_mask)
@@ -209,8 +244,10 @@ def hf_packed_attention(module, query, key, value, attention_mask, dropout: floa
     """``packed_attention`` with the signature of ``ALL_ATTENTION_FUNCTIONS``: query [B, Hq, T, D], key and
     value [B, Hk, T, D] -> ([B, T, Hq, D], None).  A packed row (B = 1) brings its offsets as
     ``cu_seq_lens_q`` (transformers' ``DataCollatorWithFlattening(return_flash_attn_kwargs=True)``);
-    otherwise each batch row is a sequence, or what its padding mask leaves of it.  Position ids that
-    restart inside a sequence are reported through the status word."""
+    otherwise each batch row is a sequence, or what its padding mask leaves of it, or the sequences that its
+    position ids start.  The last are kept apart and reported through the status word, since finding them
+    waits for the device.  transformers looks for them only in a forward without a cache; with one it takes a
+    row as one sequence, which is reported too where position ids restart."""
     b, hq, t, d = query.shape
     if dropout:
         raise ValueError(f"{HF_NAME}: attention dropout is not supported")
@@ -223,7 +260,12 @@ def hf_packed_attention(module, query, key, value, attention_mask, dropout: floa
             raise ValueError(f"{HF_NAME}: cu_seq_lens_q describes one packed row, got a batch of {b}")
         cu = cu_seq_lens_q
     elif attention_mask is not None:
+        if attention_mask.dim() != 1:
+            raise ValueError(f"{HF_NAME}: takes the mask that hf_packed_mask prepares, got one of "
+                             f"{tuple(attention_mask.shape)}")
         cu = attention_mask
+        if getattr(cu, "implied", False) and getattr(module, "layer_idx", 0) == 0:
+            _report(torch.ones((), dtype=torch.bool, device=cu.device), _lib.STATUS_IMPLIED_SEQUENCES)
     else:
         cu = torch.arange(0, (b + 1) * t, max(t, 1), dtype=torch.int32, device=query.device)[:b + 1]
         if position_ids is not None and t > 1 and getattr(module, "layer_idx", 0) == 0:

@@ -42,6 +42,7 @@ extern "C" {
 #define BT_STATUS_WAIT_MASK 0x0f
 #define BT_STATUS_BAD_LABEL 0x10
 #define BT_STATUS_BAD_SEQUENCES 0x20
+/* 0x40 is used by the Python package */
 
 /* Library version (major*10000 + minor*100 + patch). No reference counterpart
  * (the reference is a JIT Python package: src/bastile/__init__.py:23). */
