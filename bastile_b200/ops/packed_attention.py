@@ -251,8 +251,12 @@ def hf_packed_attention(module, query, key, value, attention_mask, dropout: floa
     b, hq, t, d = query.shape
     if dropout:
         raise ValueError(f"{HF_NAME}: attention dropout is not supported")
-    if sliding_window is not None or kwargs.get("softcap") is not None or is_causal is False:
+    if is_causal is None:
+        is_causal = getattr(module, "is_causal", True)
+    if sliding_window is not None or kwargs.get("softcap") is not None or not is_causal:
         raise ValueError(f"{HF_NAME}: full causal attention only")
+    if kwargs.get("s_aux") is not None:
+        raise ValueError(f"{HF_NAME}: attention sinks are not supported")
     if key.shape[2] != t:
         raise ValueError(f"{HF_NAME}: {t} queries against {key.shape[2]} keys: a cache is not supported, use 'sdpa'")
     if cu_seq_lens_q is not None:

@@ -57,3 +57,17 @@ def test_other_masks_are_refused():
                dict(and_mask_function=overlay)):
         with pytest.raises(ValueError, match="full causal"):
             _mask(1, 8, torch.arange(8)[None], config=cfg, **kw)
+
+
+def test_what_the_attention_refuses():
+    from bastile_b200.ops.packed_attention import hf_packed_attention
+
+    q, k = torch.zeros(1, 4, 8, 64), torch.zeros(1, 2, 8, 64)
+    encoder = torch.nn.Module()
+    encoder.is_causal = False
+    for module, mask, kw, text in ((encoder, None, {}, "full causal"), (None, None, dict(is_causal=False), "full causal"),
+                                   (None, None, dict(s_aux=torch.zeros(4)), "sinks"),
+                                   (None, torch.zeros(1, 1, 8, 8), {}, "hf_packed_mask"),
+                                   (None, torch.ones(1, 8), {}, "hf_packed_mask")):
+        with pytest.raises(ValueError, match=text):
+            hf_packed_attention(module, q, k, k, mask, **kw)
