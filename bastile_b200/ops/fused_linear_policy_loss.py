@@ -65,7 +65,7 @@ def _rows_of(x: Tensor) -> Tensor:
     if x2.stride(-1) != 1 or x2.data_ptr() % 16 != 0 or (x2.shape[0] > 1 and
                                                          (x2.stride(0) % vec != 0 or x2.stride(0) < x2.shape[1])):
         x2 = x2.contiguous()
-    return x2
+    return x2 if x2.data_ptr() % 16 == 0 else x2.clone()  # (dense rows may lie off a 16-byte boundary)
 
 
 def _head_weight(weight: Tensor, dtype) -> Tensor:

@@ -76,7 +76,8 @@ def _rows(t: Tensor) -> Tensor:
     if sd == 1 and (n <= 1 or (st > 0 and st % 8 == 0)) and (heads <= 1 or (sh > 0 and sh % 8 == 0)) \
             and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous()
+    c = t.contiguous()
+    return c if c.data_ptr() % 16 == 0 else c.clone()  # (dense rows off a 16-byte boundary are returned as they are)
 
 
 def _forward(q, k, v, sequences, scale, keep: bool):

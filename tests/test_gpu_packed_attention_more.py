@@ -89,3 +89,20 @@ def test_fp16_gradients_scale_with_the_upstream_gradient():
     for n in ("dq", "dk"):
         big = b[n].abs() >= 2.0 ** -14
         assert torch.equal(a[n][big], (b[n] * 8.0)[big]), n
+
+
+def shifted(x, by=1):
+    """The same values, dense, ``by`` elements off an aligned start."""
+    buf = torch.empty(x.numel() + 8, dtype=x.dtype, device=x.device)
+    y = buf[by:by + x.numel()].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16 != 0
+    return y
+
+
+def test_dense_tensors_off_a_16_byte_boundary():
+    q, k, v, cu, dout = inputs([70, 130], 4, 2, 64, torch.bfloat16, seed=36)
+    want = attend(q, k, v, cu, dout)
+    got = attend(shifted(q), shifted(k, 3), shifted(v, 4), cu, shifted(dout, 7))
+    for n in got:
+        assert torch.equal(got[n], want[n]), n

@@ -170,3 +170,30 @@ def test_a_smaller_chunk_keeps_no_more_memory(need_w):
     most = 4 * rows * h + (4 * v * h + 2 * rows * h + 2 * chunk * ld if need_w else 0) + 4 * rows
     assert kept <= most + (1 << 20), (kept, most)
     del got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_dense_tensors_off_a_16_byte_boundary(dtype):
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_log_probs, fused_linear_policy_loss
+
+    def shifted(a):
+        buf = torch.empty(a.numel() + 8, dtype=a.dtype, device=DEV)
+        y = buf[1:1 + a.numel()].view(a.shape)
+        y.copy_(a)
+        assert y.data_ptr() % 16 != 0
+        return y
+
+    x, w, t, up, g = make(40, 64, 300, dtype, seed=27)
+    o = Oracle(x, w, t)
+    old, adv, ref = policy_inputs(o, g)
+
+    def both(move):
+        a, b, *rest = (move(i) for i in (x, w, t, up, old, adv, ref))
+        a.requires_grad_(True), b.requires_grad_(True)
+        tt, u, ol, ad, rf = rest
+        lp = fused_linear_log_probs(a, b, tt)
+        pl = fused_linear_policy_loss(a, b, tt, ol, ad, rf, kl_coef=0.1)
+        return (lp.detach(), pl.loss.detach(), *torch.autograd.grad(lp, (a, b), u), *torch.autograd.grad(pl.loss, (a, b)))
+
+    for a, b in zip(both(shifted), both(lambda i: i.clone())):
+        assert torch.equal(a, b)
