@@ -270,8 +270,10 @@ policy_rows_kernel(const PolicyArgs a) {
       if (a.ref_logp != nullptr) {
         const double d = static_cast<double>(a.ref_logp[g]) - logp, em1 = expm1(d);
         kl = em1 - d;
-        term += a.kl_coef * kl;
-        coef -= a.kl_coef * em1;
+        if (a.kl_coef != 0.f) {  // 0 is for the log alone: its infinity is not the loss's
+          term += a.kl_coef * kl;
+          coef -= a.kl_coef * em1;
+        }
       }
     }
     a.logp[row] = static_cast<float>(logp);

@@ -197,3 +197,19 @@ def test_dense_tensors_off_a_16_byte_boundary(dtype):
 
     for a, b in zip(both(shifted), both(lambda i: i.clone())):
         assert torch.equal(a, b)
+
+
+def test_a_reference_for_the_log_alone_does_not_reach_the_loss():
+    """kl_coef = 0: a gap whose exponential is infinite shows in the average, not in loss or gradients."""
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    x, w, t, _, g = make(30, 64, 200, torch.bfloat16, seed=28)
+    o = Oracle(x, w, t)
+    old, adv, ref = policy_inputs(o, g)
+    ref[5] = 900.0
+    x.requires_grad_(True), w.requires_grad_(True)
+    a = fused_linear_policy_loss(x, w, t, old, adv)
+    b = fused_linear_policy_loss(x, w, t, old, adv, ref)
+    assert b.kl == float("inf") and torch.equal(a.loss, b.loss)
+    for p, q in zip(torch.autograd.grad(a.loss, (x, w)), torch.autograd.grad(b.loss, (x, w))):
+        assert torch.equal(p, q)
