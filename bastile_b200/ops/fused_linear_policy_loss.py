@@ -29,6 +29,8 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from .fused_linear_cross_entropy import _GEMM_DTYPES, AUTO_CHUNK_BYTES, AUTO_CHUNK_ROWS, DEFAULT_CHUNK
 
+_F32_MAX = torch.finfo(torch.float32).max
+
 
 class PolicyLoss(NamedTuple):
     """``loss`` is differentiable; the others are for the log: ``log_probs`` (fp32, the target's shape, 0
@@ -302,8 +304,8 @@ def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tens
     clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
         raise ValueError(f"{what}: need 0 <= clip_low <= 1 and clip_high >= 0, got {clip_low} and {clip_high}")
-    if kl_coef != kl_coef or abs(kl_coef) == float("inf"):
-        raise ValueError(f"{what}: kl_coef must be finite, got {kl_coef}")
+    if not abs(kl_coef) <= _F32_MAX:
+        raise ValueError(f"{what}: kl_coef must be finite in fp32, got {kl_coef}")
     if kl_coef != 0.0 and ref_log_probs is None:
         raise ValueError(f"{what}: kl_coef = {kl_coef} needs ref_log_probs")
     if cu_seqlens is not None:
