@@ -142,8 +142,8 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
       : "memory");
 }
 // A wait of a whole warp: all lanes leave with the same answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int32_t* status,
-                                          int code) {
+static __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                                 int32_t* status, int code) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, cta_abort, status, code));
 }
 // 32 columns of this thread's lane; the registers are valid after tmem_wait_ld().
@@ -254,9 +254,10 @@ __host__ __device__ constexpr uint32_t mma_fmt() {
 // One tile through the ring slot `dst`: rows from `valid` on are cleared before the consumers see it.
 // Called by the whole load warp; returns false when a wait ran out.
 template <int DT>
-__device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, int head, int token, int valid,
-                                          uint64_t* full, uint64_t* empty, uint32_t empty_parity, uint64_t* fix,
-                                          uint32_t* fix_phase, int lane, volatile int* cta_abort, int32_t* status) {
+static __device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap* tm, int head, int token, int valid,
+                                                 uint64_t* full, uint64_t* empty, uint32_t empty_parity, uint64_t* fix,
+                                                 uint32_t* fix_phase, int lane, volatile int* cta_abort,
+                                                 int32_t* status) {
   bool ok = true;
   const bool ragged = valid < kTile;
   if (lane == 0) {
@@ -372,9 +373,9 @@ __device__ __forceinline__ void store_sum_cols(uint32_t taddr, uint32_t place, T
 // After a warp has staged its part: say so, and (the one thread) wait for all and store the tile, and the
 // second one unless lo_tile is 0.
 template <int DT>
-__device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32_t tile, const CUtensorMap* tm,
-                                           uint32_t lo_tile, const CUtensorMap* lo_tm, int head, int token, int lane,
-                                           volatile int* cta_abort, int32_t* status) {
+static __device__ __forceinline__ void store_tile(bool issuer, uint64_t* staged, uint32_t tile, const CUtensorMap* tm,
+                                                  uint32_t lo_tile, const CUtensorMap* lo_tm, int head, int token,
+                                                  int lane, volatile int* cta_abort, int32_t* status) {
   ptx::fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) ptx::mbar_arrive(staged);

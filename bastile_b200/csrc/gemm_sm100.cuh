@@ -696,7 +696,7 @@ __device__ __forceinline__ ASource a_source(const Params& p, const CUtensorMap* 
 
 // --------------------------------------------------------------------- kernel
 template <int EPI, typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+static __global__ void __launch_bounds__(kThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
             const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
             const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmO0,
@@ -929,7 +929,6 @@ constexpr int kSchedRing = 16;
 constexpr int kSchedMaxPairs = 256;
 constexpr int kSchedWords = 1 + kSchedMaxPairs * kSchedRing;
 constexpr int kSchedSlots = 32;
-static __device__ unsigned long long g_tile_sched[kSchedSlots][kSchedWords];
 
 __device__ __forceinline__ int sched_draw(const Params& p) {
   const unsigned int t = atomicAdd(reinterpret_cast<unsigned int*>(p.sched), 1u);
@@ -942,8 +941,8 @@ __device__ __forceinline__ void sched_publish(const Params& p, int pair, int i, 
   asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(slot), "l"(v) : "memory");
 }
 // The i-th tile of this pair (-1: no more tiles, or the wait was given up).
-__device__ __forceinline__ int sched_wait(const Params& p, int pair, int npairs, int i,
-                                          volatile int* cta_abort, int status_bit) {
+static __device__ __forceinline__ int sched_wait(const Params& p, int pair, int npairs, int i,
+                                                 volatile int* cta_abort, int status_bit) {
   if (p.sched == nullptr) {
     const int t = pair + i * npairs;
     return t < p.num_tiles ? t : -1;
@@ -966,7 +965,7 @@ __device__ __forceinline__ int sched_wait(const Params& p, int pair, int npairs,
 }
 
 template <int EPI, typename T>
-__global__ void __launch_bounds__(kThreadsPair, 1)
+static __global__ void __launch_bounds__(kThreadsPair, 1)
 gemm_kernel_pair(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
                  const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
                  const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmO0,
@@ -1342,7 +1341,7 @@ inline int encode_tmap(CUtensorMap* tm, const Operand& o, int dtype, const char*
 }
 
 template <int EPI, typename T>
-int launch_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+static int launch_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
              const CUtensorMap& b1, const CUtensorMap& a2, const CUtensorMap (&o)[3], const Params& p,
              cudaStream_t s) {
   static std::atomic<uint64_t> reserved{0};
@@ -1380,20 +1379,9 @@ inline int& dynamic_tiles() {
   return mode;
 }
 
-// Device address of the scheduler pool on the current device (looked up once per device).
-inline unsigned long long* sched_pool() {
-  static std::mutex mu;
-  static unsigned long long* pools[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-  std::lock_guard<std::mutex> lock(mu);
-  if (pools[dev] == nullptr) {
-    void* ptr = nullptr;
-    if (cudaGetSymbolAddress(&ptr, g_tile_sched) != cudaSuccess) return nullptr;
-    pools[dev] = static_cast<unsigned long long*>(ptr);
-  }
-  return pools[dev];
-}
+// Device address of the scheduler pool on the current device (looked up once per device); the pool itself
+// is in tc_ops.cu, for every translation unit that launches products.  Kernels get it as an argument.
+unsigned long long* sched_pool();
 
 // Slot of the scheduler pool owned by (current device, stream): handed out first come, first
 // served, kept for the life of the process; -1 when all kSchedSlots are taken on this device.
@@ -1412,7 +1400,7 @@ inline int sched_slot_of(cudaStream_t s) {
 }
 
 template <int EPI, typename T>
-int launch_pair_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+static int launch_pair_t(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
                   const CUtensorMap& b1, const CUtensorMap& a2, const CUtensorMap (&o)[3],
                   const Params& p, cudaStream_t s) {
   static std::atomic<uint64_t> reserved{0};
@@ -1500,7 +1488,7 @@ inline void bind_context_once() {
 }
 
 template <int EPI>
-int launch(Launch& L, cudaStream_t s) {
+static int launch(Launch& L, cudaStream_t s) {
   bind_context_once();
   Params& p = L.p;
   const bool pair = pair_mode() != 0 && !L.single;

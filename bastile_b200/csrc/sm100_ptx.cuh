@@ -66,11 +66,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 constexpr uint64_t kWaitLimitNs = 1000ull * 1000ull * 1000ull;  // 1 s: the default
 // The limit in force, in nanoseconds of %globaltimer (wall time: a context that is descheduled -
 // time-slicing, MPS, a debugger - keeps counting).  One copy per translation unit and device;
-// bt_set_wait_limit_ms() writes all of them on the current device.
+// bt_set_wait_limit_ms() writes all of them on the current device, and whatever refers to it in a header
+// is static: one copy per translation unit as well.
 static __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
 
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
-                                          int32_t* status, int code) {
+static __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                                 int32_t* status, int code) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   const uint64_t limit = *reinterpret_cast<volatile unsigned long long*>(&g_wait_limit_ns);
@@ -89,7 +90,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 // Host side: set this translation unit's copy of the limit on the current device.
-inline cudaError_t set_wait_limit_ns(unsigned long long ns) {
+static inline cudaError_t set_wait_limit_ns(unsigned long long ns) {
   return cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns));
 }
 

@@ -4,6 +4,26 @@
 #include "gemm_sm100.cuh"
 
 namespace bt {
+namespace gemm {
+
+static __device__ unsigned long long g_tile_sched[kSchedSlots][kSchedWords];
+
+unsigned long long* sched_pool() {
+  static std::mutex mu;
+  static unsigned long long* pools[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  std::lock_guard<std::mutex> lock(mu);
+  if (pools[dev] == nullptr) {
+    void* ptr = nullptr;
+    if (cudaGetSymbolAddress(&ptr, g_tile_sched) != cudaSuccess) return nullptr;
+    pools[dev] = static_cast<unsigned long long*>(ptr);
+  }
+  return pools[dev];
+}
+
+}  // namespace gemm
+
 namespace {
 
 using gemm::Launch;
