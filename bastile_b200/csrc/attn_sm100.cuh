@@ -227,9 +227,11 @@ __device__ __forceinline__ void mma_pb(uint32_t d, uint32_t a_lo, uint32_t a_hi,
            idesc, (accumulate || k != 0) ? 1u : 0u);
 }
 
-// Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.
+// Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.  One lane has waited for
+// the tile's copy; the others' stores are ordered behind it by the barrier of the warp.
 template <int DT>
 __device__ __forceinline__ void zero_rows(uint32_t tile, int first, int lane) {
+  __syncwarp();
 #pragma unroll
   for (int j = 0; j < DT / 64; ++j)
     for (int i = first * 8 + lane; i < 128 * 8; i += 32)
