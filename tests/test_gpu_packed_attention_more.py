@@ -106,3 +106,75 @@ def test_dense_tensors_off_a_16_byte_boundary():
     got = attend(shifted(q), shifted(k, 3), shifted(v, 4), cu, shifted(dout, 7))
     for n in got:
         assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,hq,hk,d", [
+    ([500, 0, 130, 1, 60], 64, 32, 64), ([1100, 3, 97], 80, 16, 80), ([2000, 450], 32, 8, 128), ([257, 50], 128, 64, 8),
+    ([128] * 3 + [20], 48, 48, 128), ([40] * 16, 64, 32, 72),
+])
+def test_the_kernel_of_ordinary_batches(lens, hq, hk, d, dtype):
+    """A key tile per CTA, no clusters: what dK and dV take from 128 tokens times SMs over key/value heads on."""
+    q, k, v, cu, dout = inputs(lens, hq, hk, d, dtype, seed=41, tail=5, fused=len(lens) % 2 == 0)
+    assert q.shape[0] * hk >= 128 * torch.cuda.get_device_properties(0).multi_processor_count
+    want = oracle(q, k, v, cu, d ** -0.5, dout)
+    got = attend(q, k, v, cu, dout)
+    for n in got:
+        close(got[n], want[n], n)
+        assert (got[n][cu[-1]:] == 0).all(), n
+    again = attend(q, k, v, cu, dout)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+def test_the_benchmarks_sequence():
+    q, k, v, cu, dout = inputs([8192], 32, 8, 128, torch.bfloat16, seed=42)
+    want = oracle(q, k, v, cu, 128 ** -0.5, dout)
+    got = attend(q, k, v, cu, dout)
+    for n in got:
+        close(got[n], want[n], n)
+
+
+def mean_square_errors(q, k, v, cu, scale, dout, u):
+    """Per sequence: the 2-norms that dq's and dk's errors have in the mean, {(name, start): (with D from the
+    unrounded output, with D from the rounded one)}.  Roundings are independent and at most u / sqrt(3) of their
+    value in the mean square: of dS, of the result, and of P in the sum for the output, which moves D by
+    P_ij dP_ij each; the output's own rounding moves it by dout_id out_id each."""
+    q, k, v, dout = (x.double() for x in (q, k, v, dout))
+    g, r2 = q.shape[1] // k.shape[1], u * u / 3
+    res = {}
+    for a, b in zip(cu[:-1], cu[1:]):
+        mask = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).tril()
+        sq = {(n, w): 0.0 for n in ("dq", "dk") for w in (0, 1)}
+        dk = [0.0] * k.shape[1]
+        for h in range(q.shape[1]):
+            qh, kh, vh, do = q[a:b, h], k[a:b, h // g], v[a:b, h // g], dout[a:b, h]
+            p = torch.softmax((qh @ kh.t() * scale).masked_fill(~mask, -torch.inf), -1)
+            out, dp = p @ vh, do @ vh.t()
+            ds = p * (dp - (do * out).sum(-1, keepdim=True))
+            move = r2 * (p * dp).square().sum(-1)
+            for w, d2 in enumerate((move, move + r2 * (do * out).square().sum(-1))):
+                sq["dq", w] += scale ** 2 * (r2 * (ds.square() @ kh.square()).sum() + (d2[:, None] * (p @ kh).square()).sum())
+                sq["dk", w] += scale ** 2 * (r2 * (ds.square().t() @ qh.square()).sum()
+                                             + (p.square().t() @ (d2[:, None] * qh.square())).sum())
+                sq["dq", w] += r2 * (ds @ kh * scale).square().sum()
+            dk[h // g] = dk[h // g] + ds.t() @ qh * scale
+        for n, w in sq:
+            total = sq[n, w] + (r2 * sum(x.square().sum() for x in dk) if n == "dk" else 0.0)
+            res.setdefault((n, a), []).append(float(total) ** 0.5)
+    return res
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk", [(4, 2), (1, 1)])
+def test_the_outputs_rounding_does_not_reach_the_gradients(hq, hk, dtype):
+    """Values far from zero that differ little: D = dout . out from the rounded output alone would be far off."""
+    u = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    q, k, v, cu, dout = inputs([300, 77, 128], hq, hk, 64, dtype, seed=43)
+    v = (8.0 + 0.25 * v.float()).to(dtype)
+    want = oracle(q, k, v, cu, 0.125, dout)
+    got = attend(q, k, v, cu, dout)
+    for (n, a), (unrounded, rounded) in mean_square_errors(q, k, v, cu, 0.125, dout, u).items():
+        b = cu[cu.index(a) + 1]
+        error = float((got[n][a:b].double() - want[n][0][a:b]).norm())
+        assert error <= 1.25 * unrounded, (n, a, error, unrounded, rounded)
+        assert rounded >= 1.5 * unrounded  # so that the bar tells one from the other

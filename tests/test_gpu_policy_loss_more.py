@@ -213,3 +213,30 @@ def test_a_reference_for_the_log_alone_does_not_reach_the_loss():
     assert b.kl == float("inf") and torch.equal(a.loss, b.loss)
     for p, q in zip(torch.autograd.grad(a.loss, (x, w)), torch.autograd.grad(b.loss, (x, w))):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows,h,v", [(1, 64, 8), (7, 64, 129), (300, 256, 1000), (513, 128, 4099)])
+@pytest.mark.parametrize("chunk,kl,packed", [(4096, 0.0, False), (100, 0.1, False), (128, 0.05, True)])
+def test_policy_loss_fp32(rows, h, v, chunk, kl, packed):
+    from bastile_b200 import _lib
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    x, w, t, _, g = make(rows, h, v, torch.float32, seed=rows + 5 * v)
+    cu = None
+    if packed:
+        cu = [0, 1] if rows == 1 else ([0, 3, 3, rows] if rows < 20 else [0, 10, 20, 20, rows // 2, rows - 5])
+    o = Oracle(x, w, t)
+    old, adv, ref = policy_inputs(o, g)
+    ref = ref if kl else None
+    want, want_logp, e_logp = policy_oracle(o, old, adv, ref, 0.2, 0.28, kl, cu)
+    x.requires_grad_(True), w.requires_grad_(True)
+    cut = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=DEV)
+    got = fused_linear_policy_loss(x, w, t, old, adv, ref_log_probs=ref, clip_low=0.2, clip_high=0.28, kl_coef=kl,
+                                   cu_seqlens=cut, chunk_size=chunk)
+    close(got.loss.detach(), want["loss"], want["e_loss"] + 1e-30, "loss")
+    close(got.log_probs, want_logp, e_logp, "log_probs")
+    bounds = o.grads(want["coef"], want["e_coef"], shifted=True)
+    for name, grad, like in zip(("dhidden", "dweight"), torch.autograd.grad(got.loss, (x, w)), (x, w)):
+        assert grad.dtype == like.dtype == torch.float32
+        close(grad, *bounds[name], name)
+    _lib.check_all_status()
