@@ -45,12 +45,17 @@ class _Rank(SpawnContext.Process):
         super().__init__(group, _share_by_name, name, (target, *args), **more)
 
 
+_SPAWNING = ("test_sharded_adamw_cpu", "test_gpu_sharded_adamw", "test_vocab_parallel_cpu", "test_gpu_vocab_parallel")
+
+
 @pytest.fixture(autouse=True)
-def _tensors_outlive_their_process(monkeypatch):
+def _tensors_outlive_their_process(request, monkeypatch):
     """Spawned ranks hand tensors to the test through a queue and exit.  By default the receiver fetches a
     tensor's file descriptor from its sender, which fails if that is gone by then (a rank ends a few
-    milliseconds after its ``put``); shared by name they stay until they have been received."""
-    monkeypatch.setattr(SpawnContext, "Process", _Rank)
+    milliseconds after its ``put``); shared by name they stay until they have been received.  Only for the
+    modules that spawn ranks."""
+    if request.module.__name__.endswith(_SPAWNING):
+        monkeypatch.setattr(SpawnContext, "Process", _Rank)
 
 
 def load_golden(name: str):
