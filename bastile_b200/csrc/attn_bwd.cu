@@ -149,6 +149,13 @@ __device__ __forceinline__ float ds_scale(const Params& p, float2* place) {
     return most > 0.f ? ldexpf(1.f, min(15 - e, 60)) : 1.f;
   }
 }
+// fp16: P^T, at most 1, is the operand of dV as 2^15 P^T, for the probabilities of long rows and of keys that
+// are hardly seen (2^-14 is the smallest that fp16 holds at full precision).  The power goes into the
+// exponent, and out of dV and of the scale of dS.
+template <typename T>
+constexpr float kPUp = kScaled<T> ? 15.f : 0.f;
+template <typename T>
+constexpr float kPDown = kScaled<T> ? 1.f / 32768.f : 1.f;
 // 2^k (dP - D), D scaled before
 template <typename T>
 __device__ __forceinline__ f32x2 minus_d(f32x2 dp, f32x2 scale, f32x2 minus_scaled_d) {
@@ -247,8 +254,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
-  const float up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
-  const float dk_scale = p.scale / up;
+  const float ds_up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
+  const float dk_scale = p.scale / ds_up;
+  const float up = ds_up * kPDown<T>;
 
   const bool shared_tiles = PAIR && p.plan.area() < p.share * static_cast<float>(p.plan.longest());
   const int unit = static_cast<int>(shared_tiles ? blockIdx.x / 2 : blockIdx.x);
@@ -299,7 +307,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           const int token = it.start + tok0 + (r >> p.gp_shift);
           const int64_t at = static_cast<int64_t>(head + (r & (p.gp - 1))) * p.total + token;
           const bool in = r < valid;
-          vec[st * 256 + r] = in ? -__ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
+          vec[st * 256 + r] = in ? kPUp<T> - __ldg(p.lse2 + at) : -INFINITY;  // no row: P = 0
           vec[st * 256 + 128 + r] = in ? -__ldg(p.delta + at) * up : 0.f;
         }
         ptx::mbar_arrive(&vec_full[st]);
@@ -493,15 +501,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (ok)
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)
-            store_sum_cols<T>(mine + c, sQ + (c / 4 * 128 + row) * 16, dst, c, p.d, rank != 0 ? dk_scale : 1.0f,
-                              row_ok);
+            store_sum_cols<T>(mine + c, sQ + (c / 4 * 128 + row) * 16, dst, c, p.d,
+                              rank != 0 ? dk_scale : kPDown<T>, row_ok);
       } else if (ok) {
         T* dk = static_cast<T*>(p.dk.ptr) + token * p.dk.st + hk * p.dk.sh;
         T* dv = static_cast<T*>(p.dv.ptr) + token * p.dv.st + hk * p.dv.sh;
         // (one store per tile and output here: a staged tile store measured 1% slower)
 #pragma unroll 1
         for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32) {
-          store_cols<T>(tmem + lane_base + 256 + c, dv, nullptr, c, p.d, 1.0f, row_ok);
+          store_cols<T>(tmem + lane_base + 256 + c, dv, nullptr, c, p.d, kPDown<T>, row_ok);
           store_cols<T>(tmem + lane_base + 256 + DT + c, dk, nullptr, c, p.d, dk_scale, row_ok);
         }
       }

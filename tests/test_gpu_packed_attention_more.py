@@ -178,3 +178,24 @@ def test_the_outputs_rounding_does_not_reach_the_gradients(hq, hk, dtype):
         error = float((got[n][a:b].double() - want[n][0][a:b]).norm())
         assert error <= 1.25 * unrounded, (n, a, error, unrounded, rounded)
         assert rounded >= 1.5 * unrounded  # so that the bar tells one from the other
+
+
+@pytest.mark.parametrize("lens,hq,hk", [([600], 2, 1), ([600, 40], 64, 32)])
+def test_fp16_keys_that_are_hardly_seen(lens, hq, hk):
+    """The first key takes all but a millionth of every row: what dV of the others is formed from lies below fp16's
+    normal range.  P and the result are rounded once each."""
+    q, k, v, cu, dout = inputs(lens, hq, hk, 64, torch.float16, seed=44)
+    dout = dout * 256.0
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    for a in cu[:-1]:
+        k[a, :, 0] = 8.0 * 15.0 / 4.0  # 15 above the others' scores: e^-15 = 2^-21.6
+    want = oracle(q, k, v, cu, 0.125, dout)
+    got = attend(q, k, v, cu, dout)
+    bar = 1.25 * (2 * (2.0 ** -11) ** 2 / 3) ** 0.5
+    others = torch.ones(cu[-1], dtype=torch.bool, device=DEV)
+    others[cu[:-1]] = False
+    x, y = got["dv"][others], want["dv"][0][others]
+    own = 2.0 ** -24 / 12 ** 0.5 / float(y.square().mean().sqrt())
+    assert off(x, y) <= bar + own, (off(x, y), bar, own)
+    for n in got:
+        close(got[n], want[n], n)
