@@ -199,3 +199,53 @@ def test_fp16_keys_that_are_hardly_seen(lens, hq, hk):
     assert off(x, y) <= bar + own, (off(x, y), bar, own)
     for n in got:
         close(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_two_captured_graphs_share_a_plan_and_replay_at_once(dtype):
+    """A plan made outside the graphs, two graphs of a step each on two streams, replayed together."""
+    from bastile_b200.ops.packed_attention import pack_sequences, packed_attention
+
+    q, k, v, cu, dout = inputs([200, 101], 4, 2, 64, dtype, seed=45)
+    sets = [(q, k, v, dout), (q * 0.5, k, v * 2.0, dout * 0.25)]
+    want = [attend(*s[:3], cu, s[3]) for s in sets]
+    seqs = pack_sequences(torch.tensor(cu, dtype=torch.int32, device=DEV), 301)
+    graphs, results = [], []
+    for a, b, c, g in sets:
+        xs = [x.clone().requires_grad_(True) for x in (a, b, c)]
+
+        def step():
+            out = packed_attention(*xs, seqs)
+            return (out.detach(), *torch.autograd.grad(out, xs, g))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(step())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, w in zip(results, want):
+        for n, x in zip(("out", "dq", "dk", "dv"), got):
+            assert torch.equal(x, w[n]), n
+
+
+def test_two_backward_passes_of_one_graph():
+    from bastile_b200.ops.packed_attention import pack_sequences, packed_attention
+
+    q, k, v, cu, dout = inputs([90, 40], 4, 2, 64, torch.float16, seed=46)
+    xs = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = packed_attention(*xs, pack_sequences(torch.tensor(cu, dtype=torch.int32, device=DEV), 130))
+    for factor in (1.0, 2.0 ** -9, 16.0):  # another upstream gradient, another scale of dS
+        want = attend(q, k, v, cu, dout * factor)
+        for n, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, xs, dout * factor, retain_graph=True)):
+            assert torch.equal(x, want[n]), n

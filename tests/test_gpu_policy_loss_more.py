@@ -240,3 +240,34 @@ def test_policy_loss_fp32(rows, h, v, chunk, kl, packed):
         assert grad.dtype == like.dtype == torch.float32
         close(grad, *bounds[name], name)
     _lib.check_all_status()
+
+
+def test_captured_fp16_steps_start_from_their_own_exponents():
+    """Chunks hand the greatest exponent on; a replay begins anew, with other advantages too."""
+    from bastile_b200.ops.fused_linear_policy_loss import fused_linear_policy_loss
+
+    x, w, t, _, g = make(150, 64, 600, torch.float16, seed=29)
+    o = Oracle(x, w, t)
+    old, adv, _ = policy_inputs(o, g)
+    x.requires_grad_(True)
+    w32 = w.float().requires_grad_(True)
+
+    def step():
+        return torch.autograd.grad(fused_linear_policy_loss(x, w32, t, old, adv, chunk_size=40).loss, (x, w32))
+
+    plain = (old.clone(), adv.clone())
+    huge = (old.clone(), adv.clone())
+    huge[0][50], huge[1][50] = o.logp[50] - 14.0, -1.0
+    want = {}
+    for name, (ol, ad) in (("plain", plain), ("huge", huge)):
+        old.copy_(ol), adv.copy_(ad)
+        want[name] = step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for name, (ol, ad) in (("plain", plain), ("huge", huge), ("plain", plain)):
+        old.copy_(ol), adv.copy_(ad)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(res, want[name]):
+            assert torch.equal(a, b), name
