@@ -738,14 +738,15 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
     BT_CHECK_ARG(d->labels && d->old_logp && d->adv && d->logp, "policy_fwd: null pointer");
     BT_CHECK_ARG(!grad || (d->masked && d->logits && aligned16(d->masked) && aligned16(d->logits)),
                  "policy_fwd: gradients need 16-byte aligned buffers for the counted rows and the logits");
-    BT_CHECK_ARG(!d->want_dweight || d->rows <= d->chunk || d->dweight_acc != nullptr,
-                 "policy_fwd: more than one chunk needs an accumulator for the weight gradient");
+    BT_CHECK_ARG(!d->want_dweight || d->rows <= d->chunk || (d->dweight_acc != nullptr && aligned16(d->dweight_acc)),
+                 "policy_fwd: more than one chunk needs a 16-byte aligned accumulator for the weight gradient");
   }
   const int runs = d->rows > 0 ? dhidden_runs(d->chunk < d->rows ? d->chunk : d->rows, d->H, d->V, d->dtype) : 1;
   // one chunk: its runs are added up when the upstream gradient is known; more: each before the next
   const bool sum_now = d->rows > d->chunk && runs > 1;
-  BT_CHECK_ARG(d->dhidden == nullptr || !sum_now || (d->dhidden_parts != nullptr && aligned16(d->dhidden_parts)),
-               "policy_fwd: more than one chunk needs a 16-byte aligned buffer for the parts of the gradient of hidden");
+  BT_CHECK_ARG(d->dhidden == nullptr || !sum_now ||
+                   (d->dhidden_parts != nullptr && aligned16(d->dhidden_parts) && aligned16(d->dhidden)),
+               "policy_fwd: more than one chunk needs 16-byte aligned buffers for the gradient of hidden and its parts");
   float* scal = d->averages + 2;
   // E after chunk k is word k % 3: the one before it is still needed beside it, and the next is prepared
   int32_t* top_exp = reinterpret_cast<int32_t*>(d->averages + 5);
