@@ -255,7 +255,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   grid_dependency_wait();
 
   const float ds_up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
-  const float dk_scale = p.scale / ds_up;
+  const float dk_scale = kScaled<T> ? p.scale / ds_up : p.scale;
   const float up = ds_up * kPDown<T>;
 
   const bool shared_tiles = PAIR && p.plan.area() < p.share * static_cast<float>(p.plan.longest());
@@ -592,7 +592,6 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   grid_dependency_wait();
 
   const float up = ds_scale<T>(p, reinterpret_cast<float2*>(smem + 7 * TB + G::kVecBytes + 256));
-  const float dq_scale = p.scale / up;
 
   const int groups = p.hk * p.nsub;
   const int hs = static_cast<int>(blockIdx.x) % groups;
@@ -769,6 +768,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       if (ok) {
         ptx::tcgen05_fence_after_sync();
         const uint32_t ta = tmem + lane_base + 384;
+        const float dq_scale = kScaled<T> ? p.scale / up : p.scale;  // (only here: 1% of the time before the loop)
         if (first + p.tq <= it.len) {  // into Q's place
 #pragma unroll 1
           for (int c = half * (DT / 2); c < (half + 1) * (DT / 2); c += 32)

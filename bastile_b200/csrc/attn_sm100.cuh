@@ -227,11 +227,9 @@ __device__ __forceinline__ void mma_pb(uint32_t d, uint32_t a_lo, uint32_t a_hi,
            idesc, (accumulate || k != 0) ? 1u : 0u);
 }
 
-// Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.  One lane has waited for
-// the tile's copy; the others' stores are ordered behind it by the barrier of the warp.
+// Zero rows [first, 128) of an operand tile (one warp), before the MMA reads them.
 template <int DT>
 __device__ __forceinline__ void zero_rows(uint32_t tile, int first, int lane) {
-  __syncwarp();
 #pragma unroll
   for (int j = 0; j < DT / 64; ++j)
     for (int i = first * 8 + lane; i < 128 * 8; i += 32)
@@ -268,11 +266,13 @@ static __device__ __forceinline__ bool ring_load(uint32_t dst, const CUtensorMap
       uint64_t* bar = ragged ? fix : full;
       ptx::mbar_arrive_expect_tx(bar, (DT / 64) * kBoxBytes);
       load_tile<DT>(dst, tm, head, token, bar);
-      if (ragged) ok = ptx::mbar_wait(fix, *fix_phase, cta_abort, status, ST_LOAD);
     }
   }
   ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
   if (ok && ragged) {
+    // every lane waits for the copy itself: its stores to the tile have to come after it
+    ok = warp_wait(fix, *fix_phase, cta_abort, status, ST_LOAD);
+    if (!ok) return false;
     *fix_phase ^= 1u;
     zero_rows<DT>(dst, valid, lane);
     if (lane == 0) ptx::mbar_arrive(full);
