@@ -885,6 +885,9 @@ extern "C" int bt_attn_bwd(const void* dout, const void* q, const void* k, const
   BT_CHECK_ARG(aligned16(out_lo), "attn_bwd out_lo: must be 16-byte aligned");
   BT_CHECK_ARG(reinterpret_cast<uintptr_t>(delta) % 8 == 0, "attn_bwd delta: must be 8-byte aligned");
   BT_CHECK_ARG((dk == nullptr) == (dv == nullptr), "attn_bwd: dk and dv are computed together");
+  BT_CHECK_ARG(g_strides && q_strides && k_strides && v_strides && o_strides && (dq == nullptr || dq_strides) &&
+                   (dk == nullptr || (dk_strides && dv_strides)),
+               "attn_bwd: null strides");
   if (int rc = check_view("attn_bwd dout", dout, g_strides[0], g_strides[1], nq, total)) return rc;
   if (int rc = check_view("attn_bwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
   if (int rc = check_view("attn_bwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;

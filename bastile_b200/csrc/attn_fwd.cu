@@ -465,6 +465,7 @@ extern "C" int bt_attn_fwd(const void* q, const void* k, const void* v, void* ou
   Params p{};
   if (int rc = fill_params(&p, "attn_fwd", plan, batch, total, hq, hk, d, scale, dtype)) return rc;
   const int nq = static_cast<int>(hq), nk = static_cast<int>(hk), nd = static_cast<int>(d);
+  BT_CHECK_ARG(q_strides && k_strides && v_strides && o_strides, "attn_fwd: null strides");
   if (int rc = check_view("attn_fwd q", q, q_strides[0], q_strides[1], nq, total)) return rc;
   if (int rc = check_view("attn_fwd k", k, k_strides[0], k_strides[1], nk, total)) return rc;
   if (int rc = check_view("attn_fwd v", v, v_strides[0], v_strides[1], nk, total)) return rc;

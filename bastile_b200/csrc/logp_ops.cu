@@ -17,6 +17,7 @@ constexpr int kThreads = 256;
 bool rows_aligned(const void* p, int64_t ld, int elem_bytes) {
   return p != nullptr && aligned16(p) && (ld * elem_bytes) % 16 == 0;
 }
+bool aligned8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }  // statistics are pairs of floats
 bool known(int dtype) { return dtype == BT_BF16 || dtype == BT_FP16 || dtype == BT_FP32; }
 int esize(int dtype) { return dtype == BT_FP32 ? 4 : 2; }
 __device__ __forceinline__ bool counted(int64_t label, int64_t ignore_index, int64_t vocab) {
@@ -632,6 +633,7 @@ extern "C" int bt_logp_fwd(const void* hidden, const void* W, const int64_t* lab
     return rc;
   if (rows == 0) return BT_OK;
   BT_CHECK_ARG(labels && logp && ws, "logp_fwd: null pointer");
+  BT_CHECK_ARG(aligned8(ws), "logp_fwd: ws must be 8-byte aligned");
   float* tile_stats = ws;
   float* tgt = ws + chunk * h.n_vt * 2;
   for (int64_t r = 0; r < rows; r += chunk) {
@@ -733,6 +735,7 @@ extern "C" int bt_policy_fwd(const bt_policy_desc* d, int32_t* status, void* str
   BT_CHECK_ARG(d->n_seq >= 0 && d->n_seq < (1 << 24) && (d->cu_seqlens != nullptr || d->n_seq == 1),
                "policy_fwd: bad sequence count");
   BT_CHECK_ARG(d->ws && d->loss && d->averages, "policy_fwd: null pointer");
+  BT_CHECK_ARG(aligned8(d->ws), "policy_fwd: ws must be 8-byte aligned");
   const bool grad = d->dhidden != nullptr || d->want_dweight != 0;
   if (d->rows > 0) {
     BT_CHECK_ARG(d->labels && d->old_logp && d->adv && d->logp, "policy_fwd: null pointer");

@@ -491,7 +491,7 @@ int bt_attn_bwd(const void* dout, const void* q, const void* k, const void* v, c
  * [min(chunk, rows), (V + 7) / 8 * 8] in `dtype`.  `masked` is [rows, H] scratch in `dtype`.
  *
  * bt_logp_fwd: logp[rows] fp32 (0 where a position does not count) and, unless NULL, lse[rows], from the
- * fp32 accumulators of the logits product; ws: bt_logp_fwd_ws_floats(chunk, V) floats. */
+ * fp32 accumulators of the logits product; ws: bt_logp_fwd_ws_floats(chunk, V) floats, 8-byte aligned. */
 int64_t bt_logp_fwd_ws_floats(int64_t chunk, int64_t V);
 int bt_logp_fwd(const void* hidden, const void* W, const int64_t* labels, float* logp, float* lse, float* ws,
                 int64_t rows, int64_t H, int64_t V, int64_t ld_hidden, int64_t chunk, int64_t ignore_index, int dtype,
@@ -520,7 +520,7 @@ int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int
  * rows of hidden in `masked`) to averages[4]: the caller multiplies by it and the upstream gradient.  The two
  * differ with fp16 alone, where dlogits of coefficients outside [2^-8, 2^15) are stored scaled.
  * masked, logits: needed with either gradient.
- * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats. */
+ * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats, 8-byte aligned. */
 typedef struct {
   const void* hidden;
   const void* W;

@@ -44,3 +44,29 @@ def test_c_sizes_of_attention_scratch():
     lib = _lib.get_lib()
     assert lib.bt_attn_delta_floats(7, 3, _lib.BT_BF16) == 21
     assert lib.bt_attn_delta_floats(7, 3, _lib.BT_FP16) >= 22 + 2 * 148 and lib.bt_attn_delta_floats(-1, 3, 0) == 0
+
+
+def test_c_entry_points_refuse_unaligned_statistics_and_missing_strides():
+    import ctypes as C
+
+    from bastile_b200 import _lib
+
+    lib = _lib.get_lib()
+    one, odd, b = C.c_void_p(16), C.c_void_p(20), _lib.BT_BF16  # never dereferenced
+
+    rc = lib.bt_logp_fwd(one, one, one, one, None, odd, 4, 64, 100, 64, 4, -100, b, None, None)
+    assert rc == -1 and b"8-byte" in lib.bt_last_error()
+    d = _lib.PolicyDesc()
+    for n, t in d._fields_:
+        if t is C.c_void_p and n not in ("cu_seqlens", "ref_logp"):
+            setattr(d, n, 16)
+    d.rows, d.H, d.V, d.ld_hidden, d.chunk, d.n_seq, d.ignore_index, d.dtype, d.ws = 4, 64, 100, 64, 4, 1, -100, b, 20
+    assert lib.bt_policy_fwd(C.byref(d), None, None) == -1 and b"8-byte" in lib.bt_last_error()
+    st = _lib.I64x2(256, 64)
+    rc = lib.bt_attn_fwd(one, one, one, one, None, None, one, 1, 4, 4, 2, 64, st, st, None, st, 0.1, b, None, None)
+    assert rc == -1 and b"strides" in lib.bt_last_error()
+    for missing in range(8):
+        s = [st] * 8
+        s[missing] = None
+        rc = lib.bt_attn_bwd(one, one, one, one, one, None, one, one, one, one, one, one, 1, 4, 4, 2, 64, *s, 0.1, b, None, None)
+        assert rc == -1 and b"strides" in lib.bt_last_error(), missing
