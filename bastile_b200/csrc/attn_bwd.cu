@@ -8,10 +8,13 @@
 // dQ per query tile.  S and dO V^T are computed by both - seven products where one kernel could do
 // with five - but that one would have to add dQ tiles into memory by atomics, whose order changes
 // the result; here every launch gives the same bits.
-// Measured, 8192 tokens in one sequence, 32 / 8 heads of 128, bf16: dK and dV 783 us, dQ 593 us, which is
-// 1.40 and 1.39 PFLOP/s of the products that they execute (a library product of this length runs at 1.41:
-// the chip's power limit, at 1.4 - 1.5 GHz); D = dO . O 34 us.  At 4096 tokens the matrix pipe is busy in 63%
-// and 60% of the cycles, the exponentials' in 36% and 42%.
+// P and dS are rounded to 16 bits, the operands' type (fp16: scaled by powers of two, see ds_scale and kPUp):
+// gradients are off by 2.4e-3 of their 2-norm with bf16 and 3.0e-4 with fp16, of which the rounding of the
+// results is 1.7e-3 and 2.1e-4.
+// Measured, 8192 tokens in one sequence, 32 / 8 heads of 128, bf16: dK and dV 777 us, dQ 591 us, which is
+// 1.41 and 1.39 PFLOP/s of the products that they execute (a library product of this length runs at 1.41:
+// the chip's power limit, at 1.4 - 1.5 GHz); D = dO . O 35 us.  fp16: 808, 623 and 41 us (max|V| is read too).
+// At 4096 tokens the matrix pipe is busy in 66% and 60% of the cycles, the exponentials' in 36% and 42%.
 #include "attn_sm100.cuh"
 
 namespace bt {
@@ -127,7 +130,8 @@ attn_delta_kernel(const T* __restrict__ out, const T* __restrict__ out_lo, const
   }
 }
 
-// 2^k of dS, the same in every CTA; `place` has room for a float2 per warp.
+// 2^k of dS, the same in every CTA; `place` has room for a float2 per warp.  About 1000 values from L2 before
+// a CTA's first load: 0.4 - 0.6 us of 12 - 22 in dQ and dK/dV of 64 short sequences (fp16 alone).
 template <typename T>
 __device__ __forceinline__ float ds_scale(const Params& p, float2* place) {
   if constexpr (!kScaled<T>) {

@@ -83,6 +83,7 @@ logp_rows_kernel(const float2* __restrict__ tile_stats, const float* __restrict_
 // therefore formed from coef 2^-e, which does not; the product with W gives that row's d hidden 2^e times
 // in its fp32 epilogue, and the one with x takes the row of x times 2^(e - E), E the greatest e so far,
 // so that d weight comes out in units of 2^E.  Powers of two: rows inside the interval keep their bits.
+// (No measurable time: 4096 rows x 4096 against 151936 12.8 ms with and without it, two chunks of 8192 55 - 56.)
 __device__ __forceinline__ int row_exponent(double coef) {
   if (coef == 0.0 || !isfinite(coef)) return 0;
   int e;
