@@ -79,18 +79,21 @@ logp_rows_kernel(const float2* __restrict__ tile_stats, const float* __restrict_
 }
 
 // fp16 holds dlogits = coef (onehot - softmax) between 2^-24 and 65504 only, while a coefficient may be
-// anything: ratios and KL gaps are exponentials.  A row whose coefficient lies outside [2^-8, 2^15) is
+// anything: ratios and KL gaps are exponentials.  A row whose coefficient lies outside [1/2, 2^15) is
 // therefore formed from coef 2^-e, which does not; the product with W gives that row's d hidden 2^e times
-// in its fp32 epilogue, and the one with x takes the row of x times 2^(e - E), E the greatest e so far,
-// so that d weight comes out in units of 2^E.  Powers of two: rows inside the interval keep their bits.
-// (No measurable time: 4096 rows x 4096 against 151936 12.8 ms with and without it, two chunks of 8192 55 - 56.)
+// in its fp32 epilogue, and the one with x takes the row of x times 2^(e - E), E not below any e so far,
+// so that d weight comes out in units of 2^E.  What the row of x loses in fp16's subnormal steps, 2^-25
+// 2^(E - e), is 2^-25 of what the largest rows contribute.  (All rows at [2^14, 2^15) would round the softmax at
+// full precision down to 2^-28 instead of 2^-13, and cost 5% at 4096 and 16384 rows: digits cost power.)
 __device__ __forceinline__ int row_exponent(double coef) {
   if (coef == 0.0 || !isfinite(coef)) return 0;
   int e;
   frexp(coef, &e);
-  e = e > 15 ? e - 15 : (e < -7 ? e + 7 : 0);
+  e = e > 15 ? e - 15 : min(e, 0);
   return max(-60, min(100, e));
 }
+// E goes up in steps of four, so that it seldom does from one chunk to the next.
+__device__ __forceinline__ int step_of(int e) { return (e + 3) & ~3; }
 constexpr int kNoExponent = -1000;  // E before the first coefficient
 
 // Upstream gradient of the log-probabilities as the coefficients of the dlogits product, scaled by a
@@ -283,7 +286,7 @@ policy_rows_kernel(const PolicyArgs a) {
     coef = coef * w * static_cast<double>(a.scal[1]);
     if (a.row_scale != nullptr) {
       const int e = row_exponent(coef);
-      if (coef != 0.0) atomicMax(a.top_exp, e);
+      if (coef != 0.0) atomicMax(a.top_exp, step_of(e));
       coef = ldexp(coef, -e);
       a.row_scale[row] = ldexpf(1.f, e);
     }
@@ -321,7 +324,7 @@ policy_reduce_kernel(const float* __restrict__ terms, int64_t n, float* __restri
 // per thread and step.  exp(logit - lse) = exp(stored) exp(half-tile max - lse), the second factor
 // once per vector.  Bound by memory: 1024 rows x 151936, 622 MB in 106 us, 5.9 TB/s; kept out of the products'
 // epilogues because a row's lse needs all of its tiles.  fp16: also brings the rows of x to the common
-// 2^E (rows inside the interval of row_exponent are left alone while E is 0), and hands E to the next chunk.
+// 2^E, and hands E to the next chunk.
 struct Exponents {
   const float* row_scale;  // null: no fp16 gradients
   const int32_t* top;

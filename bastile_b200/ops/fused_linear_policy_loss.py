@@ -241,28 +241,27 @@ class LinearPolicyLossFunction(torch.autograd.Function):
         dev = w.device
         vocab, hdim = w.shape
         stream, code = _lib.stream_ptr(dev), _lib.dtype_code(x_dtype)
-        # the coefficients were stored relative to the largest token weight
-        alpha = dloss.detach().to(torch.float32) * averages[2]
+        # the coefficients were stored relative to the largest token weight; fp16 has a scale of its own for d weight
+        alphas = dloss.detach().to(torch.float32) * averages[2:5:2]
+        alpha_x, alpha_w = alphas.data_ptr(), alphas.data_ptr() + 4
         dx_out = dw = None
         with _lib.device_of(dev), _lib.timed("policy_bwd", int(need_x) + int(need_w and x_last is not None), dev):
             if need_x:
                 dx_out = torch.empty(shape, dtype=x_dtype, device=dev)
                 n = dx_out.numel()
-                _lib.check(lib.bt_sum_runs(dx.data_ptr(), dx_out.data_ptr(), n, dx.shape[0], n, alpha.data_ptr(), code,
+                _lib.check(lib.bt_sum_runs(dx.data_ptr(), dx_out.data_ptr(), n, dx.shape[0], n, alpha_x, code,
                                            stream), "bt_sum_runs(dhidden)")
             if need_w:
                 dw = _dweight_out(w, w_dtype)
                 if x_last is None:
                     dw.zero_()
                 else:
-                    # dW = alpha (dlogits^T x + the other chunks); fp16 has a scale of its own for it
-                    if x_dtype == torch.float16:
-                        alpha = dloss.detach().to(torch.float32) * averages[4]
+                    # dW = alpha (dlogits^T x + the other chunks)
                     st = _lib.status_word(dev)
                     _lib.check(lib.bt_gemm(dlogits.data_ptr(), x_last.data_ptr(), dw.data_ptr(), vocab, hdim,
                                            x_last.shape[0], dlogits.shape[1], hdim, hdim, 0, 0, code,
                                            _lib.dtype_code(dw.dtype), acc.data_ptr() if acc is not None else None,
-                                           hdim, alpha.data_ptr(), st.data_ptr(), stream), "bt_gemm(dweight)")
+                                           hdim, alpha_w, st.data_ptr(), stream), "bt_gemm(dweight)")
                 dw = dw.to(w_dtype)
         return (dx_out, dw, *none)
 
@@ -293,7 +292,7 @@ def fused_linear_policy_loss(hidden_states: Tensor, weight: Tensor, target: Tens
     without a counted token are left out, tokens behind the last sequence count as ignored.
     ``old_log_probs``, ``advantages`` and ``ref_log_probs`` have the target's shape and get no gradients.
     Gradients of logits are formed in the hidden states' type relative to the largest token weight (with
-    fp16, rows of very large or small coefficients are formed scaled by a power of two)."""
+    fp16, rows of very large or small coefficients scaled by a power of two)."""
     what = "fused_linear_policy_loss"
     for name, t in (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs)):
         if t is None and name == "ref_log_probs":

@@ -518,7 +518,7 @@ int bt_logp_bwd(const float* dlogp, const void* hidden, const void* W, const int
  * with dhidden_parts [runs, chunk, H] as scratch unless runs is 1.  It is relative to averages[2], the weight gradient
  * (want_dweight; dweight_acc [V, H] fp32 over all chunks but the last, whose dlogits stay in `logits` and whose
  * rows of hidden in `masked`) to averages[4]: the caller multiplies by it and the upstream gradient.  The two
- * differ with fp16 alone, where dlogits of coefficients outside [2^-8, 2^15) are stored scaled.
+ * differ with fp16 alone, where rows of dlogits with coefficients outside [1/2, 2^15) are stored scaled.
  * masked, logits: needed with either gradient.
  * ws: bt_policy_fwd_ws_floats(rows, chunk, n_seq, V) floats, 8-byte aligned. */
 typedef struct {
